@@ -317,6 +317,33 @@ int exl3b_unpack_states(const int16_t* dTrellis, int ntiles, int K,
 int exl3b_decode_trellis(const int16_t* dTrellis, int tk, int tn, int K, int code,
                          float* dW, void* stream);
 
+/* ===================================================================
+ * Forward operators on finished EXL3 tensors.  Asynchronous on `stream`;
+ * inference only (the weights are integers, there is no gradient).
+ * =================================================================== */
+
+/* Linear layer with its epilogue:
+ *   out = act(x . W + bias) * mul + residual
+ *   W [k][n] = diag(suh) B W_inner B diag(svh) (from_inner, quantize.py:158-164)
+ *         of an EXL3 tensor as stored: dTrellis int16 [k/16][n/16][16 K]
+ *         (16-byte aligned), suh fp16 [k] with the tensor's scale folded in
+ *         and svh fp16 [n] (8-byte aligned); k and n multiples of 128
+ *   x [M][k], mul, residual and out [M][n], bias [n]: dtype 1 = bf16 or
+ *         2 = fp16, 8-byte aligned, row pitches ld* in elements (>= the row,
+ *         multiples of 4); bias, mul and residual may be NULL.  out may be
+ *         the same rows as mul or residual, and must not overlap x
+ *   act   0 none, 1 relu, 2 silu, 3 gelu (erf), 4 gelu (tanh form)
+ * fp32 accumulation; one rounding to dtype at the end.  ws:
+ * exl3b_linear_workspace_bytes(M, k, n) bytes, 256-byte aligned (NULL when
+ * that is 0), in use until the work queued on `stream` has run. */
+size_t exl3b_linear_workspace_bytes(int M, int k, int n);
+int exl3b_linear(const void* dX, int dtype, int64_t ldx, int M, int k, int n,
+                 const int16_t* dTrellis, int K, int code, const void* d_suh_f16,
+                 const void* d_svh_f16, const void* d_bias, int act,
+                 const void* d_mul, int64_t ldmul, const void* d_residual,
+                 int64_t ldres, void* dOut, int64_t ldo, void* ws, size_t ws_bytes,
+                 void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,118 @@
+"""CPU-side checks of the forward operators: the C ABI refuses bad requests before it
+touches a device, and the Python wrappers refuse what the kernels do not take."""
+import ctypes
+
+import pytest
+import torch
+
+P = 0x7F0000001000          # an aligned address that is never dereferenced
+
+
+def _linear(**kw):
+    from exl3b import native
+    a = dict(x=P, dtype=1, ldx=256, M=4, k=256, n=128, tr=P, K=4, code=0, suh=P, svh=P, bias=None,
+             act=0, mul=None, ldmul=0, res=None, ldres=0, out=P, ldo=128, ws=None, wsb=0)
+    a.update(kw)
+    rc = native.lib().exl3b_linear(*a.values(), None)
+    return rc, native.last_error()
+
+
+@pytest.mark.parametrize("kw,rc,msg", [
+    (dict(K=1), 8, "K=1"), (dict(K=8), 8, "K=8"),
+    (dict(code=3), 7, "code 3"), (dict(code=-1), 7, "code -1"),
+    (dict(dtype=0), 7, "dtype 0"), (dict(dtype=3), 7, "dtype 3"),
+    (dict(act=5), 7, "activation 5"), (dict(act=-1), 7, "activation -1"),
+    (dict(M=-1), 7, "multiples of 128"), (dict(k=192, ldx=192), 7, "multiples of 128"),
+    (dict(n=64), 7, "multiples of 128"), (dict(k=0), 7, "multiples of 128"),
+    (dict(tr=None), 7, "aligned"), (dict(tr=P + 8), 7, "aligned"),
+    (dict(suh=P + 4), 7, "aligned"), (dict(svh=None), 7, "aligned"),
+    (dict(bias=P + 2), 7, "aligned"),
+    (dict(x=None), 7, "x:"), (dict(x=P + 4), 7, "x:"), (dict(ldx=252), 7, "x:"),
+    (dict(ldx=258), 7, "x:"), (dict(out=P + 2), 7, "out:"), (dict(ldo=127), 7, "out:"),
+    (dict(mul=P, ldmul=64), 7, "mul:"), (dict(mul=P + 4, ldmul=128), 7, "mul:"),
+    (dict(res=P, ldres=130), 7, "residual:"),
+])
+def test_linear_abi_refuses(kw, rc, msg):
+    got, text = _linear(**kw)
+    assert got == rc and msg in text, (got, text)
+
+
+def test_linear_abi_empty_is_ok():
+    assert _linear(M=0, x=None, out=None)[0] == 0
+
+
+def test_weight_refuses():
+    from exl3b import forward
+    tr = torch.zeros(8, 8, 64, dtype=torch.int16)
+    s = torch.ones(128).half()
+    for args, msg in [((tr, s, s, 1), "K=1"), ((tr, s, s, 8), "K=8"),
+                      ((tr, s, s, 5), "int16"), ((tr.int(), s, s, 4), "int16"),
+                      ((tr[0], s, s, 4), "int16"), ((tr[:4], s[:64], s, 4), "multiples of 128"),
+                      ((tr[:0], s[:0], s, 4), "multiples of 128"),
+                      ((tr, s[:64], s, 4), "suh"), ((tr, s, s[:64], 4), "svh"),
+                      ((tr, s, s, 4), "CUDA device"), ((tr, s, s, 4, "qtip"), "qtip")]:
+        with pytest.raises(ValueError, match=msg):
+            forward.TrellisWeight(*args)
+
+
+class _Weight:
+    """Stands for a weight where a call must be refused before any kernel."""
+    k, n, K, code_id = 256, 128, 4, 0
+    device = torch.device("cpu")
+
+
+def test_linear_refuses():
+    from exl3b import forward
+    w = _Weight()
+    x = torch.zeros(3, 256, dtype=torch.bfloat16)
+    y = torch.zeros(3, 128, dtype=torch.bfloat16)
+    big = torch.zeros(3, 512, dtype=torch.bfloat16)
+    cases = [
+        (dict(x=x.float()), "bf16 or fp16"), (dict(x=x[:, :128]), "in = 256"),
+        (dict(activation="swish"), "activation"), (dict(bias=y[0].half()), "bias"),
+        (dict(bias=y[0, :64]), "bias"), (dict(mul=y[:1]), "mul"),
+        (dict(residual=y.half()), "residual"), (dict(residual=y[:, :64]), "residual"),
+        (dict(out=y[:2]), "out"), (dict(out=y.half()), "out"),
+        (dict(out=torch.zeros(128, 3, dtype=torch.bfloat16).t()), "out"),
+        (dict(x=x.clone().requires_grad_()), "gradient"),
+        (dict(residual=y.clone().requires_grad_()), "gradient"),
+        # out inside x; out shifted against the residual
+        (dict(x=big[:, :256], out=big[:, 128:256]), "overlaps x"),
+        (dict(residual=big[:, :128], out=big[:, 64:192]), "overlaps an input"),
+    ]
+    for kw, msg in cases:
+        with pytest.raises(ValueError, match=msg):
+            forward.linear(kw.pop("x", x), w, **kw)
+
+
+def test_overlap_rule():
+    from exl3b.forward import _overlap
+    buf = torch.zeros(4, 64, dtype=torch.float16)
+    assert _overlap(buf[:, :32], buf[:, 16:48])
+    assert not _overlap(buf[:, :32], buf[:, 32:])       # interleaved columns
+    assert not _overlap(buf[:, 32:], buf[:, :32])
+    assert not _overlap(buf[:2], buf[2:])
+    assert _overlap(buf[:3], buf[2:])
+    assert _overlap(buf, buf)
+    assert not _overlap(buf[:0], buf)
+
+
+def test_load_reads_what_the_writer_stores(tmp_path, monkeypatch):
+    """TrellisWeight.load and from_result hold the same fields as the files."""
+    from exl3b import export, forward
+    g = torch.Generator().manual_seed(0)
+    result = {"trellis": torch.randint(-32768, 32768, (8, 16, 80), generator=g, dtype=torch.int16),
+              "suh": torch.sign(torch.randn(128, generator=g)).half(),
+              "svh": torch.sign(torch.randn(256, generator=g)).half(),
+              "Wscale": 0.0173, "K": 5, "code": "exl3_mcg", "channel_scales": False}
+    path = export.save_quantized(tmp_path, 3, "mlp.up_proj", result)
+    seen = []
+    monkeypatch.setattr(forward.TrellisWeight, "__init__",
+                        lambda self, *a: seen.append(a))
+    forward.TrellisWeight.load(path, device="cpu")
+    forward.TrellisWeight.from_result(result, device="cpu")
+    stored = export.stored_fields(result)
+    for trellis, suh, svh, K, code in seen:
+        assert torch.equal(trellis, stored["trellis"]) and torch.equal(suh, stored["suh"])
+        assert torch.equal(svh, stored["svh"]) and (K, code) == (5, "exl3_mcg")
+    assert len(seen) == 2

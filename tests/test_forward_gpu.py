@@ -1,0 +1,282 @@
+"""GPU tests of the forward operators on EXL3 tensors against 64-bit values.
+
+The dense weight comes from the oracle's decode (pinned to the reference), in fp64.
+
+Tolerance of one product, per output: with xh = (x suh) B the rotated activations and
+V = W_inner B diag(svh), y_j = sum_i xh_i V_ij.  The kernel rounds each xh_i once to
+fp16, off by at most 2^-11 |xh_i| (half a step; the block scale keeps fp16 normal), with
+a variance of at most a third of that squared; the roundings are independent, so the
+error has a standard deviation below 2^-11 / sqrt(3) * s_j, s_j = sqrt(sum_i xh_i^2
+V_ij^2), and eight of those are allowed.  The fp32 sums add at most 2^-22 of a partial sum (a few
+s_j) for each of the k / 16 steps: k / 16 * 2^-20 * s_j covers them.  The epilogue's
+few fp32 operations add 2^-20 of the magnitudes they see, and the result is rounded
+once, half a step of its type: eps / 2 of its magnitude.  The activations' slopes are
+below 1.13."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+CODES = ("exl3_mul1", "exl3_3inst", "exl3_mcg")
+
+
+@pytest.fixture(scope="module")
+def fw():
+    from exl3b import forward
+    return forward
+
+
+def _had(blocks):
+    h = np.ones((1, 1))
+    while h.shape[0] < 128:
+        h = np.block([[h, h], [h, -h]])
+    return np.kron(np.eye(blocks), h / math.sqrt(128.0))
+
+
+class Problem:
+    """A random EXL3 tensor and its fp64 pieces."""
+
+    def __init__(self, oracle, k, n, K, code="exl3_mul1", seed=0, scale=None):
+        rng = np.random.default_rng(seed)
+        self.k, self.n, self.K, self.code = k, n, K, code
+        tr = rng.integers(-32768, 32768, (k // 16, n // 16, 16 * K)).astype(np.int16)
+        std = 1.0 / math.sqrt(k) if scale is None else scale
+        sgn = lambda m: rng.choice([-1.0, 1.0], m) * np.exp(0.3 * rng.standard_normal(m))
+        self.suh = (sgn(k) * std / 1.24).astype(np.float16)
+        self.svh = sgn(n).astype(np.float16)
+        self.trellis = tr
+        inner = oracle.decode_trellis(tr, oracle.code_lut(code), K, k, n).astype(np.float64)
+        self.V = inner @ _had(n // 128) * self.svh.astype(np.float64)[None, :]
+        self.B = _had(k // 128)
+
+    def weight(self, fw):
+        t = lambda a: torch.from_numpy(a).cuda()
+        return fw.TrellisWeight(t(self.trellis), t(self.suh), t(self.svh), self.K, self.code)
+
+    def product(self, x):
+        """x (fp64 numpy [M, k]) -> (x W, its tolerance)"""
+        xh = (x * self.suh.astype(np.float64)) @ self.B
+        s = np.sqrt((xh ** 2) @ (self.V ** 2))
+        return xh @ self.V, s * (8 * 2.0 ** -11 / math.sqrt(3) + self.k / 16 * 2.0 ** -20)
+
+
+def act64(v, act):
+    t = torch.from_numpy(v)
+    if act == "relu":
+        t = t.clamp(min=0)
+    elif act == "silu":
+        t = t * torch.sigmoid(t)
+    elif act == "gelu":
+        t = torch.nn.functional.gelu(t)
+    elif act == "gelu_tanh":
+        t = torch.nn.functional.gelu(t, approximate="tanh")
+    return t.numpy()
+
+
+def f64(t):
+    return None if t is None else t.detach().double().cpu().numpy()
+
+
+def expect(prob, x, bias=None, act=None, mul=None, residual=None):
+    """(value, tolerance) of linear in fp64"""
+    y, tol = prob.product(f64(x))
+    if bias is not None:
+        y = y + f64(bias)
+    tol = tol + 2.0 ** -20 * np.abs(y)
+    y, tol = act64(y, act), tol * (1.13 if act else 1.0)
+    if mul is not None:
+        y, tol = y * f64(mul), tol * np.abs(f64(mul))
+    if residual is not None:
+        y = y + f64(residual)
+        tol = tol + 2.0 ** -23 * np.abs(f64(residual))
+    half = torch.finfo(x.dtype).eps / 2
+    return y, tol + half * (np.abs(y) + tol) + torch.finfo(x.dtype).smallest_normal * half
+
+
+def check(got, want, tol):
+    d = np.abs(f64(got) - want)
+    bad = ~(d <= tol)
+    assert not bad.any(), (int(bad.sum()), float(np.nanmax(d / tol)), np.argwhere(bad)[:4])
+
+
+def rnd(shape, dtype, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(shape, generator=g) * scale
+    if x.dim() > 1:
+        x[..., ::97] *= 15.0                     # a few loud channels
+    return x.to(dtype).cuda()
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("K", range(2, 8))
+def test_linear_codes(fw, oracle, K, code):
+    prob = Problem(oracle, 384, 256, K, code, seed=K)
+    w = prob.weight(fw)
+    for M in (3, 40):
+        x = rnd((M, 384), torch.float16, M)
+        check(fw.linear(x, w), *expect(prob, x))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M", [1, 2, 7, 8, 9, 15, 16, 17, 31, 32, 33, 63, 65, 128, 129, 223, 225,
+                               300, 517])
+def test_linear_rows(fw, oracle, M, dtype):
+    prob = Problem(oracle, 640, 384, 4, seed=7)
+    x = rnd((M, 640), dtype, M)
+    check(fw.linear(x, prob.weight(fw)), *expect(prob, x))
+
+
+@pytest.mark.parametrize("k,n", [(128, 128), (128, 1152), (1152, 128), (4992, 256), (256, 2176),
+                                 (17408, 128)])
+def test_linear_shapes(fw, oracle, k, n):
+    prob = Problem(oracle, k, n, 5, seed=k + n)
+    w = prob.weight(fw)
+    for M in (1, 11, 70):
+        x = rnd((M, k), torch.bfloat16, M)
+        check(fw.linear(x, w), *expect(prob, x))
+
+
+@pytest.mark.parametrize("M", [5, 50])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", [None, "relu", "silu", "gelu", "gelu_tanh"])
+def test_linear_epilogue(fw, oracle, act, dtype, M):
+    prob = Problem(oracle, 256, 384, 3, seed=3)
+    w = prob.weight(fw)
+    x, bias = rnd((M, 256), dtype, 1), rnd((384,), dtype, 2)
+    mul, res = rnd((M, 384), dtype, 3), rnd((M, 384), dtype, 4)
+    for kw in ({}, {"bias": bias}, {"mul": mul}, {"residual": res},
+               {"bias": bias, "mul": mul, "residual": res}):
+        got = fw.linear(x, w, activation=act, **kw)
+        check(got, *expect(prob, x, act=act, **kw))
+
+
+@pytest.mark.parametrize("M", [3, 40])
+@pytest.mark.parametrize("scale", [1e-36, 1e-30, 1e30])
+def test_linear_range_of_bf16(fw, oracle, scale, M):
+    """Activations far outside fp16's range are no matter: blocks are scaled."""
+    prob = Problem(oracle, 384, 128, 4, seed=9)
+    x = rnd((M, 384), torch.bfloat16, 5, scale)
+    x[:, 128:256] *= 1e-3                     # blocks of different magnitude
+    x[1] = 0                                  # and a row of zeros
+    got = fw.linear(x, prob.weight(fw))
+    check(got, *expect(prob, x))
+    assert not got[1].any()
+
+
+@pytest.mark.parametrize("M", [4, 48])
+def test_linear_rows_are_independent(fw, oracle, M):
+    """A NaN or infinite row spoils itself only; rows do not depend on the batch."""
+    prob = Problem(oracle, 512, 256, 6, seed=11)
+    w = prob.weight(fw)
+    x = rnd((M, 512), torch.bfloat16, 6)
+    clean = fw.linear(x, w)
+    x[1, 130] = float("inf")
+    x[2, 5] = float("nan")
+    got = fw.linear(x, w)
+    keep = [i for i in range(M) if i not in (1, 2)]
+    assert torch.equal(got[keep], clean[keep])
+    assert not torch.isfinite(got[1]).any() and torch.isnan(got[2]).all()
+
+
+@pytest.mark.parametrize("M", [6, 60])
+def test_linear_layouts(fw, oracle, M):
+    prob = Problem(oracle, 256, 128, 4, seed=13)
+    w = prob.weight(fw)
+    dt = torch.float16
+    x, res = rnd((M, 256), dt, 1), rnd((M, 128), dt, 2)
+    ref = fw.linear(x, w, residual=res)
+    check(ref, *expect(prob, x, residual=res))
+    # row pitch, odd offset, transposed storage, expanded rows, leading dimensions
+    wide = torch.zeros(M, 520, dtype=dt, device="cuda")
+    for off in (0, 4, 3):
+        v = wide[:, off:off + 256]
+        v.copy_(x)
+        assert torch.equal(fw.linear(v, w, residual=res), ref)
+    assert torch.equal(fw.linear(x.t().contiguous().t(), w,
+                                 residual=res.t().contiguous().t()), ref)
+    assert torch.equal(fw.linear(x[:1].expand(M, 256), w), fw.linear(x[:1], w).expand(M, 128))
+    assert torch.equal(fw.linear(x.view(2, M // 2, 256), w, residual=res.view(2, M // 2, 128)),
+                       ref.view(2, M // 2, 128))
+    assert torch.equal(fw.linear(x[0], w), fw.linear(x[:1], w)[0])
+    assert fw.linear(x[:0], w).shape == (0, 128)
+    # out: a column range of a wider buffer, whose other columns stay
+    buf = torch.full((M + 2, 384), 7.0, dtype=dt, device="cuda")
+    o = buf[1:M + 1, 128:256]
+    assert fw.linear(x, w, residual=res, out=o) is o
+    assert torch.equal(o, ref)
+    o.fill_(7.0)
+    assert bool((buf == 7.0).all())
+    # in place on the residual, and on mul
+    r2 = res.clone()
+    fw.linear(x, w, residual=r2, out=r2)
+    assert torch.equal(r2, ref)
+    m2 = res.clone()
+    fw.linear(x, w, mul=m2, out=m2)
+    assert torch.equal(m2, fw.linear(x, w, mul=res))
+    with pytest.raises(ValueError, match="overlaps"):
+        fw.linear(wide[:, :256], w, out=wide[:, 128:256])
+
+
+@pytest.mark.parametrize("M", [1, 9, 90, 260])
+def test_linear_repeats_and_streams(fw, oracle, M):
+    """The same bits every time: on another stream, and from a replayed graph."""
+    prob = Problem(oracle, 1280, 512, 5, seed=17)
+    w = prob.weight(fw)
+    x, res = rnd((M, 1280), torch.bfloat16, 1), rnd((M, 512), torch.bfloat16, 2)
+    ref = fw.linear(x, w, residual=res, activation="silu")
+    for _ in range(3):
+        assert torch.equal(fw.linear(x, w, residual=res, activation="silu"), ref)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = fw.linear(x, w, residual=res, activation="silu")
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, ref)
+    graphs, outs = [], []
+    xs = x.clone()
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(fw.linear(xs, w, residual=res, activation="silu"))
+        graphs.append(g)
+    xs.copy_(x.flip(0))
+    for g in graphs:
+        g.replay()
+    want = fw.linear(xs, w, residual=res, activation="silu")
+    assert all(torch.equal(o, want) for o in outs)
+
+
+def test_linear_refuses_gradients_and_devices(fw, oracle):
+    prob = Problem(oracle, 128, 128, 4)
+    w = prob.weight(fw)
+    x = rnd((2, 128), torch.bfloat16, 1).requires_grad_()
+    with pytest.raises(ValueError, match="gradient"):
+        fw.linear(x, w)
+    with torch.no_grad():
+        assert not fw.linear(x, w).requires_grad
+    with pytest.raises(ValueError, match="is on"):
+        fw.linear(x.detach().cpu(), w)
+
+
+@pytest.mark.parametrize("channel_scales", [False, True])
+def test_linear_of_a_quantized_layer(fw, tmp_path, channel_scales):
+    """quantize_linear_fused -> stored fields -> linear: the forward product equals
+    x W_hat^T of the quantizer's own W_hat, from the result and from the files."""
+    from exl3b import api, export
+    g = torch.Generator().manual_seed(0)
+    W = torch.randn(256, 128, generator=g) * 0.05
+    r = api.quantize_linear(W, torch.eye(128), K=4, channel_scales=channel_scales,
+                            out_device="cuda")
+    x = rnd((5, 128), torch.float16, 3)
+    w = fw.TrellisWeight.from_result(r)
+    got = fw.linear(x, w)
+    ref = x.double() @ r["W_hat"].double().t()
+    # suh is stored in fp16 (its scale folded in): 2^-11 of each weight, the
+    # operand's and the result's rounding as much again each
+    scale = (x.double() ** 2 @ r["W_hat"].double().t() ** 2).sqrt()
+    assert bool(((got.double() - ref).abs() <= 3 * 8 * 2.0 ** -11 * scale + 2.0 ** -11 * ref.abs()).all())
+    path = export.save_quantized(tmp_path, 0, "mlp.up_proj", r)
+    assert torch.equal(fw.linear(x, fw.TrellisWeight.load(path)), got)

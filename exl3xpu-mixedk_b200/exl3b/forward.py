@@ -1,6 +1,7 @@
 """Forward operators on finished EXL3 tensors.
 
     linear   act(x W^T + bias) * mul + residual, W an EXL3 tensor
+    moe      a mixture-of-experts layer for a few tokens, its experts EXL3 tensors
 
 The consumer's side of the quantizer: what a layer computes from the fields the
 quantizer stores (trellis, suh, svh), without writing a dense weight.  Weights
@@ -15,6 +16,7 @@ is refused while gradients are enabled.
 from __future__ import annotations
 
 import json
+import struct
 from pathlib import Path
 
 import torch
@@ -209,3 +211,97 @@ def linear(x: torch.Tensor, w: TrellisWeight, bias: torch.Tensor | None = None,
                  0 if rr is None else rr.data_ptr(), 0 if rr is None else _ld(rr),
                  o.data_ptr(), _ld(o), ws_ptr, nbytes, ops.stream_handle(dev))
     return o.view(*lead, w.n) if out is None else out
+
+
+# ------------------------------------------------------------------ mixture of experts
+MOE_TOKENS = 256            # of one launch; longer inputs are cut
+MOE_EXPERTS, MOE_TOP_K = 1024, 32
+
+
+class TrellisExperts:
+    """The experts of one mixture-of-experts layer: gate and up [D -> F] and down
+    [F -> D], one TrellisWeight per expert each, of one code and on one device;
+    bit widths may differ from tensor to tensor."""
+
+    def __init__(self, gate, up, down):
+        gate, up, down = list(gate), list(up), list(down)
+        if not gate or len(gate) != len(up) or len(gate) != len(down):
+            raise ValueError(f"{len(gate)} gate, {len(up)} up and {len(down)} down weights: "
+                             "need one of each per expert")
+        if len(gate) > MOE_EXPERTS:
+            raise ValueError(f"{len(gate)} experts: at most {MOE_EXPERTS}")
+        first = gate[0]
+        self.D, self.F, self.E = first.k, first.n, len(gate)
+        for what, ws, shape in (("gate", gate, (self.D, self.F)), ("up", up, (self.D, self.F)),
+                                ("down", down, (self.F, self.D))):
+            for e, w in enumerate(ws):
+                if (w.k, w.n) != shape or w.code != first.code or w.device != first.device:
+                    raise ValueError(f"{what} of expert {e} is {w}, expected [{shape[0]}, "
+                                     f"{shape[1]}] {first.code} on {first.device}")
+        self.device, self.code_id = first.device, first.code_id
+        self.weights = (gate, up, down)
+        self.Kmax = tuple(max(w.K for w in ws) for ws in self.weights)
+        table = b"".join(struct.pack("<QQQii", w.trellis.data_ptr(), w.suh.data_ptr(),
+                                     w.svh.data_ptr(), w.K, 0)
+                         for ws in self.weights for w in ws)
+        self.table = torch.frombuffer(bytearray(table), dtype=torch.uint8).to(self.device)
+
+
+def _rows16(t: torch.Tensor, cols: int) -> torch.Tensor:
+    """_rows with 16-byte aligned rows (8 elements of 2 bytes, 4 of 4)."""
+    t = t.reshape(-1, cols)
+    if t.stride(1) == 1 and t.data_ptr() % 16 == 0 and \
+            (t.shape[0] <= 1 or (t.stride(0) >= cols and t.stride(0) % 8 == 0)):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def moe(x: torch.Tensor, router: torch.Tensor, experts: TrellisExperts, top_k: int,
+        normalize: bool = True, residual: torch.Tensor | None = None, *,
+        out: torch.Tensor | None = None) -> torch.Tensor:
+    """Mixture-of-experts layer, for the few tokens of a decoding batch:
+
+        l = x router^T; S = the top_k largest (ties: lowest index); p = softmax(l)
+        y = sum_{e in S} w_e down_e(silu(gate_e x) * up_e x) + residual
+
+    with w = p, or p / sum_S p if `normalize`.  x [..., D] bf16 or fp16, router
+    [E, D] of x's dtype or fp32, residual [..., D].  Returns [..., D] in x's
+    dtype, or writes `out`, which may be `residual` itself.  More than 256 tokens
+    are taken 256 at a time; every chosen expert is read once per launch for 8 or
+    16 of its tokens, so long prompts are better served by linear per expert."""
+    if x.dtype not in DTYPE_IDS:
+        raise ValueError(f"x must be bf16 or fp16, got {x.dtype}")
+    if x.device != experts.device:
+        raise ValueError(f"x is on {x.device}, the experts on {experts.device}")
+    if x.dim() < 1 or x.shape[-1] != experts.D:
+        raise ValueError(f"x {tuple(x.shape)} for experts with in = {experts.D}")
+    top_k = int(top_k)
+    if not 1 <= top_k <= min(experts.E, MOE_TOP_K):
+        raise ValueError(f"top_k={top_k} with {experts.E} experts (at most {MOE_TOP_K})")
+    if router.dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"router must be {x.dtype} or float32, got {router.dtype}")
+    _check_input("moe", "router", router, (experts.E, experts.D), router.dtype, x.device)
+    _no_grad("moe", x, router, residual)
+    lead, D = x.shape[:-1], experts.D
+    if residual is not None:
+        _check_input("moe", "residual", residual, (*lead, D), x.dtype, x.device)
+    xr = _rows16(x, D)
+    rt = _rows16(router, D)
+    rr = None if residual is None else _rows(residual, D)
+    o = _out_rows("moe", out, lead, D, xr, (rr,))
+    T = xr.shape[0]
+    if T:
+        with torch.cuda.device(x.device):
+            dev = ops.select_device(xr)
+            nbytes = lib().exl3b_moe_workspace_bytes(min(T, MOE_TOKENS), D, experts.F, experts.E,
+                                                     top_k)
+            ws, ws_ptr = _workspace(nbytes, x.device)
+            for t in range(0, T, MOE_TOKENS):
+                n = min(MOE_TOKENS, T - t)
+                call("exl3b_moe", xr[t:].data_ptr(), DTYPE_IDS[x.dtype], _ld(xr), n, D, experts.F,
+                     experts.E, top_k, int(bool(normalize)), rt.data_ptr(),
+                     0 if router.dtype == torch.float32 else DTYPE_IDS[x.dtype], _ld(rt),
+                     experts.table.data_ptr(), *experts.Kmax, experts.code_id,
+                     0 if rr is None else rr[t:].data_ptr(), 0 if rr is None else _ld(rr),
+                     o[t:].data_ptr(), _ld(o), ws_ptr, nbytes, ops.stream_handle(dev))
+    return o.view(*lead, D) if out is None else out

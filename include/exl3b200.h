@@ -344,6 +344,38 @@ int exl3b_linear(const void* dX, int dtype, int64_t ldx, int M, int k, int n,
                  int64_t ldres, void* dOut, int64_t ldo, void* ws, size_t ws_bytes,
                  void* stream);
 
+/* One EXL3 tensor in device memory, as in exl3b_linear. */
+typedef struct {
+    const void* trellis;      /* int16 [in/16][out/16][16 K], 16-byte aligned */
+    const void* suh;          /* fp16 [in], 8-byte aligned */
+    const void* svh;          /* fp16 [out], 8-byte aligned */
+    int32_t K;
+    int32_t reserved;
+} exl3b_expert;
+
+/* Mixture-of-experts layer for a few tokens:
+ *   l = x . router^T, S = the top_k largest l of a token (ties: the lowest
+ *   index), p = softmax(l) over all E, w = p / sum_S p (normalize != 0) or p
+ *   out = sum_{e in S} w_e ((silu(x . gate_e) * (x . up_e)) . down_e) + residual
+ *   x [T][D] and router [E][D] with 16-byte aligned rows (pitches multiples of
+ *         8 elements); residual (nullable) and out [T][D] with 8-byte aligned
+ *         rows; dtype 1 = bf16, 2 = fp16; router_dtype the same, or 0 = fp32
+ *   dExperts device table [3][E]: gate [D][F], up [D][F], down [F][D] of every
+ *         expert, all of one code; each K in 2..Kmax of its kind (an entry
+ *         outside is not computed, and its tokens' rows are not written)
+ *   T <= 256, E <= 1024, top_k <= 32; D and F multiples of 128
+ * Logits are summed in fp64, so a token's choice does not depend on the batch;
+ * every other sum is fp32 in a fixed order; one rounding to dtype at the end.
+ * ws: exl3b_moe_workspace_bytes bytes, 256-byte aligned, in use until the work
+ * queued on `stream` has run.  out may be residual's rows; it must not overlap
+ * x otherwise. */
+size_t exl3b_moe_workspace_bytes(int T, int D, int F, int E, int top_k);
+int exl3b_moe(const void* dX, int dtype, int64_t ldx, int T, int D, int F, int E,
+              int top_k, int normalize, const void* dRouter, int router_dtype,
+              int64_t ldr, const exl3b_expert* dExperts, int Kmax_gate, int Kmax_up,
+              int Kmax_down, int code, const void* d_residual, int64_t ldres,
+              void* dOut, int64_t ldo, void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

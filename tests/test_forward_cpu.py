@@ -116,3 +116,71 @@ def test_load_reads_what_the_writer_stores(tmp_path, monkeypatch):
         assert torch.equal(trellis, stored["trellis"]) and torch.equal(suh, stored["suh"])
         assert torch.equal(svh, stored["svh"]) and (K, code) == (5, "exl3_mcg")
     assert len(seen) == 2
+
+
+def _moe(**kw):
+    from exl3b import native
+    a = dict(x=P, dtype=1, ldx=256, T=4, D=256, F=128, E=8, top_k=2, norm=1, router=P, rdt=1,
+             ldr=256, table=P, Kg=4, Ku=4, Kd=4, code=0, res=None, ldres=0, out=P, ldo=256, ws=P,
+             wsb=1 << 30)
+    a.update(kw)
+    rc = native.lib().exl3b_moe(*a.values(), None)
+    return rc, native.last_error()
+
+
+@pytest.mark.parametrize("kw,rc,msg", [
+    (dict(Kg=1), 8, "K=1"), (dict(Kd=8), 8, "K=8"), (dict(code=3), 7, "code 3"),
+    (dict(dtype=0), 7, "dtype 0"), (dict(rdt=2), 7, "router dtype 2"),
+    (dict(T=257), 7, "257 tokens"), (dict(T=-1), 7, "tokens"), (dict(D=192), 7, "hidden 192"),
+    (dict(F=64), 7, "width 64"), (dict(E=0), 7, "0 experts"), (dict(E=1025), 7, "1025 experts"),
+    (dict(top_k=0), 7, "top_k 0"), (dict(top_k=9), 7, "top_k 9"),
+    (dict(E=64, top_k=33), 7, "top_k 33"),
+    (dict(x=P + 8), 7, "16-byte"), (dict(ldx=260), 7, "16-byte"), (dict(router=None), 7, "16-byte"),
+    (dict(ldr=248), 7, "16-byte"), (dict(table=P + 4), 7, "16-byte"),
+    (dict(out=P + 4), 7, "8-byte"), (dict(ldo=128), 7, "8-byte"),
+    (dict(res=P, ldres=254), 7, "8-byte"),
+    (dict(ws=None), 11, "workspace"), (dict(wsb=64), 11, "workspace"),
+    (dict(ws=P + 16), 11, "workspace"),
+])
+def test_moe_abi_refuses(kw, rc, msg):
+    got, text = _moe(**kw)
+    assert got == rc and msg in text, (got, text)
+
+
+def test_moe_workspace_bytes():
+    from exl3b import native
+    f = native.lib().exl3b_moe_workspace_bytes
+    assert f(0, 256, 128, 8, 2) == 0 and f(257, 256, 128, 8, 2) == 0 and f(4, 256, 100, 8, 2) == 0
+    # ids, weights, counters, h and its scales, partial rows
+    assert f(4, 256, 128, 8, 2) >= 8 * 4 + 8 * 4 + 4 * 2 * 4 + 8 * 128 * 2 + 8 * 4 + 8 * 256 * 4
+    assert _moe(T=0, x=None, ws=None)[0] == 0
+
+
+def test_experts_and_moe_refuse():
+    from exl3b import forward
+
+    class W:
+        def __init__(self, k, n, code="exl3_mul1"):
+            self.k, self.n, self.K, self.code, self.code_id = k, n, 4, code, 0
+            self.device = torch.device("cpu")
+            self.trellis = self.suh = self.svh = torch.zeros(1)
+    g, d = W(256, 128), W(128, 256)
+    for args, msg in [(([], [], []), "one of each"), (([g], [g, g], [d]), "one of each"),
+                      (([g], [d], [d]), "up of expert 0"), (([g, g], [g, g], [d, g]), "down of expert 1"),
+                      (([g, W(256, 128, "exl3_mcg")], [g, g], [d, d]), "gate of expert 1"),
+                      (([g] * 1025, [g] * 1025, [d] * 1025), "at most 1024")]:
+        with pytest.raises(ValueError, match=msg):
+            forward.TrellisExperts(*args)
+    ex = forward.TrellisExperts([g] * 4, [g] * 4, [d] * 4)
+    assert (ex.D, ex.F, ex.E, ex.Kmax) == (256, 128, 4, (4, 4, 4)) and ex.table.numel() == 12 * 32
+    x = torch.zeros(3, 256, dtype=torch.bfloat16)
+    r = torch.zeros(4, 256, dtype=torch.bfloat16)
+    for args, kw, msg in [((x.float(), r, ex, 2), {}, "bf16 or fp16"),
+                          ((x[:, :128], r, ex, 2), {}, "in = 256"),
+                          ((x, r, ex, 0), {}, "top_k=0"), ((x, r, ex, 5), {}, "top_k=5"),
+                          ((x, r[:3], ex, 2), {}, "router"), ((x, r.half(), ex, 2), {}, "router"),
+                          ((x, r, ex, 2), dict(residual=x[:2]), "residual"),
+                          ((x, r, ex, 2), dict(out=x), "overlaps x"),
+                          ((x, r.clone().requires_grad_(), ex, 2), {}, "gradient")]:
+        with pytest.raises(ValueError, match=msg):
+            forward.moe(*args, **kw)

@@ -280,3 +280,190 @@ def test_linear_of_a_quantized_layer(fw, tmp_path, channel_scales):
     assert bool(((got.double() - ref).abs() <= 3 * 8 * 2.0 ** -11 * scale + 2.0 ** -11 * ref.abs()).all())
     path = export.save_quantized(tmp_path, 0, "mlp.up_proj", r)
     assert torch.equal(fw.linear(x, fw.TrellisWeight.load(path)), got)
+
+
+# ------------------------------------------------------------------ mixture of experts
+class Layer:
+    """Random experts, each tensor at its own K."""
+
+    def __init__(self, oracle, fw, D, F, E, Ks, code="exl3_mul1", seed=0):
+        self.D, self.F, self.E = D, F, E
+        K = lambda i: Ks[i % len(Ks)]
+        self.gate = [Problem(oracle, D, F, K(3 * e), code, 1000 * seed + 3 * e) for e in range(E)]
+        self.up = [Problem(oracle, D, F, K(3 * e + 1), code, 1000 * seed + 3 * e + 1) for e in range(E)]
+        self.down = [Problem(oracle, F, D, K(3 * e + 2), code, 1000 * seed + 3 * e + 2)
+                     for e in range(E)]
+        self.experts = fw.TrellisExperts(*([p.weight(fw) for p in ps]
+                                           for ps in (self.gate, self.up, self.down)))
+
+    def expect(self, x, router, top_k, normalize=True, residual=None):
+        """(value, tolerance) in fp64.  The tolerance of h = silu(g) u follows from
+        those of g and u; its errors (each eight deviations, nearly uncorrelated
+        over F) reach the output through the down weights as the root of the sum
+        of squares, with half as much again for what correlation there is."""
+        X, R = f64(x), f64(router)
+        logits = X @ R.T
+        T = X.shape[0]
+        y, tol = np.zeros((T, self.D)), np.zeros((T, self.D))
+        for t in range(T):
+            order = sorted(range(self.E), key=lambda e: (-logits[t, e], e))[:top_k]
+            p = np.exp(logits[t] - logits[t].max())
+            p /= p.sum()
+            total = p[order].sum() if normalize else 1.0
+            for e in order:
+                xt = X[t:t + 1]
+                g, tg = self.gate[e].product(xt)
+                u, tu = self.up[e].product(xt)
+                s = act64(g, "silu")
+                h = s * u
+                th = 1.1 * tg * (np.abs(u) + tu) + np.abs(s) * tu + 2.0 ** -20 * np.abs(h)
+                d = self.down[e]
+                v, tv = d.product(h)
+                W = (d.suh.astype(np.float64)[:, None] * (d.B @ d.V))
+                tv = tv + 1.5 * np.sqrt(th ** 2 @ W ** 2)
+                y[t] += p[e] / total * v[0]
+                tol[t] += p[e] / total * tv[0]
+        tol += 2.0 ** -20 * np.abs(y)
+        if residual is not None:
+            y = y + f64(residual)
+        half = torch.finfo(x.dtype).eps / 2
+        return y, tol + half * (np.abs(y) + tol) + torch.finfo(x.dtype).smallest_normal
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,D,F,E,top_k,code", [
+    (1, 128, 128, 4, 1, "exl3_mul1"), (1, 384, 256, 6, 6, "exl3_mcg"),
+    (2, 256, 128, 40, 8, "exl3_3inst"), (7, 640, 384, 5, 2, "exl3_mul1"),
+    (9, 256, 640, 9, 3, "exl3_mul1"), (40, 256, 128, 2, 1, "exl3_mul1"),
+    (70, 384, 256, 3, 3, "exl3_mcg"), (33, 256, 256, 1, 1, "exl3_mul1")])
+def test_moe_values(fw, oracle, T, D, F, E, top_k, code, dtype):
+    layer = Layer(oracle, fw, D, F, E, [4, 7, 2, 5, 3, 6, 4], code, seed=T)
+    x = rnd((T, D), dtype, T)
+    router = (rnd((E, D), torch.float32, 99) / math.sqrt(D)).to(dtype)
+    res = rnd((T, D), dtype, 5)
+    for kw in ({}, {"normalize": False}, {"residual": res}):
+        check(fw.moe(x, router, layer.experts, top_k, **kw),
+              *layer.expect(x, router, top_k, **kw))
+    r32 = router.float() * 1.01
+    check(fw.moe(x, r32, layer.experts, top_k), *layer.expect(x, r32, top_k))
+
+
+def test_moe_ties_take_the_lowest_index(fw, oracle):
+    layer = Layer(oracle, fw, 256, 128, 6, [4], seed=3)
+    x = rnd((3, 256), torch.float16, 1)
+    router = rnd((6, 256), torch.float16, 2) / 16
+    router[4] = router[1]
+    router[5] = router[1]
+    check(fw.moe(x, router, layer.experts, 3), *layer.expect(x, router, 3))
+    zero = torch.zeros_like(router)                       # all equal: experts 0 and 1
+    check(fw.moe(x, zero, layer.experts, 2), *layer.expect(x, zero, 2))
+
+
+def test_moe_many_experts_and_long_inputs(fw, oracle):
+    """1024 experts; more than 256 tokens are cut."""
+    layer = Layer(oracle, fw, 128, 128, 8, [4], seed=4)
+    gate, up, down = layer.experts.weights
+    many = fw.TrellisExperts(*([ws[e % 8] for e in range(1024)] for ws in (gate, up, down)))
+    x = rnd((5, 128), torch.bfloat16, 1)
+    router = torch.full((1024, 128), 0.0, dtype=torch.bfloat16, device="cuda")
+    pick = [1023, 31, 512, 704, 64]
+    for t, e in enumerate(pick):
+        router[e] = x[t] * 0.25
+    got = fw.moe(x, router, many, 1)
+    # the loud channels make some token prefer another token's expert
+    for t, e in enumerate((f64(x) @ f64(router).T).argmax(axis=1)):
+        one = torch.zeros(8, 128, dtype=torch.bfloat16, device="cuda")
+        one[e % 8] = x[t]
+        want, tol = layer.expect(x[t:t + 1], one, 1)
+        check(got[t:t + 1], want, tol)
+    # each token its own expert: one-hot tokens and router rows
+    x = torch.zeros(5, 128, dtype=torch.bfloat16, device="cuda")
+    router.zero_()
+    for t, e in enumerate(pick):
+        x[t, 9 * t] = router[e, 9 * t] = 2.0
+    got = fw.moe(x, router, many, 1)
+    for t, e in enumerate(pick):
+        one = torch.zeros(8, 128, dtype=torch.bfloat16, device="cuda")
+        one[e % 8] = x[t]
+        check(got[t:t + 1], *layer.expect(x[t:t + 1], one, 1))
+    x = rnd((517, 128), torch.bfloat16, 2)
+    r = rnd((8, 128), torch.float32, 3) / 12
+    got = fw.moe(x, r, layer.experts, 2, residual=x)
+    check(got[200:300], *layer.expect(x[200:300], r, 2, residual=x[200:300]))
+    check(got[500:], *layer.expect(x[500:], r, 2, residual=x[500:]))
+
+
+def test_moe_rows_are_independent(fw, oracle):
+    layer = Layer(oracle, fw, 256, 128, 4, [4], seed=5)
+    x = rnd((12, 256), torch.bfloat16, 1)
+    router = rnd((4, 256), torch.bfloat16, 2) / 16
+    clean = fw.moe(x, router, layer.experts, 2)
+    x[3, 7] = float("nan")
+    x[8, 200] = float("inf")
+    got = fw.moe(x, router, layer.experts, 2)
+    keep = [i for i in range(12) if i not in (3, 8)]
+    assert torch.equal(got[keep], clean[keep])
+    assert torch.isnan(got[3]).all() and not torch.isfinite(got[8]).any()
+    # a router row that is NaN or infinite spoils the softmax, and nothing else
+    router[2, 0] = float("nan")
+    assert torch.isnan(fw.moe(x[:1], router, layer.experts, 2)).all()
+    assert not fw.moe(torch.zeros_like(x[:2]), router.nan_to_num(), layer.experts, 2).any()
+
+
+def test_moe_layouts_graphs_and_streams(fw, oracle):
+    layer = Layer(oracle, fw, 384, 256, 5, [3, 5], seed=6)
+    x, res = rnd((6, 384), torch.bfloat16, 1), rnd((6, 384), torch.bfloat16, 2)
+    router = rnd((5, 384), torch.bfloat16, 3) / 20
+    call = lambda x, **kw: fw.moe(x, router, layer.experts, 2, **kw)
+    ref = call(x, residual=res)
+    for _ in range(3):
+        assert torch.equal(call(x, residual=res), ref)
+    wide = torch.zeros(6, 900, dtype=torch.bfloat16, device="cuda")
+    for off in (0, 8, 4, 1):
+        v = wide[:, off:off + 384]
+        v.copy_(x)
+        assert torch.equal(call(v, residual=res), ref)
+    assert torch.equal(call(x.view(2, 3, 384), residual=res.view(2, 3, 384)), ref.view(2, 3, 384))
+    assert call(x[:0]).shape == (0, 384)
+    assert torch.equal(fw.moe(x, router.t().contiguous().t(), layer.experts, 2, residual=res), ref)
+    r2 = res.clone()
+    assert call(x, residual=r2, out=r2) is r2 and torch.equal(r2, ref)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = call(x, residual=res)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, ref)
+    xs, graphs, outs = x.clone(), [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call(xs, residual=res))
+        graphs.append(g)
+    xs.copy_(x.flip(0))
+    for _ in range(2):
+        for g in graphs:
+            g.replay()
+    want = call(xs, residual=res)
+    assert all(torch.equal(o, want) for o in outs)
+
+
+def test_block_of_quantized_layers(fw):
+    """Quantized gate, up and down as a user runs them: a dense gated block with its
+    residual, then the same tensors as a one-expert layer."""
+    from exl3b import api
+    g = torch.Generator().manual_seed(1)
+    D, F = 256, 384
+    mk = lambda o, i, K: fw.TrellisWeight.from_result(api.quantize_linear(
+        torch.randn(o, i, generator=g) / math.sqrt(i), None, K=K, out_device="cuda"))
+    gate, up, down = mk(F, D, 4), mk(F, D, 5), mk(D, F, 6)
+    x = rnd((4, D), torch.float16, 1)
+    h = fw.linear(x, gate, activation="silu", mul=fw.linear(x, up))
+    y = fw.linear(h, down, residual=x)
+    z = fw.moe(x, torch.zeros(1, D, dtype=torch.float16, device="cuda"),
+               fw.TrellisExperts([gate], [up], [down]), 1, residual=x)
+    # the dense path rounds up(x) and h to fp16 (2^-11 of each) and the moe path
+    # rotates and rounds h itself; both sum the same 384 products of down
+    scale = (h.double().abs() @ torch.ones(F, 1, dtype=torch.float64, device="cuda")) / math.sqrt(F)
+    assert bool(((y.double() - z.double()).abs()
+                 <= 2.0 ** -10 * (z.double().abs() + 4 * scale)).all())

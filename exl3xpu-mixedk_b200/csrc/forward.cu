@@ -3,13 +3,10 @@
 //
 // x W = (((x suh) B) W_inner) B svh: the activations are rotated instead of the
 // weights, so the weight is only ever read as its trellis (K / 8 bytes per weight).
-#include <cooperative_groups.h>
 
 #include "exl3b_internal.h"
 #include "forward_few.cuh"
 #include "../../include/exl3b200.h"
-
-namespace cg = cooperative_groups;
 
 namespace exl3b {
 
@@ -32,129 +29,153 @@ struct LinearArgs {
     int64_t ldo;
 };
 
-// act(v * svh + bias) * mul + residual of four columns of one row, rounded once.
-__device__ __forceinline__ void linear_finish(const LinearArgs& a, int row, int col, float (&v)[4]) {
-    float t[4];
-    load4(a.svh + col, t);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] *= t[j];
-    if (a.bias) {
-        load4x(a.bias, col, a.dtype, t);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] += t[j];
+// Epilogue operands of four columns of one row, loaded ahead of the product's sums.
+struct LinearEpilogue {
+    float svh[4], bias[4], mul[4], res[4];
+    __device__ __forceinline__ void load(const LinearArgs& a, int row, int col) {
+        load4(a.svh + col, svh);
+        if (a.bias) load4x(a.bias, col, a.dtype, bias);
+        if (a.mul) load4x(a.mul, (size_t)row * a.ldmul + col, a.dtype, mul);
+        if (a.residual) load4x(a.residual, (size_t)row * a.ldres + col, a.dtype, res);
     }
-    if (a.act != ACT_NONE) {
+    // act(v * svh + bias) * mul + residual, rounded once
+    __device__ __forceinline__ void finish(const LinearArgs& a, int row, int col, float (&v)[4]) const {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = activate(v[j], a.act);
-    }
-    if (a.mul) {
-        load4x(a.mul, (size_t)row * a.ldmul + col, a.dtype, t);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] *= t[j];
-    }
-    if (a.residual) {
-        load4x(a.residual, (size_t)row * a.ldres + col, a.dtype, t);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] += t[j];
-    }
-    store4x(a.out, (size_t)row * a.ldo + col, a.dtype, v);
-}
-
-// Few rows: CTA (128-column block, row group of 8 G), k split over the CTAs of a
-// cluster, whose partial sums meet through distributed shared memory in rank order.
-template <int CODE, int G>
-__global__ void __launch_bounds__(32 * kFewWarps, 2) linear_few_kernel(const LinearArgs a) {
-    extern __shared__ __align__(16) uint8_t sm[];
-    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-    const int nrank = gridDim.x, rank = blockIdx.x;        // cluster = x dimension
-    const int nb = blockIdx.y, r0 = blockIdx.z * 8 * G;
-    const int rows = min(8 * G, a.M - r0);
-    const int kb = a.k >> 7;
-    const int b0 = (int)((long long)kb * rank / nrank), b1 = (int)((long long)kb * (rank + 1) / nrank);
-    const int nblk = b1 - b0;
-    const int maxblk = (kb + nrank - 1) / nrank;
-    const int xpitch = few_row_bytes(maxblk);
-    uint8_t* ring = sm + warp * few_ring_bytes(a.K);
-    uint8_t* xh = sm + kFewWarps * few_ring_bytes(a.K);
-    float* inv = reinterpret_cast<float*>(xh + 8 * G * xpitch);
-    float* part = inv + maxblk * 8 * G;
-
-    const int tn = a.n >> 4;
-    const size_t kt_bytes = (size_t)tn * 32 * a.K;
-    const uint8_t* src = a.trellis + (size_t)b0 * 8 * kt_bytes + (size_t)(nb * 8 + warp) * 32 * a.K;
-    few_prologue(src, kt_bytes, a.K, nblk, ring, lane);
-    // rotate this CTA's share of the rows; rows past the last are zero
-    for (int i = warp; i < nblk * 8 * G; i += kFewWarps) {
-        const int r = i % (8 * G), b = i / (8 * G);
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (r < rows) {
-            const int k = (b0 + b) * 128 + 4 * lane;
-            float s[4];
-            load4x(a.x, (size_t)(r0 + r) * a.ldx + k, a.dtype, v);
-            load4(a.suh + k, s);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] *= s[j];
+        for (int j = 0; j < 4; ++j) {
+            v[j] *= svh[j];
+            if (a.bias) v[j] += bias[j];
+            if (a.act != ACT_NONE) v[j] = activate(v[j], a.act);
+            if (a.mul) v[j] *= mul[j];
+            if (a.residual) v[j] += res[j];
         }
-        few_put_block(v, xh + r * xpitch + b * 256, inv + i, lane);
+        store4x(a.out, (size_t)row * a.ldo + col, a.dtype, v);
     }
-    __syncthreads();
-    float acc[G][4];
+};
+
+// ------------------------------------------------------------------ few rows
+struct FewScratch {
+    uint8_t* xh;               // [kb][M][256] rotated rows
+    float* inv;                // [kb][M] reciprocal scales
+    float* park;
+};
+
+// suh, rotation and rounding of block b of row r.  A warp.
+__device__ __forceinline__ void linear_rotate(const LinearArgs& a, int r, int b, uint8_t* dst,
+                                              float* inv, int swz) {
+    const int lane = threadIdx.x & 31, k = b * 128 + 4 * lane;
+    float v[4], s[4];
+    load4x(a.x, (size_t)r * a.ldx + k, a.dtype, v);
+    load4(a.suh + k, s);
 #pragma unroll
-    for (int g = 0; g < G; ++g) acc[g][0] = acc[g][1] = acc[g][2] = acc[g][3] = 0.0f;
-    few_product_k<CODE, G>(a.K, src, kt_bytes, nblk, ring, xh, xpitch, inv, acc, lane);
-    few_store_part<G>(part, acc, warp, lane);
-    if (nrank > 1) cg::this_cluster().sync();
-    else __syncthreads();
-    for (int r = rank + nrank * warp; r < rows; r += nrank * kFewWarps) {
-        float v[4];
-        few_sum_row(part, r, nrank, lane, v);
-        linear_finish(a, r0 + r, nb * 128 + 4 * lane, v);
-    }
-    if (nrank > 1) cg::this_cluster().sync();       // partial blocks are read by the others
+    for (int j = 0; j < 4; ++j) v[j] *= s[j];
+    few_put_block(v, dst, inv, lane, swz);
 }
 
-static size_t few_smem(int K, int G, int kb, int S) {
-    const int blk = (kb + S - 1) / S;
-    return (size_t)kFewWarps * few_ring_bytes(K) + (size_t)8 * G * few_row_bytes(blk) +
-           (size_t)blk * 8 * G * 4 + (size_t)8 * G * kPartPitch * 4;
+__global__ void __launch_bounds__(128) linear_rotate_kernel(const LinearArgs a, const FewScratch w) {
+    pdl_launch();
+    const int i = blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (i >= (a.k >> 7) * a.M) return;
+    linear_rotate(a, i % a.M, i / a.M, w.xh + (size_t)i * kRowBytes, w.inv + i, 0);
+}
+
+// Units: (group of 8 G rows, column block).
+template <int G, bool ROTATE>
+struct LinearJob {
+    static constexpr bool kRotate = ROTATE;
+    const LinearArgs& a;
+    const FewScratch& w;
+    int nbn;
+    __device__ __forceinline__ FewUnit unit(int u) const {
+        const int rg = u / nbn, nb = u - rg * nbn;
+        return {a.trellis + (size_t)nb * 256 * a.K, (uint32_t)nbn * 256 * a.K, a.K};
+    }
+    __device__ __forceinline__ int rows(int u) const { return min(8 * G, a.M - u / nbn * 8 * G); }
+    __device__ __forceinline__ size_t row(int u, int r, int b) const {
+        return (size_t)b * a.M + u / nbn * 8 * G + r;
+    }
+    __device__ __forceinline__ const uint8_t* xh() const { return w.xh; }
+    __device__ __forceinline__ const float* inv() const { return w.inv; }
+    __device__ __forceinline__ void wait() const { if (!ROTATE) pdl_wait(); }
+    __device__ __forceinline__ void rotate(int u, int r, int b, uint8_t* dst, float* inv, int swz) const {
+        linear_rotate(a, u / nbn * 8 * G + r, b, dst, inv, swz);
+    }
+};
+
+template <int CODE, int G, bool ROTATE>
+__global__ void __launch_bounds__(32 * kFewWarps, 1)
+linear_few_kernel(const LinearArgs a, const FewScratch w, const FewRun run) {
+    extern __shared__ __align__(16) uint8_t sm[];
+    pdl_launch();
+    const LinearJob<G, ROTATE> job = {a, w, a.n >> 7};
+    few_run<CODE, G>(job, run, a.K, sm, w.park);
+}
+
+// Sum of a unit's parked sums of one row, output rotation and epilogue: a CTA each,
+// whose four warps take every fourth parked sum.
+template <int G>
+__global__ void __launch_bounds__(128)
+linear_finish_kernel(const LinearArgs a, const FewScratch w, const FewRun run) {
+    __shared__ float4 sum[3][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int nb = blockIdx.x, row = blockIdx.y, col = nb * 128 + 4 * lane;
+    LinearEpilogue ep;
+    if (warp == 0) ep.load(a, row, col);
+    pdl_wait();
+    float v[4];
+    few_sum<G>(w.park, run, row / (8 * G) * gridDim.x + nb, row % (8 * G), lane, warp, 4, v);
+    if (warp) sum[warp - 1][lane] = make_float4(v[0], v[1], v[2], v[3]);
+    __syncthreads();
+    if (warp) return;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) add4(v, sum[i][lane]);
+    few_rotate_back(v, lane);
+    ep.finish(a, row, col, v);
+}
+
+static size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
+
+static FewRun linear_run(int M, int k, int n, int G, int sms) {
+    return FewRun(k >> 7, (n >> 7) * ((M + 8 * G - 1) / (8 * G)), sms);
+}
+
+// Workspace of the few-rows path, laid out at ws.
+static size_t few_layout(FewScratch* w, int M, int k, int n, int G, int sms, uint8_t* ws) {
+    const FewRun run = linear_run(M, k, n, G, sms);
+    size_t off = 0;
+    auto take = [&](size_t bytes) { const size_t o = off; off += up256(bytes); return ws + o; };
+    w->park = reinterpret_cast<float*>(take(few_park_bytes(run.units, run.ctas, G)));
+    w->xh = take((size_t)run.kb * M * kRowBytes);
+    w->inv = reinterpret_cast<float*>(take((size_t)run.kb * M * 4));
+    return off;
 }
 
 template <int CODE, int G>
-static int launch_few(const LinearArgs& a, int S, cudaStream_t stream) {
-    const size_t smem = few_smem(a.K, G, a.k >> 7, S);
-    auto kern = linear_few_kernel<CODE, G>;
-    if (check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        227 * 1024), "cudaFuncSetAttribute(linear_few)"))
-        return RC_DEVICE_ERROR;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(S, a.n >> 7, (a.M + 8 * G - 1) / (8 * G));
-    cfg.blockDim = dim3(32 * kFewWarps);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = S;
-    at[0].val.clusterDim.y = 1;
-    at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a);
-    note_launch();
-    return check_cuda(e, "linear_few launch") ? RC_DEVICE_ERROR : RC_OK;
+static int few_launch(const LinearArgs& a, int sms, uint8_t* ws, cudaStream_t stream) {
+    FewScratch w;
+    few_layout(&w, a.M, a.k, a.n, G, sms, ws);
+    const FewRun run = linear_run(a.M, a.k, a.n, G, sms);
+    const dim3 fin(a.n >> 7, a.M);
+    int rc;
+    if (a.M <= 2) {            // rotated where they are used: cheaper than a launch
+        rc = launch_kernel(linear_few_kernel<CODE, G, true>, "linear_few launch", dim3(run.ctas),
+                           32 * kFewWarps, few_smem(a.K), false, stream, a, w, run);
+    } else {
+        rc = launch_kernel(linear_rotate_kernel, "linear_rotate launch", dim3((run.kb * a.M + 3) / 4),
+                           128, 0, false, stream, a, w);
+        if (rc) return rc;
+        rc = launch_kernel(linear_few_kernel<CODE, G, false>, "linear_few launch", dim3(run.ctas),
+                           32 * kFewWarps, few_smem(a.K), true, stream, a, w, run);
+    }
+    if (rc) return rc;
+    return launch_kernel(linear_finish_kernel<G>, "linear_finish launch", fin, 128, 0, true, stream, a,
+                         w, run);
 }
 
-static int few_run(const LinearArgs& a, int sms, cudaStream_t stream) {
-    const int G = a.M > 8 ? 2 : 1;
-    const int kb = a.k >> 7, units = (a.n >> 7) * ((a.M + 8 * G - 1) / (8 * G));
-    int S = 1;
-    while (S < 8 && 2 * S <= kb && units * S < 2 * sms) S *= 2;
-    while (S < 8 && S < kb && few_smem(a.K, G, kb, S) > 200 * 1024) S *= 2;
-    if (S > kb) S = kb;
-    if (few_smem(a.K, G, kb, S) > 227 * 1024) {
-        set_error("linear: in = %d is too long for %d rows", a.k, a.M);
-        return RC_BAD_REQUEST;
-    }
-#define EXL3B_FEW(C) (G == 1 ? launch_few<C, 1>(a, S, stream) : launch_few<C, 2>(a, S, stream))
+static int few_groups(int M) { return M > 8 ? 2 : 1; }
+
+static int few_dispatch(const LinearArgs& a, int sms, uint8_t* ws, cudaStream_t stream) {
+    const int G = few_groups(a.M);
+#define EXL3B_FEW(C) (G == 1 ? few_launch<C, 1>(a, sms, ws, stream) : few_launch<C, 2>(a, sms, ws, stream))
     switch (a.code) {
         case CODE_MUL1: return EXL3B_FEW(CODE_MUL1);
         case CODE_3INST: return EXL3B_FEW(CODE_3INST);
@@ -186,9 +207,11 @@ int check_rows(const char* what, const void* p, int64_t ld, int rows, int cols) 
 extern "C" {
 
 size_t exl3b_linear_workspace_bytes(int M, int k, int n) {
-    (void)n;
-    if (M <= 0 || k <= 0) return 0;
-    return 0;
+    if (M <= 0 || k <= 0 || n <= 0 || k % 128 || n % 128) return 0;
+    const int sms = device_sms();
+    if (sms <= 0) return 0;
+    FewScratch w;
+    return few_layout(&w, M, k, n, few_groups(M), sms, nullptr);
 }
 
 int exl3b_linear(const void* dX, int dtype, int64_t ldx, int M, int k, int n,
@@ -216,17 +239,17 @@ int exl3b_linear(const void* dX, int dtype, int64_t ldx, int M, int k, int n,
         (d_mul && check_rows("linear: mul", d_mul, ldmul, M, n)) ||
         (d_residual && check_rows("linear: residual", d_residual, ldres, M, n)))
         return RC_BAD_REQUEST;
+    DeviceState* st;
+    if (device_state(&st)) { set_error("no usable CUDA device"); return RC_NO_DEVICE; }
     const size_t need = exl3b_linear_workspace_bytes(M, k, n);
     if (need && (!ws || ws_bytes < need || !aligned(ws, 256))) {
         set_error("linear: workspace %zu < %zu bytes or misaligned", ws_bytes, need);
         return RC_WORKSPACE;
     }
-    DeviceState* st;
-    if (device_state(&st)) { set_error("no usable CUDA device"); return RC_NO_DEVICE; }
     LinearArgs a = {dX, ldx, dtype, M, k, n, reinterpret_cast<const uint8_t*>(dTrellis), K, code,
                     static_cast<const __half*>(d_suh_f16), static_cast<const __half*>(d_svh_f16),
                     d_bias, act, d_mul, ldmul, d_residual, ldres, dOut, ldo};
-    return few_run(a, st->sms, static_cast<cudaStream_t>(stream));
+    return few_dispatch(a, st->sms, static_cast<uint8_t*>(ws), static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

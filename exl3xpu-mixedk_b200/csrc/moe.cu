@@ -2,15 +2,17 @@
 //   l = x R^T;  S = the top_k largest l (ties: lowest index);  p = softmax(l)
 //   y = sum_{e in S} w_e ((silu(x Wg_e) * (x Wu_e)) Wd_e) + residual,  w = p or p / sum_S p
 //
-// Three launches: the router (logits, choice, weights), gate and up of every chosen
-// expert down to the down projection's rotated operand, and the down projection with
-// the weighted sum.  Each chosen expert's tensors are read once for all of its tokens
-// (up to 8 G at a time); the work is bound by their decode, as in forward_few.cuh.
-// Nothing depends on the order in which CTAs run: partial sums are joined in rank
-// order and a token's experts in the order of their choice.
+// The router (logits, choice, weights, and the chosen experts' rotations of the
+// token), then the gate and up products of every chosen expert, the down products, and
+// after each a kernel that joins the parked sums: to the down projection's rotated
+// rows, and to the weighted sum.  Every launch but the first overlaps the one before
+// it.  Each chosen expert's tensors are read once for 8 G of its tokens; the work is
+// bound by their decode, spread evenly over the SMs as in forward_few.cuh.  Nothing depends on
+// the order in which CTAs run: partial sums are added in a fixed order, and a token's
+// experts in the order of their choice.
 #include <cooperative_groups.h>
+#include <utility>
 
-#include "exl3b_internal.h"
 #include "forward_few.cuh"
 #include "../../include/exl3b200.h"
 
@@ -19,8 +21,9 @@ namespace cg = cooperative_groups;
 namespace exl3b {
 
 constexpr int kMaxExperts = 1024;
-constexpr int kMaxTokens = 256;           // of one call: bounds the token list of an expert
+constexpr int kMaxTokens = 256;
 constexpr int kMaxTopK = 32;
+constexpr int kMaxPairs = 2048;           // (token, choice) pairs of one call
 
 struct MoeArgs {
     const void* x;
@@ -37,12 +40,15 @@ struct MoeArgs {
     void* out;
     int64_t ldo;
     // workspace
+    int slots_max;                        // experts x groups of 8 G rows at most
     int* ids;                             // [T * top_k]
     float* wts;                           // [T * top_k]
-    int* arrived;                         // [T][D / 128]
-    uint8_t* xh;                          // [T * top_k][F] fp16, few_put_block order
-    float* inv;                           // [T * top_k][F / 128]
-    float* part;                          // [T * top_k][D]
+    int* place;                           // [1 + T * top_k]: slots, then slot << 8 | row of a pair
+    uint8_t* xh1;                         // [2][T * top_k][D / 128][256], few_put_block order
+    float* inv1;
+    uint8_t* xh2;                         // [T * top_k][F / 128][256]
+    float* inv2;
+    float* park;
 };
 
 // ------------------------------------------------------------------ router
@@ -87,28 +93,62 @@ __device__ __forceinline__ double dot8(const MoeArgs& a, const uint4& xv, size_t
     return s;
 }
 
-// Cluster (8 CTAs) per token: 64 warps share the experts, rank 0 chooses.
+// An order on fp64 values as integers; NaN counts as largest (its weights are NaN
+// whatever is chosen).
+__device__ __forceinline__ long long order_key(double v) {
+    if (v != v) return 0x7FFFFFFFFFFFFFFFLL;
+    const long long b = __double_as_longlong(v == 0.0 ? 0.0 : v);
+    return b < 0 ? b ^ 0x7FFFFFFFFFFFFFFFLL : b;
+}
+
+__device__ __forceinline__ uint32_t peer(const void* p, int rank) {
+    uint32_t addr;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;"
+        : "=r"(addr) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    return addr;
+}
+
+// Cluster (8 CTAs) per token.  Its 64 warps share the experts' logits, which go to
+// every CTA; the CTAs share the experts again to find their place in the order (the
+// number of larger logits, and of equal ones before); an expert placed below top_k is
+// chosen.  Then all rotate the token for the chosen experts.
 __global__ void __cluster_dims__(kRouterRanks, 1, 1) __launch_bounds__(256)
 moe_router_kernel(const MoeArgs a) {
     __shared__ double logit[kMaxExperts];
+    __shared__ int chosen[kMaxTopK];
+    __shared__ float share[kMaxTopK];
+    pdl_launch();
     cg::cluster_group cl = cg::this_cluster();
-    const int rank = cl.block_rank(), token = blockIdx.y;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    cl.sync();                               // rank 0 runs: its shared memory may be written
-    double* l0 = cl.map_shared_rank(logit, 0);
+    auto started = cl.barrier_arrive();
+    const int rank = cl.block_rank(), token = blockIdx.y, t = threadIdx.x;
+    const int warp = t >> 5, lane = t & 31;
     const uint4* xr = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) + token * a.ldx);
-    for (int e = rank * 8 + warp; e < a.E; e += 8 * kRouterRanks) {
-        double s = 0.0;
-        for (int c = lane; c < a.D / 8; c += 32) s += dot8(a, xr[c], (size_t)e * a.ldr + 8 * c);
+    bool wait = true;
+    for (int e0 = rank * 8 + warp; e0 < a.E; e0 += 16 * kRouterRanks) {
+        const int e1 = e0 + 8 * kRouterRanks;
+        const bool two = e1 < a.E;
+        double s0 = 0.0, s1 = 0.0;
+#pragma unroll 4
+        for (int c = lane; c < a.D / 8; c += 32) {
+            const uint4 xv = xr[c];
+            s0 += dot8(a, xv, (size_t)e0 * a.ldr + 8 * c);
+            if (two) s1 += dot8(a, xv, (size_t)e1 * a.ldr + 8 * c);
+        }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0) l0[e] = s;
+        for (int o = 16; o > 0; o >>= 1) {
+            s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+            s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+        }
+        if (wait) { cl.barrier_wait(std::move(started)); wait = false; }   // the others run
+        if (lane < kRouterRanks) {
+            asm volatile("st.shared::cluster.f64 [%0], %1;" :: "r"(peer(logit + e0, lane)), "d"(s0) : "memory");
+            if (two)
+                asm volatile("st.shared::cluster.f64 [%0], %1;" :: "r"(peer(logit + e1, lane)), "d"(s1) : "memory");
+        }
     }
-    for (int i = rank * 256 + threadIdx.x; i < a.D / 128; i += 256 * kRouterRanks)
-        a.arrived[(size_t)token * (a.D / 128) + i] = 0;
+    if (wait) cl.barrier_wait(std::move(started));
     cl.sync();
-    if (rank != 0 || warp != 0) return;
-    // largest logit, softmax sum
+    // largest logit and softmax sum, in every warp
     double m = -INFINITY;
     for (int e = lane; e < a.E; e += 32) m = fmax(m, logit[e]);
 #pragma unroll
@@ -117,356 +157,301 @@ moe_router_kernel(const MoeArgs a) {
     for (int e = lane; e < a.E; e += 32) sum += expf((float)(logit[e] - m));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    // top_k rounds of (largest value, then lowest index); a NaN counts as largest (its
-    // weights are NaN whatever is chosen), a chosen entry is marked by its lane
-    uint32_t taken = 0;                      // bit i: entry lane + 32 i
-    float my_w = 0.0f, picked = 0.0f;
-    int my_id = 0;
-    for (int j = 0; j < a.top_k; ++j) {
-        double best = -INFINITY;
-        int bi = kMaxExperts;
-        for (int i = 0; lane + 32 * i < a.E; ++i) {
-            if (taken >> i & 1) continue;
-            const double v = logit[lane + 32 * i];
-            const double key = v != v ? INFINITY : v;
-            if (bi == kMaxExperts || key > best) { best = key; bi = lane + 32 * i; }
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const double ov = __shfl_xor_sync(0xffffffffu, best, o);
-            const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
-            if (oi != kMaxExperts && (bi == kMaxExperts || ov > best || (ov == best && oi < bi))) {
-                best = ov;
-                bi = oi;
+    // 8 lanes count for one expert
+    for (int e = rank * 32 + (t >> 3); e - (t >> 3) < a.E; e += 32 * kRouterRanks) {
+        int place = 0;
+        if (e < a.E) {
+            const long long mine = order_key(logit[e]);
+            for (int o = t & 7; o < a.E; o += 8) {
+                const long long k = order_key(logit[o]);
+                place += k > mine || (k == mine && o < e);
             }
         }
-        if ((bi & 31) == lane) taken |= 1u << (bi >> 5);
-        const float p = expf((float)(logit[bi] - m)) / sum;
-        picked += p;
-        if (lane == j) { my_w = p; my_id = bi; }
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+        if (e < a.E && place < a.top_k) {
+            const float p = expf((float)(logit[e] - m)) / sum;
+            asm volatile("st.shared::cluster.s32 [%0], %1;" :: "r"(peer(chosen + place, t & 7)), "r"(e) : "memory");
+            asm volatile("st.shared::cluster.f32 [%0], %1;" :: "r"(peer(share + place, t & 7)), "f"(p) : "memory");
+        }
     }
-    if (lane < a.top_k) {
-        a.ids[token * a.top_k + lane] = my_id;
-        a.wts[token * a.top_k + lane] = a.normalize ? my_w / picked : my_w;
+    cl.sync();
+    if (rank == 0 && t < a.top_k) {
+        float all = 0.0f;
+        for (int j = 0; j < a.top_k; ++j) all += share[j];
+        a.ids[token * a.top_k + t] = chosen[t];
+        a.wts[token * a.top_k + t] = a.normalize ? share[t] / all : share[t];
+    }
+    // rotate the token for gate and up of every chosen expert
+    const int kd = a.D >> 7, P = a.T * a.top_k;
+#pragma unroll 2
+    for (int i = rank * 8 + warp; i < 2 * a.top_k * kd; i += 8 * kRouterRanks) {
+        const int m2 = i & 1, j = (i >> 1) % a.top_k, b = (i >> 1) / a.top_k, k = b * 128 + 4 * lane;
+        const exl3b_expert* w = a.experts + (size_t)m2 * a.E + chosen[j];
+        float v[4], s[4];
+        load4x(a.x, (size_t)token * a.ldx + k, a.dtype, v);
+        load4(static_cast<const __half*>(w->suh) + k, s);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c] *= s[c];
+        const size_t to = ((size_t)m2 * P + token * a.top_k + j) * kd + b;
+        few_put_block(v, a.xh1 + to * kRowBytes, a.inv1 + to, lane, 0);
     }
 }
 
 // ------------------------------------------------------------------ experts
-// The slot-th chosen expert (ascending), and its (token, choice) pairs in order.
-struct ExpertTokens {
-    uint32_t bits[kMaxExperts / 32];
-    int pair[kMaxTokens];
-    int count;
+// The chosen experts in ascending order, each cut into slots of up to 8 G of its
+// (token, choice) pairs, which are in ascending order too; with the tensors of the
+// slots' experts, so that the product need not fetch them.
+struct Plan {
+    int* pair;                 // [P]
+    int2* slot;                // {expert, first pair << 8 | rows}
+    const uint8_t** tiles;     // [kinds][slots]
+    int* K;                    // [kinds][slots]
+    int slots;
 };
 
-// Returns the expert, or -1 when fewer than slot + 1 were chosen.  All threads.
-__device__ __forceinline__ int find_expert(const MoeArgs& a, int slot, ExpertTokens& s) {
+__host__ __device__ inline int plan_bytes(int P, int slots_max, int kinds) {
+    return (P * 4 + 7) / 8 * 8 + slots_max * (8 + 12 * kinds);
+}
+
+// For tensors `first` .. first + kinds - 1 of every expert.  `tmp`: room for P + E ints.
+// `place`: where to note the pairs' slots (nullable).  All threads.
+template <int G>
+__device__ __forceinline__ Plan make_plan(const MoeArgs& a, int first, int kinds, uint8_t* where,
+                                          int* tmp, int* place) {
+    __shared__ int nslots;
     const int t = threadIdx.x, P = a.T * a.top_k;
-    if (t < kMaxExperts / 32) s.bits[t] = 0;
+    Plan p;
+    p.pair = reinterpret_cast<int*>(where);
+    p.slot = reinterpret_cast<int2*>(where + (P * 4 + 7) / 8 * 8);
+    p.tiles = reinterpret_cast<const uint8_t**>(p.slot + a.slots_max);
+    p.K = reinterpret_cast<int*>(p.tiles + kinds * a.slots_max);
+    int* count = tmp + P;
+    for (int i = t; i < P; i += blockDim.x) tmp[i] = a.ids[i];
     __syncthreads();
-    for (int i = t; i < P; i += blockDim.x) {
-        const int e = a.ids[i];
-        atomicOr(&s.bits[e >> 5], 1u << (e & 31));
+    for (int e = t; e < a.E; e += blockDim.x) {
+        int c = 0;
+        for (int i = 0; i < P; ++i) c += tmp[i] == e;
+        count[e] = c;
     }
     __syncthreads();
-    int e = -1, left = slot;
-    for (int w = 0; w < kMaxExperts / 32; ++w) {
-        const uint32_t b = s.bits[w];
-        const int c = __popc(b);
-        if (left < c) {
-            uint32_t r = b;
-            for (int i = 0; i < left; ++i) r &= r - 1;
-            e = 32 * w + __ffs(r) - 1;
-            break;
+    if (t < 32) {              // running sums of pairs (low half) and slots (high half)
+        int sum = 0;
+        for (int base = 0; base < a.E; base += 32) {
+            const int c = base + t < a.E ? count[base + t] : 0;
+            const int mine = c | ((c + 8 * G - 1) / (8 * G)) << 16;
+            int run = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, run, o);
+                if (t >= o) run += up;
+            }
+            if (base + t < a.E) count[base + t] = sum + run - mine;
+            sum += __shfl_sync(0xffffffffu, run, 31);
         }
-        left -= c;
-    }
-    if (e < 0) return -1;
-    if (t < 32) {
-        int n = 0;
-        for (int base = 0; base < P; base += 32) {
-            const bool hit = base + t < P && a.ids[base + t] == e;
-            const uint32_t m = __ballot_sync(0xffffffffu, hit);
-            if (hit) s.pair[n + __popc(m & ((1u << t) - 1))] = base + t;
-            n += __popc(m);
+        if (t == 0) {
+            nslots = sum >> 16;
+            if (place) place[0] = nslots;
         }
-        if (t == 0) s.count = n;
     }
     __syncthreads();
-    return e;
+    p.slots = nslots;
+    for (int e = t; e < a.E; e += blockDim.x) {
+        const int from = count[e] & 0xFFFF;
+        int at = from, slot = count[e] >> 16;
+        for (int i = 0; i < P; ++i)
+            if (tmp[i] == e) {
+                if (place) place[1 + i] = (slot + (at - from) / (8 * G)) << 8 | (at - from) % (8 * G);
+                p.pair[at++] = i;
+            }
+        for (int r = from; r < at; r += 8 * G, ++slot) {
+            p.slot[slot] = make_int2(e, r << 8 | min(8 * G, at - r));
+            for (int m = 0; m < kinds; ++m) {
+                const exl3b_expert* w = a.experts + (size_t)(first + m) * a.E + e;
+                p.tiles[m * p.slots + slot] = static_cast<const uint8_t*>(w->trellis);
+                p.K[m * p.slots + slot] = min(max(w->K, 2), a.Kmax[first + m]);
+            }
+        }
+    }
+    __syncthreads();
+    return p;
 }
 
-struct MoeShare { int b0, nblk, maxblk; };
+// Units: (tensor, slot, column block); rows: rotated rows of the pairs.
+template <int G>
+struct ExpertJob {
+    static constexpr bool kRotate = false;
+    const MoeArgs& a;
+    const Plan& p;
+    const uint8_t* x;          // [kinds][P][kb][256]
+    const float* s;
+    int kb, cols;              // blocks of a row, column blocks
+    bool early;                // the rows are there already
+    __device__ __forceinline__ FewUnit unit(int u) const {
+        const int v = u / cols, K = p.K[v];
+        return {p.tiles[v] + (size_t)(u - v * cols) * 256 * K, (uint32_t)cols * 256 * K, K};
+    }
+    __device__ __forceinline__ int rows(int u) const { return p.slot[u / cols % p.slots].y & 0xFF; }
+    __device__ __forceinline__ size_t row(int u, int r, int b) const {
+        const int v = u / cols, m = v / p.slots;
+        return ((size_t)m * a.T * a.top_k + p.pair[(p.slot[v - m * p.slots].y >> 8) + r]) * kb + b;
+    }
+    __device__ __forceinline__ const uint8_t* xh() const { return x; }
+    __device__ __forceinline__ const float* inv() const { return s; }
+    __device__ __forceinline__ void wait() const { if (!early) pdl_wait(); }
+};
 
-__device__ __forceinline__ MoeShare share_of(int kb, int rank, int nrank) {
-    MoeShare s;
-    s.b0 = (int)((long long)kb * rank / nrank);
-    s.nblk = (int)((long long)kb * (rank + 1) / nrank) - s.b0;
-    s.maxblk = (kb + nrank - 1) / nrank;
-    return s;
-}
-
-// gate and up of one expert, 128 columns of F, the share of D of this rank; then
-// h = silu(g) * u and the down projection's operand, rotated and rounded.
 template <int CODE, int G>
-__global__ void __launch_bounds__(32 * kFewWarps, 2) moe_gate_up_kernel(const MoeArgs a) {
+__global__ void __launch_bounds__(32 * kFewWarps, 1) moe_gate_up_kernel(const MoeArgs a) {
     extern __shared__ __align__(16) uint8_t sm[];
-    __shared__ ExpertTokens et;
-    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-    const int nrank = gridDim.x, rank = blockIdx.x, fb = blockIdx.y;
-    const int e = find_expert(a, blockIdx.z, et);
-    if (e < 0) return;                        // the whole cluster
-    const exl3b_expert w[2] = {a.experts[e], a.experts[a.E + e]};
-    const exl3b_expert down = a.experts[2 * a.E + e];
-    if (w[0].K < 2 || w[0].K > a.Kmax[0] || w[1].K < 2 || w[1].K > a.Kmax[1]) return;
-    const MoeShare sh = share_of(a.D >> 7, rank, nrank);
-    const int xpitch = few_row_bytes(sh.maxblk);
-    uint8_t* ring[2];
-    ring[0] = sm + warp * few_ring_bytes(a.Kmax[0]);
-    uint8_t* p = sm + kFewWarps * few_ring_bytes(a.Kmax[0]);
-    ring[1] = p + warp * few_ring_bytes(a.Kmax[1]);
-    p += kFewWarps * few_ring_bytes(a.Kmax[1]);
-    uint8_t* xh = p;                                            // [2][8 G] rows
-    float* inv = reinterpret_cast<float*>(xh + 16 * G * xpitch);     // [2][maxblk][8 G]
-    float* part = inv + 16 * G * sh.maxblk;                     // [2][8 G][kPartPitch]
-    const int tn = a.F >> 4;
-    const int count = et.count;
-    for (int r0 = 0; r0 < count; r0 += 8 * G) {
-        const int rows = min(8 * G, count - r0);
-        const uint8_t* src[2];
-        size_t kt_bytes[2];
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            kt_bytes[m] = (size_t)tn * 32 * w[m].K;
-            src[m] = static_cast<const uint8_t*>(w[m].trellis) + (size_t)sh.b0 * 8 * kt_bytes[m] +
-                     (size_t)(fb * 8 + warp) * 32 * w[m].K;
-            few_prologue(src[m], kt_bytes[m], w[m].K, sh.nblk, ring[m], lane);
-        }
-        for (int i = warp; i < sh.nblk * 8 * G; i += kFewWarps) {
-            const int r = i % (8 * G), b = i / (8 * G);
-            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            const int k = (sh.b0 + b) * 128 + 4 * lane;
-            if (r < rows)
-                load4x(a.x, (size_t)(et.pair[r0 + r] / a.top_k) * a.ldx + k, a.dtype, x);
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                float v[4], s[4];
-                load4(static_cast<const __half*>(w[m].suh) + k, s);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = x[j] * s[j];
-                few_put_block(v, xh + (m * 8 * G + r) * xpitch + b * 256,
-                              inv + m * 8 * G * sh.maxblk + i, lane);
-            }
-        }
-        __syncthreads();
-        float acc[G][4];
-        // the up ring's first blocks were issued before the gate's later ones, so the
-        // group count that few_product waits for covers both
-        for (int m = 0; m < 2; ++m) {
-#pragma unroll
-            for (int g = 0; g < G; ++g) acc[g][0] = acc[g][1] = acc[g][2] = acc[g][3] = 0.0f;
-            few_product_k<CODE, G>(w[m].K, src[m], kt_bytes[m], sh.nblk, ring[m],
-                                   xh + m * 8 * G * xpitch, xpitch, inv + m * 8 * G * sh.maxblk, acc,
-                                   lane);
-            few_store_part<G>(part + m * 8 * G * kPartPitch, acc, warp, lane);
-        }
-        if (nrank > 1) cg::this_cluster().sync();
-        else __syncthreads();
-        for (int r = rank + nrank * warp; r < rows; r += nrank * kFewWarps) {
-            float g[4], u[4], s[4];
-            const int f = fb * 128 + 4 * lane;
-            few_sum_row(part, r, nrank, lane, g);
-            few_sum_row(part + 8 * G * kPartPitch, r, nrank, lane, u);
-            load4(static_cast<const __half*>(w[0].svh) + f, s);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) g[j] = silu_f(g[j] * s[j]);
-            load4(static_cast<const __half*>(w[1].svh) + f, s);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) g[j] *= u[j] * s[j];
-            load4(static_cast<const __half*>(down.suh) + f, s);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) g[j] *= s[j];
-            const size_t pair = et.pair[r0 + r];
-            few_put_block(g, a.xh + (pair * (a.F >> 7) + fb) * 256,
-                          a.inv + pair * (a.F >> 7) + fb, lane);
-        }
-        if (nrank > 1) cg::this_cluster().sync();
-        else __syncthreads();
-    }
+    const int Kmax = max(a.Kmax[0], a.Kmax[1]);
+    pdl_wait();
+    pdl_launch();              // from here on the router's results are there for everyone
+    const Plan p = make_plan<G>(a, 0, 2, sm + few_smem(Kmax), reinterpret_cast<int*>(sm),
+                                blockIdx.x == 0 ? a.place : nullptr);
+    const FewRun run(a.D >> 7, 2 * p.slots * (a.F >> 7), gridDim.x);
+    if (blockIdx.x >= run.ctas) return;
+    const ExpertJob<G> job = {a, p, a.xh1, a.inv1, a.D >> 7, a.F >> 7, true};
+    few_run<CODE, G>(job, run, Kmax, sm, a.park);
 }
 
-// down of one expert, 128 columns of D, the share of F of this rank.  A finished
-// (token, choice) row is weighted and parked; whoever parks a token's last row adds
-// them up in the order of choice and writes the output.
 template <int CODE, int G>
-__global__ void __launch_bounds__(32 * kFewWarps, 2) moe_down_kernel(const MoeArgs a) {
+__global__ void __launch_bounds__(32 * kFewWarps, 1) moe_down_kernel(const MoeArgs a) {
     extern __shared__ __align__(16) uint8_t sm[];
-    __shared__ ExpertTokens et;
-    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-    const int nrank = gridDim.x, rank = blockIdx.x, nb = blockIdx.y;
-    const int e = find_expert(a, blockIdx.z, et);
-    if (e < 0) return;
-    const exl3b_expert w = a.experts[2 * a.E + e];
-    if (w.K < 2 || w.K > a.Kmax[2]) return;
-    const MoeShare sh = share_of(a.F >> 7, rank, nrank);
-    const int xpitch = few_row_bytes(sh.maxblk), fbn = a.F >> 7, nbn = a.D >> 7;
-    uint8_t* ring = sm + warp * few_ring_bytes(a.Kmax[2]);
-    uint8_t* xh = sm + kFewWarps * few_ring_bytes(a.Kmax[2]);
-    float* inv = reinterpret_cast<float*>(xh + 8 * G * xpitch);
-    float* part = inv + 8 * G * sh.maxblk;
-    const int tn = a.D >> 4;
-    const size_t kt_bytes = (size_t)tn * 32 * w.K;
-    const uint8_t* src = static_cast<const uint8_t*>(w.trellis) + (size_t)sh.b0 * 8 * kt_bytes +
-                         (size_t)(nb * 8 + warp) * 32 * w.K;
-    const int count = et.count;
-    for (int r0 = 0; r0 < count; r0 += 8 * G) {
-        const int rows = min(8 * G, count - r0);
-        few_prologue(src, kt_bytes, w.K, sh.nblk, ring, lane);
-        // 16 lanes copy one block of one row
-        for (int i = t >> 4; i < sh.nblk * 8 * G; i += 2 * kFewWarps) {
-            const int r = i % (8 * G), b = i / (8 * G), c = t & 15;
-            uint4 v = {0u, 0u, 0u, 0u};
-            float s = 1.0f;
-            if (r < rows) {
-                const size_t blk = (size_t)et.pair[r0 + r] * fbn + sh.b0 + b;
-                v = *reinterpret_cast<const uint4*>(a.xh + blk * 256 + 16 * c);
-                s = a.inv[blk];
-            }
-            *reinterpret_cast<uint4*>(xh + r * xpitch + b * 256 + 16 * c) = v;
-            if (c == 0) inv[i] = s;
-        }
-        __syncthreads();
-        float acc[G][4];
-#pragma unroll
-        for (int g = 0; g < G; ++g) acc[g][0] = acc[g][1] = acc[g][2] = acc[g][3] = 0.0f;
-        few_product_k<CODE, G>(w.K, src, kt_bytes, sh.nblk, ring, xh, xpitch, inv, acc, lane);
-        few_store_part<G>(part, acc, warp, lane);
-        if (nrank > 1) cg::this_cluster().sync();
-        else __syncthreads();
-        for (int r = rank + nrank * warp; r < rows; r += nrank * kFewWarps) {
-            float v[4], s[4];
-            const int col = nb * 128 + 4 * lane, pair = et.pair[r0 + r], token = pair / a.top_k;
-            few_sum_row(part, r, nrank, lane, v);
-            load4(static_cast<const __half*>(w.svh) + col, s);
-            const float wt = a.wts[pair];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] *= s[j] * wt;
-            __stcg(reinterpret_cast<float4*>(a.part + (size_t)pair * a.D + col),
-                   make_float4(v[0], v[1], v[2], v[3]));
-            __threadfence();
-            __syncwarp();
-            int n = 0;
-            if (lane == 0) n = atomicAdd(a.arrived + (size_t)token * nbn + nb, 1) + 1;
-            n = __shfl_sync(0xffffffffu, n, 0);
-            if (n != a.top_k) continue;
-            __threadfence();
-            v[0] = v[1] = v[2] = v[3] = 0.0f;
-            for (int j = 0; j < a.top_k; ++j) {
-                const float4 f = __ldcg(reinterpret_cast<const float4*>(
-                    a.part + ((size_t)token * a.top_k + j) * a.D + col));
-                v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
-            }
-            if (a.residual) {
-                load4x(a.residual, (size_t)token * a.ldres + col, a.dtype, s);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] += s[j];
-            }
-            store4x(a.out, (size_t)token * a.ldo + col, a.dtype, v);
-        }
-        if (nrank > 1) cg::this_cluster().sync();
-        else __syncthreads();
+    pdl_launch();
+    const Plan p = make_plan<G>(a, 2, 1, sm + few_smem(a.Kmax[2]), reinterpret_cast<int*>(sm), nullptr);
+    const FewRun run(a.F >> 7, p.slots * (a.D >> 7), gridDim.x);
+    if (blockIdx.x >= run.ctas) return;
+    const ExpertJob<G> job = {a, p, a.xh2, a.inv2, a.F >> 7, a.D >> 7, false};
+    few_run<CODE, G>(job, run, a.Kmax[2], sm, a.park);
+}
+
+// h = silu(gate) * up of a (pair, column block of F), and the down projection's rotated
+// row: a CTA each; two warps add the gate's parked sums, two those of up.
+template <int G>
+__global__ void __launch_bounds__(128) moe_gate_up_finish_kernel(const MoeArgs a, int ctas) {
+    __shared__ float4 sum[3][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int fb = blockIdx.x, pair = blockIdx.y, f = fb * 128 + 4 * lane, fbn = gridDim.x;
+    pdl_wait();
+    pdl_launch();
+    const int e = a.ids[pair], slots = a.place[0], at = a.place[1 + pair];
+    float sg[4], su[4], sd[4], v[4];
+    if (warp == 0) {
+        load4(static_cast<const __half*>(a.experts[e].svh) + f, sg);
+        load4(static_cast<const __half*>(a.experts[a.E + e].svh) + f, su);
+        load4(static_cast<const __half*>(a.experts[2 * a.E + e].suh) + f, sd);
     }
+    const FewRun run(a.D >> 7, 2 * slots * fbn, ctas);
+    few_sum<G>(a.park, run, ((warp >> 1) * slots + (at >> 8)) * fbn + fb, at & 0xFF, lane, warp & 1, 2, v);
+    if (warp) sum[warp - 1][lane] = make_float4(v[0], v[1], v[2], v[3]);
+    __syncthreads();
+    if (warp) return;
+    add4(v, sum[0][lane]);
+    float h[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    add4(h, sum[1][lane]);
+    add4(h, sum[2][lane]);
+    few_rotate_back(v, lane);
+    few_rotate_back(h, lane);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = silu_f(v[j] * sg[j]) * (h[j] * su[j]) * sd[j];
+    const size_t to = (size_t)pair * fbn + fb;
+    few_put_block(v, a.xh2 + to * kRowBytes, a.inv2 + to, lane, 0);
+}
+
+// Weighted sum over a token's experts of one column block, and the residual: a CTA
+// each, whose four warps take every fourth expert in the order of choice.
+template <int G>
+__global__ void __launch_bounds__(128) moe_down_finish_kernel(const MoeArgs a, int ctas) {
+    __shared__ float4 sum[3][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int nb = blockIdx.x, token = blockIdx.y, n = nb * 128 + 4 * lane, nbn = gridDim.x;
+    float res[4] = {0.0f, 0.0f, 0.0f, 0.0f}, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (warp == 0 && a.residual) load4x(a.residual, (size_t)token * a.ldres + n, a.dtype, res);
+    pdl_wait();
+    const FewRun run(a.F >> 7, a.place[0] * nbn, ctas);
+    for (int j = warp; j < a.top_k; j += 4) {
+        const int pair = token * a.top_k + j, at = a.place[1 + pair];
+        float v[4], s[4];
+        load4(static_cast<const __half*>(a.experts[2 * a.E + a.ids[pair]].svh) + n, s);
+        const float wt = a.wts[pair];
+        few_sum<G>(a.park, run, (at >> 8) * nbn + nb, at & 0xFF, lane, 0, 1, v);
+        few_rotate_back(v, lane);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) y[c] = fmaf(v[c], s[c] * wt, y[c]);
+    }
+    if (warp) sum[warp - 1][lane] = make_float4(y[0], y[1], y[2], y[3]);
+    __syncthreads();
+    if (warp) return;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) add4(y, sum[i][lane]);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) y[c] += res[c];
+    store4x(a.out, (size_t)token * a.ldo + n, a.dtype, y);
 }
 
 // ------------------------------------------------------------------ host side
 static size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 
-static size_t moe_layout(MoeArgs* a, int T, int D, int F, int top_k, uint8_t* ws) {
-    const size_t P = (size_t)T * top_k;
+// Groups of 16 rows where an expert has more than 8 tokens on average; below that the
+// few experts with more are read twice, which costs less than twice the rows for all.
+static int moe_groups(int T, int E, int top_k) { return T * top_k > 8 * E ? 2 : 1; }
+
+// Slots at most: every pair's expert its own, plus the full groups beyond the first.
+static int moe_slots(int T, int E, int top_k) {
+    const int P = T * top_k, rows = 8 * moe_groups(T, E, top_k);
+    return (P < E ? P : E) + P / rows;
+}
+
+static size_t moe_layout(MoeArgs* a, int T, int D, int F, int E, int top_k, int sms, uint8_t* ws) {
+    const size_t P = (size_t)T * top_k, kd = D / 128, kf = F / 128;
+    const int slots = moe_slots(T, E, top_k), G = moe_groups(T, E, top_k);
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t o = off; off += up256(bytes); return ws + o; };
+    const size_t park1 = few_park_bytes((int)(2 * slots * kf), sms, G);
+    const size_t park2 = few_park_bytes((int)(slots * kd), sms, G);
     uint8_t* ids = take(P * 4);
     uint8_t* wts = take(P * 4);
-    uint8_t* arrived = take((size_t)T * (D / 128) * 4);
-    uint8_t* xh = take(P * F * 2);
-    uint8_t* inv = take(P * (F / 128) * 4);
-    uint8_t* part = take(P * D * 4);
+    uint8_t* place = take((1 + P) * 4);
+    uint8_t* xh1 = take(2 * P * kd * kRowBytes);
+    uint8_t* inv1 = take(2 * P * kd * 4);
+    uint8_t* xh2 = take(P * kf * kRowBytes);
+    uint8_t* inv2 = take(P * kf * 4);
+    uint8_t* park = take(park1 > park2 ? park1 : park2);
     if (a) {
+        a->slots_max = slots;
         a->ids = reinterpret_cast<int*>(ids);
         a->wts = reinterpret_cast<float*>(wts);
-        a->arrived = reinterpret_cast<int*>(arrived);
-        a->xh = xh;
-        a->inv = reinterpret_cast<float*>(inv);
-        a->part = reinterpret_cast<float*>(part);
+        a->place = reinterpret_cast<int*>(place);
+        a->xh1 = xh1;
+        a->inv1 = reinterpret_cast<float*>(inv1);
+        a->xh2 = xh2;
+        a->inv2 = reinterpret_cast<float*>(inv2);
+        a->park = reinterpret_cast<float*>(park);
     }
     return off;
 }
 
-static size_t moe_smem(int nmat, int K0, int K1, int G, int kb, int S) {
-    const int blk = (kb + S - 1) / S;
-    size_t b = (size_t)kFewWarps * few_ring_bytes(K0);
-    if (nmat == 2) b += (size_t)kFewWarps * few_ring_bytes(K1);
-    return b + (size_t)nmat * 8 * G * (few_row_bytes(blk) + 4 * blk + 4 * kPartPitch);
-}
-
-// Ranks k is split over: enough CTAs to fill the SMs twice, and a share that fits.
-static int moe_split(int nmat, int K0, int K1, int G, int kb, double units, int sms) {
-    int S = 1;
-    while (S < 8 && 2 * S <= kb &&
-           (units * S < 2.0 * sms || moe_smem(nmat, K0, K1, G, kb, S) > 112 * 1024))
-        S *= 2;
-    return S;
-}
-
-template <typename Kern>
-static int launch_cluster(Kern kern, const char* what, dim3 grid, size_t smem, const MoeArgs& a,
-                          cudaStream_t stream) {
-    if (check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        220 * 1024), what))
-        return RC_DEVICE_ERROR;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(32 * kFewWarps);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = grid.x;
-    at[0].val.clusterDim.y = 1;
-    at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a);
-    note_launch();
-    return check_cuda(e, what) ? RC_DEVICE_ERROR : RC_OK;
-}
-
 template <int CODE, int G>
 static int moe_run(const MoeArgs& a, int sms, cudaStream_t stream) {
-    const int P = a.T * a.top_k;
-    const int slots = P < a.E ? P : a.E;
-    // chosen experts if every token chose at random; only balances the split
-    double miss = 1.0;
-    for (int t = 0; t < a.T; ++t) miss *= 1.0 - (double)a.top_k / a.E;
-    double active = a.E * (1.0 - miss);
-    if (active < 1.0) active = 1.0;
-    const int kd = a.D >> 7, kf = a.F >> 7;
-    const int S1 = moe_split(2, a.Kmax[0], a.Kmax[1], G, kd, active * kf, sms);
-    const int S2 = moe_split(1, a.Kmax[2], 0, G, kf, active * kd, sms);
-    const size_t m1 = moe_smem(2, a.Kmax[0], a.Kmax[1], G, kd, S1);
-    const size_t m2 = moe_smem(1, a.Kmax[2], 0, G, kf, S2);
-    if (m1 > 220 * 1024 || m2 > 220 * 1024) {
-        set_error("moe: hidden %d / expert width %d too long", a.D, a.F);
-        return RC_BAD_REQUEST;
-    }
-    moe_router_kernel<<<dim3(kRouterRanks, a.T), 256, 0, stream>>>(a);
-    note_launch();
-    if (check_cuda(cudaGetLastError(), "moe_router launch")) return RC_DEVICE_ERROR;
-    int rc = launch_cluster(moe_gate_up_kernel<CODE, G>, "moe_gate_up launch", dim3(S1, kf, slots), m1,
-                            a, stream);
+    int rc = launch_kernel(moe_router_kernel, "moe_router launch", dim3(kRouterRanks, a.T), 256, 0, false,
+                           stream, a);
     if (rc) return rc;
-    return launch_cluster(moe_down_kernel<CODE, G>, "moe_down launch", dim3(S2, kd, slots), m2, a,
-                          stream);
+    const int P = a.T * a.top_k, kd = a.D >> 7, kf = a.F >> 7;
+    const int K1 = a.Kmax[0] > a.Kmax[1] ? a.Kmax[0] : a.Kmax[1];
+    const long long t1 = 2LL * a.slots_max * kf * kd, t2 = t1 / 2;
+    const int c1 = (int)(t1 < sms ? t1 : sms), c2 = (int)(t2 < sms ? t2 : sms);
+    rc = launch_kernel(moe_gate_up_kernel<CODE, G>, "moe_gate_up launch", dim3(c1), 32 * kFewWarps,
+                       few_smem(K1) + plan_bytes(P, a.slots_max, 2), true, stream, a);
+    if (rc) return rc;
+    rc = launch_kernel(moe_gate_up_finish_kernel<G>, "moe_gate_up_finish launch", dim3(kf, P), 128, 0,
+                       true, stream, a, c1);
+    if (rc) return rc;
+    rc = launch_kernel(moe_down_kernel<CODE, G>, "moe_down launch", dim3(c2), 32 * kFewWarps,
+                       few_smem(a.Kmax[2]) + plan_bytes(P, a.slots_max, 1), true, stream, a);
+    if (rc) return rc;
+    return launch_kernel(moe_down_finish_kernel<G>, "moe_down_finish launch", dim3(kd, a.T), 128, 0, true,
+                         stream, a, c2);
 }
 
 }  // namespace exl3b
@@ -479,7 +464,7 @@ bool aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
 bool moe_dims(int T, int D, int F, int E, int top_k) {
     return T >= 0 && T <= kMaxTokens && D > 0 && D % 128 == 0 && F > 0 && F % 128 == 0 && E > 0 &&
-           E <= kMaxExperts && top_k > 0 && top_k <= kMaxTopK && top_k <= E;
+           E <= kMaxExperts && top_k > 0 && top_k <= kMaxTopK && top_k <= E && T * top_k <= kMaxPairs;
 }
 
 }  // namespace
@@ -488,7 +473,8 @@ extern "C" {
 
 size_t exl3b_moe_workspace_bytes(int T, int D, int F, int E, int top_k) {
     if (T <= 0 || !moe_dims(T, D, F, E, top_k)) return 0;
-    return moe_layout(nullptr, T, D, F, top_k, nullptr);
+    const int sms = device_sms();
+    return sms > 0 ? moe_layout(nullptr, T, D, F, E, top_k, sms, nullptr) : 0;
 }
 
 int exl3b_moe(const void* dX, int dtype, int64_t ldx, int T, int D, int F, int E, int top_k,
@@ -505,8 +491,8 @@ int exl3b_moe(const void* dX, int dtype, int64_t ldx, int T, int D, int F, int E
     }
     if (!moe_dims(T, D, F, E, top_k)) {
         set_error("moe: %d tokens (at most %d), hidden %d and expert width %d (multiples of 128), "
-                  "%d experts (at most %d), top_k %d (at most %d)", T, kMaxTokens, D, F, E,
-                  kMaxExperts, top_k, kMaxTopK);
+                  "%d experts (at most %d), top_k %d (at most %d; tokens x top_k at most %d)", T,
+                  kMaxTokens, D, F, E, kMaxExperts, top_k, kMaxTopK, kMaxPairs);
         return RC_BAD_REQUEST;
     }
     if (T == 0) return RC_OK;
@@ -523,13 +509,17 @@ int exl3b_moe(const void* dX, int dtype, int64_t ldx, int T, int D, int F, int E
                   (long long)ldo, (long long)ldres);
         return RC_BAD_REQUEST;
     }
+    if (!ws || !aligned(ws, 256)) {
+        set_error("moe: workspace missing or misaligned");
+        return RC_WORKSPACE;
+    }
+    DeviceState* st;
+    if (device_state(&st)) { set_error("no usable CUDA device"); return RC_NO_DEVICE; }
     const size_t need = exl3b_moe_workspace_bytes(T, D, F, E, top_k);
     if (!ws || ws_bytes < need || !aligned(ws, 256)) {
         set_error("moe: workspace %zu < %zu bytes or misaligned", ws_bytes, need);
         return RC_WORKSPACE;
     }
-    DeviceState* st;
-    if (device_state(&st)) { set_error("no usable CUDA device"); return RC_NO_DEVICE; }
     MoeArgs a = {};
     a.x = dX; a.ldx = ldx; a.dtype = dtype;
     a.T = T; a.D = D; a.F = F; a.E = E; a.top_k = top_k; a.normalize = normalize;
@@ -537,10 +527,9 @@ int exl3b_moe(const void* dX, int dtype, int64_t ldx, int T, int D, int F, int E
     a.experts = dExperts;
     a.Kmax[0] = Kmax_gate; a.Kmax[1] = Kmax_up; a.Kmax[2] = Kmax_down;
     a.residual = d_residual; a.ldres = ldres; a.out = dOut; a.ldo = ldo;
-    moe_layout(&a, T, D, F, top_k, static_cast<uint8_t*>(ws));
+    moe_layout(&a, T, D, F, E, top_k, st->sms, static_cast<uint8_t*>(ws));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    // groups of 16 rows once an expert may have more than 8 tokens
-#define EXL3B_MOE(C) (T > 8 ? moe_run<C, 2>(a, st->sms, s) : moe_run<C, 1>(a, st->sms, s))
+#define EXL3B_MOE(C) (moe_groups(T, E, top_k) == 2 ? moe_run<C, 2>(a, st->sms, s) : moe_run<C, 1>(a, st->sms, s))
     switch (code) {
         case CODE_MUL1: return EXL3B_MOE(CODE_MUL1);
         case CODE_3INST: return EXL3B_MOE(CODE_3INST);

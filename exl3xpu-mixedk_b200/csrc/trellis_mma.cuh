@@ -23,34 +23,41 @@ namespace exl3b {
 
 // Values of two states, packed in fp16 (lo: s0).  The formulas are those of
 // build_code_lut; each value is one rounding to fp16 of an exact expression, as
-// the table's.
+// the table's.  Integer multiplies, dp4a and packed fp16 share one pipe at half rate,
+// logic, shifts, byte permutes and vabsdiff4 the other: the work is spread over both
+// (mul1, K = 4: 53 cycles a tile and scheduler; both byte sums as dp4a and the pack as
+// a permute 58; byte sums by an 8-bit matrix instruction 60).
 template <int CODE>
 __device__ __forceinline__ uint32_t code_pair(uint32_t s0, uint32_t s1) {
-    if (CODE == CODE_MUL1) {
+    uint32_t r;
+    if constexpr (CODE == CODE_MUL1) {
         // 0x6400 | b is 1024 + b in fp16 for b < 1024: the byte sum (<= 1020) lands
         // in the mantissa, and one fused multiply-add gives the value
         const uint32_t h0 = __dp4a(s0 * 0x83DCD12Du, 0x01010101u, 0x6400u);
-        const uint32_t h1 = __dp4a(s1 * 0x83DCD12Du, 0x01010101u, 0x6400u);
-        const uint32_t p = __byte_perm(h0, h1, 0x5410);
-        uint32_t r;
+        uint32_t h1;
+        asm("vabsdiff4.u32.u32.u32.add %0, %1, %2, %3;"
+            : "=r"(h1) : "r"(s1 * 0x83DCD12Du), "r"(0), "r"(0x6400));
+        const uint32_t p = h1 * 65536u + h0;
         asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(p), "r"(0x1EEE1EEEu), "r"(0xC931C931u));
-        return r;
     } else {
         uint32_t x0, x1;
-        if (CODE == CODE_3INST) {
+        if constexpr (CODE == CODE_3INST) {
             x0 = s0 * 89226354u + 64248484u;
             x1 = s1 * 89226354u + 64248484u;
         } else {
             x0 = s0 * 0xCBAC1FEDu;
             x1 = s1 * 0xCBAC1FEDu;
         }
-        x0 = (x0 & 0x8FFF8FFFu) ^ 0x3B603B60u;
-        x1 = (x1 & 0x8FFF8FFFu) ^ 0x3B603B60u;
-        const uint32_t lo = __byte_perm(x0, x1, 0x5410), hi = __byte_perm(x0, x1, 0x7632);
-        uint32_t r;
-        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(lo), "r"(hi));
-        return r;
+        // (x & m) ^ c as one instruction: 0x6a is (a & b) ^ c
+        asm("lop3.b32 %0, %0, %1, %2, 0x6a;" : "+r"(x0) : "r"(0x8FFF8FFFu), "r"(0x3B603B60u));
+        asm("lop3.b32 %0, %0, %1, %2, 0x6a;" : "+r"(x1) : "r"(0x8FFF8FFFu), "r"(0x3B603B60u));
+        const __half2 y0 = *reinterpret_cast<const __half2*>(&x0);
+        const __half2 y1 = *reinterpret_cast<const __half2*>(&x1);
+        const __half2 v = __halves2half2(__hadd_rn(__low2half(y0), __high2half(y0)),
+                                         __hadd_rn(__low2half(y1), __high2half(y1)));
+        r = *reinterpret_cast<const uint32_t*>(&v);
     }
+    return r;
 }
 
 // 16 bits at bit POS (from the top) of the 96-bit string v0 : v1 : v2.
@@ -58,11 +65,11 @@ template <int POS>
 __device__ __forceinline__ uint32_t window16(uint32_t v0, uint32_t v1, uint32_t v2) {
     const uint32_t a = POS < 32 ? v0 : v1, b = POS < 32 ? v1 : v2;
     constexpr int o = POS & 31;
-    if (o == 0) return a >> 16;
-    if (o == 8) return __byte_perm(a, 0, 0x4421);
-    if (o == 16) return a & 0xFFFFu;
-    if (o < 16) return (a >> (16 - o)) & 0xFFFFu;
-    return __funnelshift_l(b, a, o - 16) & 0xFFFFu;
+    if constexpr (o == 0) return a >> 16;
+    else if constexpr (o == 8) return __byte_perm(a, 0, 0x4421);
+    else if constexpr (o == 16) return a & 0xFFFFu;
+    else if constexpr (o < 16) return (a >> (16 - o)) & 0xFFFFu;
+    else return __funnelshift_l(b, a, o - 16) & 0xFFFFu;
 }
 
 // One lane's place in a tile's stream: its eight windows are the bits
@@ -91,37 +98,39 @@ template <int K, int CODE>
 __device__ __forceinline__ void decode_tile(const uint32_t* __restrict__ tile,
                                             const LaneWindow<K>& lw, uint32_t (&a)[4]) {
     const uint32_t x0 = tile[lw.w0], x1 = tile[lw.w1];
-    const uint32_t x2 = LaneWindow<K>::kThree ? tile[lw.w2] : 0u;
-    const uint32_t v0 = __funnelshift_l(x1, x0, lw.shift);
-    const uint32_t v1 = __funnelshift_l(x2, x1, lw.shift);
-    const uint32_t v2 = LaneWindow<K>::kThree ? x2 << lw.shift : 0u;
     uint32_t s[8];
-    if (K == 2) {          // windows 8 bits apart share a shift
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const uint32_t u = v0 << (2 * r);
-            s[r] = u >> 16;
-            s[r + 4] = __byte_perm(u, 0, 0x4421);
-        }
-    } else if (K == 4) {
-        const uint32_t u = __funnelshift_l(v1, v0, 4);
-        s[0] = v0 >> 16;
-        s[1] = u >> 16;
-        s[2] = __byte_perm(v0, 0, 0x4421);
-        s[3] = __byte_perm(u, 0, 0x4421);
-        s[4] = v0 & 0xFFFFu;
-        s[5] = u & 0xFFFFu;
-        s[6] = window16<24>(v0, v1, v2);
-        s[7] = window16<28>(v0, v1, v2);
+    if (K == 4) {          // a lane's word and the one before it, at fixed places
+        const uint32_t u = x1 << 4;
+        s[0] = window16<20>(x0, x1, 0u);
+        s[1] = window16<24>(x0, x1, 0u);
+        s[2] = window16<28>(x0, x1, 0u);
+        s[3] = x1 >> 16;
+        s[4] = u >> 16;
+        s[5] = __byte_perm(x1, 0, 0x4421);
+        s[6] = __byte_perm(u, 0, 0x4421);
+        s[7] = x1 & 0xFFFFu;
     } else {
-        s[0] = window16<0>(v0, v1, v2);
-        s[1] = window16<K>(v0, v1, v2);
-        s[2] = window16<2 * K>(v0, v1, v2);
-        s[3] = window16<3 * K>(v0, v1, v2);
-        s[4] = window16<4 * K>(v0, v1, v2);
-        s[5] = window16<5 * K>(v0, v1, v2);
-        s[6] = window16<6 * K>(v0, v1, v2);
-        s[7] = window16<7 * K>(v0, v1, v2);
+        const uint32_t x2 = LaneWindow<K>::kThree ? tile[lw.w2] : 0u;
+        const uint32_t v0 = __funnelshift_l(x1, x0, lw.shift);
+        if (K == 2) {      // windows 8 bits apart share a shift
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t u = v0 << (2 * r);
+                s[r] = u >> 16;
+                s[r + 4] = __byte_perm(u, 0, 0x4421);
+            }
+        } else {
+            const uint32_t v1 = __funnelshift_l(x2, x1, lw.shift);
+            const uint32_t v2 = K == 7 ? x2 << lw.shift : 0u;
+            s[0] = window16<0>(v0, v1, v2);
+            s[1] = window16<K>(v0, v1, v2);
+            s[2] = window16<2 * K>(v0, v1, v2);
+            s[3] = window16<3 * K>(v0, v1, v2);
+            s[4] = window16<4 * K>(v0, v1, v2);
+            s[5] = window16<5 * K>(v0, v1, v2);
+            s[6] = window16<6 * K>(v0, v1, v2);
+            s[7] = window16<7 * K>(v0, v1, v2);
+        }
     }
     a[0] = code_pair<CODE>(s[0], s[1]);
     a[2] = code_pair<CODE>(s[2], s[3]);
@@ -132,8 +141,7 @@ __device__ __forceinline__ void decode_tile(const uint32_t* __restrict__ tile,
 // acc[16 n][8 rows] += A (16 n x 16 k) . B (16 k x 8 rows)
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                           uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
         "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));

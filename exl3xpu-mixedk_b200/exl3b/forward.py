@@ -214,7 +214,7 @@ def linear(x: torch.Tensor, w: TrellisWeight, bias: torch.Tensor | None = None,
 
 
 # ------------------------------------------------------------------ mixture of experts
-MOE_TOKENS = 256            # of one launch; longer inputs are cut
+MOE_TOKENS, MOE_PAIRS = 256, 2048      # tokens and (token, expert) pairs of one call
 MOE_EXPERTS, MOE_TOP_K = 1024, 32
 
 
@@ -267,8 +267,9 @@ def moe(x: torch.Tensor, router: torch.Tensor, experts: TrellisExperts, top_k: i
     with w = p, or p / sum_S p if `normalize`.  x [..., D] bf16 or fp16, router
     [E, D] of x's dtype or fp32, residual [..., D].  Returns [..., D] in x's
     dtype, or writes `out`, which may be `residual` itself.  More than 256 tokens
-    are taken 256 at a time; every chosen expert is read once per launch for 8 or
-    16 of its tokens, so long prompts are better served by linear per expert."""
+    (or 2048 choices) are taken in pieces of that many; a chosen expert is read once
+    for 8 or 16 of its tokens, so long prompts are better served by linear per
+    expert."""
     if x.dtype not in DTYPE_IDS:
         raise ValueError(f"x must be bf16 or fp16, got {x.dtype}")
     if x.device != experts.device:
@@ -293,11 +294,11 @@ def moe(x: torch.Tensor, router: torch.Tensor, experts: TrellisExperts, top_k: i
     if T:
         with torch.cuda.device(x.device):
             dev = ops.select_device(xr)
-            nbytes = lib().exl3b_moe_workspace_bytes(min(T, MOE_TOKENS), D, experts.F, experts.E,
-                                                     top_k)
+            most = min(MOE_TOKENS, MOE_PAIRS // top_k)
+            nbytes = lib().exl3b_moe_workspace_bytes(min(T, most), D, experts.F, experts.E, top_k)
             ws, ws_ptr = _workspace(nbytes, x.device)
-            for t in range(0, T, MOE_TOKENS):
-                n = min(MOE_TOKENS, T - t)
+            for t in range(0, T, most):
+                n = min(most, T - t)
                 call("exl3b_moe", xr[t:].data_ptr(), DTYPE_IDS[x.dtype], _ld(xr), n, D, experts.F,
                      experts.E, top_k, int(bool(normalize)), rt.data_ptr(),
                      0 if router.dtype == torch.float32 else DTYPE_IDS[x.dtype], _ld(rt),

@@ -361,9 +361,8 @@ typedef struct {
  *         8 elements); residual (nullable) and out [T][D] with 8-byte aligned
  *         rows; dtype 1 = bf16, 2 = fp16; router_dtype the same, or 0 = fp32
  *   dExperts device table [3][E]: gate [D][F], up [D][F], down [F][D] of every
- *         expert, all of one code; each K in 2..Kmax of its kind (an entry
- *         outside is not computed, and its tokens' rows are not written)
- *   T <= 256, E <= 1024, top_k <= 32; D and F multiples of 128
+ *         expert, all of one code; each K in 2..Kmax of its kind
+ *   T <= 256, E <= 1024, top_k <= 32, T top_k <= 2048; D and F multiples of 128
  * Logits are summed in fp64, so a token's choice does not depend on the batch;
  * every other sum is fp32 in a fixed order; one rounding to dtype at the end.
  * ws: exl3b_moe_workspace_bytes bytes, 256-byte aligned, in use until the work

@@ -84,29 +84,41 @@ struct LinearJob {
     static constexpr bool kRotate = ROTATE;
     const LinearArgs& a;
     const FewScratch& w;
-    int nbn;
-    __device__ __forceinline__ FewUnit unit(int u) const {
-        const int rg = u / nbn, nb = u - rg * nbn;
-        return {a.trellis + (size_t)nb * 256 * a.K, (uint32_t)nbn * 256 * a.K, a.K};
+    const FastDiv& nbn;
+    struct Cursor {
+        const uint8_t* tiles;
+        uint32_t kt_bytes;
+        int K, left;               // column blocks from here to the last
+    };
+    __device__ __forceinline__ Cursor cursor(int u) const {
+        int rg;
+        const int nb = nbn.mod(u, rg);
+        return {a.trellis + (size_t)nb * 256 * a.K, nbn.d * 256 * a.K, a.K, (int)nbn.d - nb};
     }
-    __device__ __forceinline__ int rows(int u) const { return min(8 * G, a.M - u / nbn * 8 * G); }
-    __device__ __forceinline__ size_t row(int u, int r, int b) const {
-        return (size_t)b * a.M + u / nbn * 8 * G + r;
+    __device__ __forceinline__ void next(Cursor& c) const {
+        c.tiles += 256 * a.K;
+        if (--c.left == 0) {       // the next group of rows
+            c.tiles = a.trellis;
+            c.left = (int)nbn.d;
+        }
     }
+    __device__ __forceinline__ int rows(int u) const { return min(8 * G, a.M - nbn.div(u) * 8 * G); }
+    __device__ __forceinline__ size_t row(int u, int r) const { return nbn.div(u) * 8 * G + r; }
+    __device__ __forceinline__ int row_step() const { return a.M; }
     __device__ __forceinline__ const uint8_t* xh() const { return w.xh; }
     __device__ __forceinline__ const float* inv() const { return w.inv; }
     __device__ __forceinline__ void wait() const { if (!ROTATE) pdl_wait(); }
-    __device__ __forceinline__ void rotate(int u, int r, int b, uint8_t* dst, float* inv, int swz) const {
-        linear_rotate(a, u / nbn * 8 * G + r, b, dst, inv, swz);
+    __device__ __forceinline__ void rotate(int r, int b, uint8_t* dst, float* inv, int swz) const {
+        linear_rotate(a, r, b, dst, inv, swz);
     }
 };
 
 template <int CODE, int G, bool ROTATE>
 __global__ void __launch_bounds__(32 * kFewWarps, 1)
-linear_few_kernel(const LinearArgs a, const FewScratch w, const FewRun run) {
+linear_few_kernel(const LinearArgs a, const FewScratch w, const FewRun run, const FastDiv nbn) {
     extern __shared__ __align__(16) uint8_t sm[];
     pdl_launch();
-    const LinearJob<G, ROTATE> job = {a, w, a.n >> 7};
+    const LinearJob<G, ROTATE> job = {a, w, nbn};
     few_run<CODE, G>(job, run, a.K, sm, w.park);
 }
 
@@ -114,15 +126,17 @@ linear_few_kernel(const LinearArgs a, const FewScratch w, const FewRun run) {
 // whose four warps take every fourth parked sum.
 template <int G>
 __global__ void __launch_bounds__(128)
-linear_finish_kernel(const LinearArgs a, const FewScratch w, const FewRun run) {
+linear_finish_kernel(const LinearArgs a, const FewScratch w, const FewJoin join) {
     __shared__ float4 sum[3][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int nb = blockIdx.x, row = blockIdx.y, col = nb * 128 + 4 * lane;
     LinearEpilogue ep;
     if (warp == 0) ep.load(a, row, col);
+    const int u = row / (8 * G) * gridDim.x + nb;
+    const FewParts parts(join, u);
     pdl_wait();
     float v[4];
-    few_sum<G>(w.park, run, row / (8 * G) * gridDim.x + nb, row % (8 * G), lane, warp, 4, v);
+    few_sum<G>(w.park, join, parts, u, row % (8 * G), lane, warp, 4, v);
     if (warp) sum[warp - 1][lane] = make_float4(v[0], v[1], v[2], v[3]);
     __syncthreads();
     if (warp) return;
@@ -135,7 +149,7 @@ linear_finish_kernel(const LinearArgs a, const FewScratch w, const FewRun run) {
 static size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 static FewRun linear_run(int M, int k, int n, int G, int sms) {
-    return FewRun(k >> 7, (n >> 7) * ((M + 8 * G - 1) / (8 * G)), sms);
+    return FewRun(FastDiv(k >> 7), (n >> 7) * ((M + 8 * G - 1) / (8 * G)), sms);
 }
 
 // Workspace of the few-rows path, laid out at ws.
@@ -144,8 +158,8 @@ static size_t few_layout(FewScratch* w, int M, int k, int n, int G, int sms, uin
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t o = off; off += up256(bytes); return ws + o; };
     w->park = reinterpret_cast<float*>(take(few_park_bytes(run.units, run.ctas, G)));
-    w->xh = take((size_t)run.kb * M * kRowBytes);
-    w->inv = reinterpret_cast<float*>(take((size_t)run.kb * M * 4));
+    w->xh = take((size_t)(k >> 7) * M * kRowBytes);
+    w->inv = reinterpret_cast<float*>(take((size_t)(k >> 7) * M * 4));
     return off;
 }
 
@@ -155,20 +169,29 @@ static int few_launch(const LinearArgs& a, int sms, uint8_t* ws, cudaStream_t st
     few_layout(&w, a.M, a.k, a.n, G, sms, ws);
     const FewRun run = linear_run(a.M, a.k, a.n, G, sms);
     const dim3 fin(a.n >> 7, a.M);
-    int rc;
-    if (a.M <= 2) {            // rotated where they are used: cheaper than a launch
-        rc = launch_kernel(linear_few_kernel<CODE, G, true>, "linear_few launch", dim3(run.ctas),
-                           32 * kFewWarps, few_smem(a.K), false, stream, a, w, run);
-    } else {
-        rc = launch_kernel(linear_rotate_kernel, "linear_rotate launch", dim3((run.kb * a.M + 3) / 4),
-                           128, 0, false, stream, a, w);
+    const FastDiv nbn(a.n >> 7);
+    const int most = run.least + (run.longer ? 1 : 0), ring = kFewGroups * kRowStages;
+    int rc = RC_OK;
+    bool done = false;
+    if constexpr (G == 1) {
+        // one or two rows are rotated where they are used, cheaper than a launch (5120 x
+        // 5120, K = 4: 12.2 us against 12.9), if a CTA's share of them fits
+        if (a.M <= 2 && few_smem(a.K, G, most) <= kFewRoom) {
+            rc = launch_kernel(linear_few_kernel<CODE, G, true>, "linear_few launch", dim3(run.ctas),
+                               32 * kFewWarps, few_smem(a.K, G, most), false, stream, a, w, run, nbn);
+            done = true;
+        }
+    }
+    if (!done) {
+        rc = launch_kernel(linear_rotate_kernel, "linear_rotate launch",
+                           dim3(((a.k >> 7) * a.M + 3) / 4), 128, 0, false, stream, a, w);
         if (rc) return rc;
         rc = launch_kernel(linear_few_kernel<CODE, G, false>, "linear_few launch", dim3(run.ctas),
-                           32 * kFewWarps, few_smem(a.K), true, stream, a, w, run);
+                           32 * kFewWarps, few_smem(a.K, G, ring), true, stream, a, w, run, nbn);
     }
     if (rc) return rc;
     return launch_kernel(linear_finish_kernel<G>, "linear_finish launch", fin, 128, 0, true, stream, a,
-                         w, run);
+                         w, FewJoin(run));
 }
 
 static int few_groups(int M) { return M > 8 ? 2 : 1; }

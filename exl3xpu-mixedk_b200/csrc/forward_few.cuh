@@ -16,7 +16,8 @@ namespace exl3b {
 
 constexpr int kFewGroups = 2;         // groups of eight warps, taking k blocks in turn
 constexpr int kFewWarps = 8 * kFewGroups;
-constexpr int kFewStages = 3;         // ring depth in blocks of 128 k
+constexpr int kFewStages = 3;         // weight ring of a warp, in blocks of 128 k
+constexpr int kRowStages = 4;         // row ring of a group: one more, see few_run
 
 // element types of activations (the ABI's dtype values)
 enum XType : int { X_BF16 = 1, X_FP16 = 2 };
@@ -39,31 +40,37 @@ constexpr int kRowBytes = 256;
 __device__ __forceinline__ int few_swizzle(int row, int byte) { return byte ^ ((row & 1) << 6); }
 
 // A warp's stream of k blocks: 16 K pieces of 16 bytes a block, piece c by lane
-// c mod 32 in turn.  Where a lane's pieces lie inside a block does not change, so
-// they are found once.
+// c mod 32 in turn.
 template <int K>
 struct FewStream {
     static constexpr int kPieces = (16 * K + 31) / 32;         // per lane
-    uint32_t kt[kPieces], off[kPieces];    // k tile of a piece and its place in the tile
+    const uint8_t* src;        // the next block's first tile, plus this lane's first piece
+    uint32_t off[kPieces];     // its other pieces from there
+    uint32_t dst;              // its place in the ring
     int lane;
 
-    __device__ __forceinline__ explicit FewStream(int lane_) : lane(lane_) {
+    __device__ __forceinline__ FewStream(uint8_t* ring, int lane_) : lane(lane_) {
+        dst = (uint32_t)__cvta_generic_to_shared(ring) + 16 * lane;
+    }
+    // Go on at the block whose first tile is at `tile`, `kt_bytes` between k tiles.
+    __device__ __forceinline__ void seek(const uint8_t* tile, uint32_t kt_bytes) {
+        uint32_t first = 0;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-            const int c = lane + 32 * i;
-            kt[i] = c / (2 * K);
-            off[i] = 16 * (c - kt[i] * 2 * K);
+            const int c = lane + 32 * i, kt = c / (2 * K);
+            const uint32_t o = kt * kt_bytes + 16 * (c - kt * 2 * K);
+            if (i == 0) first = o;
+            off[i] = o - first;
         }
+        src = tile + first;
     }
-    // Copy the block whose first tile is at `src` into stage `stage` of the ring.
-    __device__ __forceinline__ void issue(const uint8_t* src, uint32_t kt_bytes, uint8_t* ring,
-                                          int stage) {
-        const uint32_t dst = (uint32_t)__cvta_generic_to_shared(ring) + stage * 256 * K + 16 * lane;
+    // Copy that block into stage `stage` of the ring.
+    __device__ __forceinline__ void issue(int stage) const {
 #pragma unroll
         for (int i = 0; i < kPieces; ++i)
             if (16 * K % 32 == 0 || i + 1 < kPieces || lane + 32 * i < 16 * K)
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
-                             :: "r"(dst + 512 * i), "l"(src + (kt[i] * kt_bytes + off[i])) : "memory");
+                             :: "r"(dst + stage * 256 * K + 512 * i), "l"(src + off[i]) : "memory");
     }
 };
 
@@ -165,23 +172,55 @@ __device__ __forceinline__ void with_bits(int K, const F& f) {
 // clusters that join through distributed shared memory 11.3 at the one cluster size
 // that fits the 40 column blocks and 14 to 16 at the others (row of 17408 x 5120: 31 to
 // 37 and up); with the last CTA of a unit to arrive adding the sums 14.7.
+
+// Division of an int >= 0 by a divisor known ahead: q = mulhi and shifts (the
+// round-up method of Granlund and Montgomery, exact for all 32-bit dividends).
+struct FastDiv {
+    uint32_t d, mul, sh1, sh2;
+    __host__ __device__ FastDiv() {}
+    __host__ __device__ explicit FastDiv(uint32_t d_) : d(d_) {
+        uint32_t l = 0;
+        while (l < 32 && (1ull << l) < d) ++l;
+        mul = (uint32_t)((((1ull << l) - d) << 32) / d) + 1;
+        sh1 = l < 1 ? l : 1;
+        sh2 = l > 1 ? l - 1 : 0;
+    }
+    __device__ __forceinline__ int div(int n) const {
+        const uint32_t t = __umulhi(mul, (uint32_t)n);
+        return (int)((t + (((uint32_t)n - t) >> sh1)) >> sh2);
+    }
+    // n = q * d + returned remainder
+    __device__ __forceinline__ int mod(int n, int& q) const {
+        q = div(n);
+        return n - q * (int)d;
+    }
+};
+
 struct FewRun {
-    int kb, units, ctas;
+    int units, ctas;
     int least, longer;         // blocks of a CTA's run; the first `longer` have one more
-    __host__ __device__ FewRun(int kb_, int units_, int sms) : kb(kb_), units(units_) {
-        const int total = kb * units;
+    FastDiv kb;                // blocks of a unit
+    __host__ __device__ FewRun() {}
+    __host__ __device__ FewRun(const FastDiv& kb_, int units_, int sms) : units(units_), kb(kb_) {
+        const int total = (int)kb.d * units;
         ctas = total < sms ? total : sms;
         least = ctas ? total / ctas : 0;
         longer = ctas ? total % ctas : 0;
     }
     __host__ __device__ int start(int cta) const { return cta * least + (cta < longer ? cta : longer); }
-    // the CTA whose run holds block g
-    __host__ __device__ int owner(int g) const {
-        const int head = longer * (least + 1);
-        return g < head ? g / (least + 1) : longer + (g - head) / least;
+};
+
+// A run as the joining kernels see it: which CTA's run holds block g.
+struct FewJoin {
+    FewRun run;
+    FastDiv least, more;       // by the blocks of the short runs and of the longer ones
+    __host__ __device__ FewJoin() {}
+    __host__ __device__ explicit FewJoin(const FewRun& r)
+        : run(r), least(r.least ? r.least : 1), more(r.least + 1) {}
+    __device__ __forceinline__ int owner(int g) const {
+        const int head = run.longer * (run.least + 1);
+        return g < head ? more.div(g) : run.longer + least.div(g - head);
     }
-    __host__ __device__ int first(int u) const { return owner(u * kb); }
-    __host__ __device__ int last(int u) const { return owner(u * kb + kb - 1); }
 };
 
 // Parked sums: CTA c's of unit u at slot u + c (along the sequence u or c grows, so
@@ -190,141 +229,179 @@ __host__ __device__ inline size_t few_park_bytes(int units, int ctas, int G) {
     return (size_t)(units + ctas) * kFewGroups * 8 * G * 512;
 }
 
-// Rows are in shared memory for a chunk of blocks at a time (two buffers of 16 / G).
-// A group of warps issues at least kFewStages copies per chunk, which is what makes
-// the next chunk's rows older than any copy in flight when the chunk ends.
-template <int G> struct FewChunk { static constexpr int value = 16 / G; };
-
-__host__ __device__ inline int few_smem(int Kmax) {
-    return kFewWarps * few_ring_bytes(Kmax) + 2 * 16 * 8 * (kRowBytes + 4);
+// Shared memory of the product: weight rings, then the rows -- rings of kRowStages
+// blocks per group, or (rotated in place) all `blocks` of the run.
+constexpr int kFewRoom = 222 * 1024;      // of the 227 KB a CTA may have
+__host__ __device__ inline int few_smem(int Kmax, int G, int blocks) {
+    return kFewWarps * few_ring_bytes(Kmax) + blocks * 8 * G * (kRowBytes + 4);
 }
 
-// A job tells what the units are:
-//   unit(u)      -> FewUnit, the weight
-//   rows(u)      -> its rows, at most 8 G
-//   row(u, r, b) -> index of the rotated block b of row r (blocks of 256 bytes at
-//                   xh(), reciprocal scales at inv()); or, where kRotate is set,
-//   rotate(u, r, b, dst, inv, swz)  puts the block itself (a warp)
-//   wait()       -> returns once the rows are there
-struct FewUnit {
-    const uint8_t* tiles;      // first tile of the column block
-    uint32_t kt_bytes;         // to the next k tile
-    int K;
-};
+// A job tells what the units are.  Its Cursor stands at one unit: tiles (first tile of
+// the column block), kt_bytes (to the next k tile), K.
+//   cursor(u), next(cursor)   the weight of unit u, of the one after it
+//   rows(u)                   its rows, at most 8 G
+// and, unless kRotate,
+//   row(u, r) -> index of block 0 of the unit's row r among the rotated blocks (256
+//                bytes each at xh(), reciprocal scales at inv()); block b is b * kRowStep on
+//   wait()    -> returns once the rows are there
+// or, with kRotate (every unit has the same rows),
+//   rotate(r, b, dst, inv, swz)   puts block b of row r itself (a warp)
 
 // Multiply this CTA's run and park the sums.  All threads.
+//
+// Each iteration of a group is one block: every warp copies its tiles of the block two
+// ahead into its own ring and the group's warps share the copy of that block's rows;
+// then the group meets at a barrier, which makes the rows of the present block visible
+// to all and tells that the block before is read, so that its place may be refilled in
+// the next iteration -- hence a row ring one deeper than the distance needs.
 template <int CODE, int G, typename Job>
 __device__ __forceinline__ void few_run(const Job& job, const FewRun& run, int Kmax, uint8_t* sm,
                                         float* park) {
-    constexpr int kChunk = FewChunk<G>::value;
-    static_assert(kChunk / kFewGroups > kFewStages, "a chunk outlasts the ring");
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31, grp = warp >> 3, col = warp & 7;
     const int cta = blockIdx.x, g0 = run.start(cta), count = run.start(cta + 1) - g0;
+    const int kb = (int)run.kb.d;
     uint8_t* ring = sm + warp * few_ring_bytes(Kmax);
+    const int blocks = Job::kRotate ? count : kFewGroups * kRowStages;
     uint8_t* xh = sm + kFewWarps * few_ring_bytes(Kmax);
-    float* inv = reinterpret_cast<float*>(xh + 2 * kChunk * 8 * G * kRowBytes);
-    const int kb = run.kb, u0 = g0 / kb, b0 = g0 - u0 * kb;
-
-    // Rows of a chunk's blocks.  Rows past the unit's last stay unwritten: a row is a
-    // column of the matrix instruction, and only rows that exist are read back.
-    auto load_rows = [&](int c) {
-        const int lo = c * kChunk, n = min(kChunk, count - lo);
-        uint8_t* x = xh + (c & 1) * kChunk * 8 * G * kRowBytes;
-        float* s = inv + (c & 1) * kChunk * 8 * G;
-        if constexpr (Job::kRotate) {
-            const int rows = job.rows(u0);                    // of every unit
-            for (int j = warp; j < n * rows; j += kFewWarps) {
-                const int blk = j / rows, r = j - blk * rows, f = b0 + lo + blk, u = u0 + f / kb;
-                job.rotate(u, r, f - f / kb * kb, x + (blk * 8 * G + r) * kRowBytes, s + blk * 8 * G + r,
-                           (r & 1) << 6);
-            }
-        } else {
-            // 16 lanes copy four rows of one block
-            const int half = t >> 4, blk = half / (2 * G), q = t & 15, r0 = half % (2 * G) * 4;
-            if (blk < n) {
-                const int f = b0 + lo + blk, u = u0 + f / kb, b = f - f / kb * kb, rows = job.rows(u);
-                const uint32_t dst = (uint32_t)__cvta_generic_to_shared(x) + blk * 8 * G * kRowBytes;
-                const uint32_t dsi = (uint32_t)__cvta_generic_to_shared(s + blk * 8 * G);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = r0 + e;
-                    if (r >= rows) break;
-                    const size_t from = job.row(u, r, b);
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
-                                 :: "r"(dst + r * kRowBytes + few_swizzle(r, 16 * q)),
-                                    "l"(job.xh() + from * kRowBytes + 16 * q) : "memory");
-                    if (q == 0)
-                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;"
-                                     :: "r"(dsi + 4 * r), "l"(job.inv() + from) : "memory");
-                }
-            }
-        }
-    };
-
+    float* inv = reinterpret_cast<float*>(xh + blocks * 8 * G * kRowBytes);
+    const int mine = Job::kRotate ? 0 : grp * kRowStages;      // the group's first row stage
+    int u0;
+    const int b0 = run.kb.mod(g0, u0);
     float acc[G][4];
 #pragma unroll
     for (int g = 0; g < G; ++g) acc[g][0] = acc[g][1] = acc[g][2] = acc[g][3] = 0.0f;
     int i = grp;                              // this group's next block of the run
-    int chunk = 0;                            // chunk whose rows are ready, once i >= 0
-    bool rows_ready = false;
-    // Stretches of equal bit width: the ring restarts where it changes.
+    int u;                                    // its unit and block there
+    int b = run.kb.mod(b0 + i, u);
+    u += u0;
+    auto at = job.cursor(u);
+    bool waited = false;
+    // this warp's rows of a block: G, sixteen lanes each
+    const int rr = G == 1 ? col : 2 * col + (lane >> 4);
+    const uint32_t rdst = (uint32_t)__cvta_generic_to_shared(xh) + mine * 8 * G * kRowBytes +
+                          rr * kRowBytes + few_swizzle(rr, 16 * (lane & 15));
+    const uint32_t idst = (uint32_t)__cvta_generic_to_shared(inv) + 4 * (mine * 8 * G + rr);
+    // Stretches of equal bit width: the weight ring restarts where it changes.
     while (i < count) {
-        const int K0 = job.unit(u0 + (b0 + i) / kb).K;
-        with_bits(K0, [&](auto bits) {
+        with_bits(at.K, [&](auto bits) {
             constexpr int K = decltype(bits)::value;
-            int u = u0 + (b0 + i) / kb, b = (b0 + i) % kb;
-            // the issuing side runs kFewStages - 1 of the group's blocks ahead
-            FewUnit to = job.unit(u);
-            int iu = u, ib = b, ii = i;
-            bool more = true;                 // the next block to issue has this width
-            FewStream<K> st(lane);
-            auto issue = [&](int stage) {
-                if (more && ii < count) {
-                    st.issue(to.tiles + (size_t)ib * 8 * to.kt_bytes + (size_t)col * 32 * K, to.kt_bytes,
-                             ring, stage);
-                    ii += kFewGroups;
-                    ib += kFewGroups;
-                    if (ib >= kb && ii < count) {
-                        while (ib >= kb) { ib -= kb; ++iu; }
-                        to = job.unit(iu);
-                        more = to.K == K;
+            // the issuing side runs kFewStages - 1 of the group's blocks ahead: `left`
+            // blocks of unit `to`, 0 once there are no more of this width
+            auto to = at;
+            int iu = u, ib = b, ii = i, left = 0;
+            size_t step = 0;
+            [[maybe_unused]] size_t xstep = 0;
+            [[maybe_unused]] const uint8_t* xsrc = nullptr;    // this lane's piece of its row there
+            [[maybe_unused]] const float* isrc = nullptr;
+            [[maybe_unused]] bool has = false;
+            FewStream<K> st(ring, lane);
+            auto seek = [&]() {
+                left = (min(kb - ib, count - ii) + kFewGroups - 1) / kFewGroups;
+                st.seek(to.tiles + (size_t)ib * 8 * to.kt_bytes + (size_t)col * 32 * K, to.kt_bytes);
+                step = (size_t)kFewGroups * 8 * to.kt_bytes;
+                if constexpr (!Job::kRotate) {
+                    has = rr < job.rows(iu) && (G == 2 || lane < 16);
+                    if (has) {
+                        const size_t from = job.row(iu, rr) + (size_t)ib * job.row_step();
+                        xsrc = job.xh() + from * kRowBytes + 16 * (lane & 15);
+                        isrc = job.inv() + from;
+                    }
+                    xstep = (size_t)kFewGroups * job.row_step();
+                }
+            };
+            // rows past the unit's last stay unwritten: a row is a column of the matrix
+            // instruction, and only rows that exist are read back
+            auto issue_rows = [&](int stage) {
+                if constexpr (!Job::kRotate) {
+                    if (has) {
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                                     :: "r"(rdst + stage * 8 * G * kRowBytes), "l"(xsrc) : "memory");
+                        if ((lane & 15) == 0)
+                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;"
+                                         :: "r"(idst + stage * 32 * G), "l"(isrc) : "memory");
+                        xsrc += xstep * kRowBytes;
+                        isrc += xstep;
                     }
                 }
-                cp_commit();
             };
-#pragma unroll
-            for (int s = 0; s < kFewStages - 1; ++s) issue(s);
-            if (!rows_ready) {
-                job.wait();                   // the rows come from the kernel before
-                load_rows(0);
-                cp_commit();
-                cp_wait<0>();
-                __syncthreads();
-                rows_ready = true;
-                if (kChunk < count) load_rows(1);     // joins the next commit
-            }
-            const LaneWindow<K> lw(lane);
-            int cur = 0, fill = kFewStages - 1;
-            while (true) {
-                if (i / kChunk != chunk) {
-                    // the next chunk's rows were issued a chunk ago: older than every
-                    // copy still in flight
-                    cp_wait<kFewStages - 1>();
+            auto issued = [&](int n) {
+                left -= n;
+                ib += n * kFewGroups;
+                ii += n * kFewGroups;
+                if (left > 0 || ii >= count) return;
+                while (ib >= kb) { ib -= kb; ++iu; job.next(to); }
+                if (to.K != K) { ii = count; return; }
+                seek();
+            };
+            seek();
+            if (!waited) {
+                // the weights do not depend on the kernel before; the rows do
+                st.issue(0);
+                if constexpr (Job::kRotate) {
+                    for (int j = warp; j < count * job.rows(0); j += kFewWarps) {
+                        const int rows = job.rows(0), blk = rows == 1 ? j : j >> 1, r = j - blk * rows;
+                        int q;
+                        const int kblk = run.kb.mod(b0 + blk, q);
+                        job.rotate(r, kblk, xh + (blk * 8 * G + r) * kRowBytes, inv + blk * 8 * G + r,
+                                   (r & 1) << 6);
+                    }
                     __syncthreads();
-                    ++chunk;
-                    if ((chunk + 1) * kChunk < count) load_rows(chunk + 1);
+                } else {
+                    job.wait();
                 }
-                issue(fill);
-                cp_wait<kFewStages - 1>();
-                __syncwarp();
-                const int slot = (chunk & 1) * kChunk + (i - chunk * kChunk);
-                few_block<K, CODE, G>(lw, ring + cur * 256 * K, xh + slot * 8 * G * kRowBytes,
-                                      inv + slot * 8 * G, acc, lane);
-                fill = cur;
-                cur = cur + 1 == kFewStages ? 0 : cur + 1;
-                __syncwarp();      // every lane has read the stage before it is refilled
-                i += kFewGroups;
-                b += kFewGroups;
+            } else {
+                // the group's warps have all read the last block of the stretch before
+                asm volatile("bar.sync %0, 256;" :: "r"(1 + grp) : "memory");
+            }
+#pragma unroll
+            for (int s = 0; s < kFewStages - 1; ++s) {
+                if (left > 0) {
+                    if (s > 0 || waited) st.issue(s);
+                    issue_rows(s);
+                    st.src += step;
+                    issued(1);
+                }
+                cp_commit();
+            }
+            waited = true;
+            const LaneWindow<K> lw(lane);
+            int cur = 0, fill = kFewStages - 1, rcur = 0;
+            while (true) {
+                // blocks until the unit, the run or the issued unit ends
+                int n = (min(kb - b, count - i) + kFewGroups - 1) / kFewGroups;
+                const bool feed = left > 0;
+                if (feed) n = min(n, left);
+                const int from = Job::kRotate ? i : mine;
+                const uint8_t* x = xh + from * 8 * G * kRowBytes;
+                const float* f = inv + from * 8 * G;
+#pragma unroll 1
+                for (int j = 0; j < n; ++j) {
+                    if (feed) {
+                        st.issue(fill);
+                        st.src += step;
+                        issue_rows((rcur + kFewStages - 1) & (kRowStages - 1));
+                    }
+                    cp_commit();
+                    cp_wait<kFewStages - 1>();
+                    if constexpr (Job::kRotate) {
+                        __syncwarp();
+                        few_block<K, CODE, G>(lw, ring + cur * 256 * K, x, f, acc, lane);
+                        x += kFewGroups * 8 * G * kRowBytes;
+                        f += kFewGroups * 8 * G;
+                        __syncwarp();      // every lane has read the stage before it is refilled
+                    } else {
+                        asm volatile("bar.sync %0, 256;" :: "r"(1 + grp) : "memory");
+                        few_block<K, CODE, G>(lw, ring + cur * 256 * K, x + rcur * 8 * G * kRowBytes,
+                                              f + rcur * 8 * G, acc, lane);
+                        rcur = (rcur + 1) & (kRowStages - 1);
+                        __syncwarp();
+                    }
+                    fill = cur;
+                    cur = cur + 1 == kFewStages ? 0 : cur + 1;
+                }
+                if (feed) issued(n);
+                i += n * kFewGroups;
+                b += n * kFewGroups;
                 if (b < kb && i < count) continue;
                 // the group's last block of this unit here: park the sums
                 const int rows = job.rows(u);
@@ -344,38 +421,41 @@ __device__ __forceinline__ void few_run(const Job& job, const FewRun& run, int K
                     acc[g][0] = acc[g][1] = acc[g][2] = acc[g][3] = 0.0f;
                 }
                 if (i >= count) break;
-                while (b >= kb) { b -= kb; ++u; }
-                if (job.unit(u).K != K) break;
+                while (b >= kb) { b -= kb; ++u; job.next(at); }
+                if (at.K != K) break;
             }
             cp_wait<0>();
             __syncwarp();
         });
     }
-    // every warp takes part in every chunk's barrier
-    if (!rows_ready) { job.wait(); load_rows(0); cp_commit(); cp_wait<0>(); __syncthreads(); if (kChunk < count) load_rows(1); }
-    while ((chunk + 1) * kChunk < count) {
-        cp_commit();
-        cp_wait<0>();
+    // a group without a block meets the others all the same
+    if (Job::kRotate && !waited) {
         __syncthreads();
-        ++chunk;
-        if ((chunk + 1) * kChunk < count) load_rows(chunk + 1);
     }
 }
 
 // Sum of unit u's parked sums of row r, elements 4 lane .. 4 lane + 3: the ones at
 // `part`, part + parts, ... in the order of the CTAs and their groups.  A warp.
+struct FewParts {
+    int lo, hi, c0, n;
+    __device__ __forceinline__ FewParts(const FewJoin& j, int u) {
+        lo = u * (int)j.run.kb.d;
+        hi = lo + (int)j.run.kb.d;
+        c0 = j.owner(lo);
+        n = (j.owner(hi - 1) - c0 + 1) * kFewGroups;
+    }
+};
+
 template <int G>
-__device__ __forceinline__ void few_sum(const float* park, const FewRun& run, int u, int r, int lane,
-                                        int part, int parts, float (&v)[4]) {
-    const int lo = u * run.kb, hi = lo + run.kb;
-    const int c0 = run.first(u), n = (run.last(u) - c0 + 1) * kFewGroups;
-    const float* from = park + (size_t)(u + c0) * kFewGroups * 8 * G * 128 + r * 128 + 4 * lane;
+__device__ __forceinline__ void few_sum(const float* park, const FewJoin& join, const FewParts& p, int u,
+                                        int r, int lane, int part, int parts, float (&v)[4]) {
+    const float* from = park + (size_t)(u + p.c0) * kFewGroups * 8 * G * 128 + r * 128 + 4 * lane;
     v[0] = v[1] = v[2] = v[3] = 0.0f;
 #pragma unroll 4
-    for (int i = part; i < n; i += parts) {
-        const int c = c0 + i / kFewGroups, g = i % kFewGroups;
-        const int s = run.start(c), e = run.start(c + 1);
-        const int f = s > lo ? s : lo, l = e < hi ? e : hi;      // the CTA's blocks of u
+    for (int i = part; i < p.n; i += parts) {
+        const int c = p.c0 + i / kFewGroups, g = i % kFewGroups;
+        const int s = join.run.start(c), e = join.run.start(c + 1);
+        const int f = s > p.lo ? s : p.lo, l = e < p.hi ? e : p.hi;      // the CTA's blocks of u
         // a group takes every other block of the run: none of a single one, maybe
         if (l - f >= kFewGroups || ((f - s) & 1) == g) {
             const float4 q = __ldcg(reinterpret_cast<const float4*>(from + (size_t)i * 8 * G * 128));
@@ -401,6 +481,11 @@ int launch_kernel(void (*kern)(P...), const char* what, dim3 grid, int threads, 
     if (smem > 48 * 1024 &&
         check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
                    what))
+        return RC_DEVICE_ERROR;
+    // the same split of L1 for all: a kernel that wants another waits for the SM to empty
+    if (smem <= 48 * 1024 &&
+        check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                        cudaSharedmemCarveoutMaxShared), what))
         return RC_DEVICE_ERROR;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;

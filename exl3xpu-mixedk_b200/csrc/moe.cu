@@ -2,15 +2,17 @@
 //   l = x R^T;  S = the top_k largest l (ties: lowest index);  p = softmax(l)
 //   y = sum_{e in S} w_e ((silu(x Wg_e) * (x Wu_e)) Wd_e) + residual,  w = p or p / sum_S p
 //
-// The router (logits, choice, weights, and the chosen experts' rotations of the
-// token), then the gate and up products of every chosen expert, the down products, and
-// after each a kernel that joins the parked sums: to the down projection's rotated
-// rows, and to the weighted sum.  Every launch but the first overlaps the one before
-// it.  Each chosen expert's tensors are read once for 8 G of its tokens; the work is
+// Six launches, every one but the first started while the one before still runs: the
+// router (logits, choice, weights); the chosen experts' rotations of the tokens, and
+// the plan of the products; the gate and up products of every chosen expert; their
+// join, to the down projection's rotated rows; the down products; their join, to the
+// weighted sum.  Each chosen expert's tensors are read once for 8 G of its tokens; the work is
 // bound by their decode, spread evenly over the SMs as in forward_few.cuh.  Nothing depends on
 // the order in which CTAs run: partial sums are added in a fixed order, and a token's
 // experts in the order of their choice.
 #include <cooperative_groups.h>
+#include <string.h>
+
 #include <utility>
 
 #include "forward_few.cuh"
@@ -25,11 +27,21 @@ constexpr int kMaxTokens = 256;
 constexpr int kMaxTopK = 32;
 constexpr int kMaxPairs = 2048;           // (token, choice) pairs of one call
 
+// What the later kernels need of a chosen expert.
+struct Chosen {
+    const uint8_t* tiles[3];              // gate, up, down
+    const __half* svh[3];
+    const __half* suh[3];
+    int K[3];
+    int expert;
+};
+
 struct MoeArgs {
     const void* x;
     int64_t ldx;
     int dtype;
     int T, D, F, E, top_k, normalize;
+    FastDiv kd, kf;                       // blocks of D and of F
     const void* router;
     int64_t ldr;
     int router_dtype;                     // 0 fp32, else XType
@@ -41,9 +53,11 @@ struct MoeArgs {
     int64_t ldo;
     // workspace
     int slots_max;                        // experts x groups of 8 G rows at most
-    int* ids;                             // [T * top_k]
+    Chosen* chosen;                       // [T * top_k]
     float* wts;                           // [T * top_k]
-    int* place;                           // [1 + T * top_k]: slots, then slot << 8 | row of a pair
+    int* place;                           // [T * top_k] slot << 8 | row of a pair
+    uint8_t* plan;                        // PlanHead and arrays
+    int ctas1, ctas2;                     // of the products
     uint8_t* xh1;                         // [2][T * top_k][D / 128][256], few_put_block order
     float* inv1;
     uint8_t* xh2;                         // [T * top_k][F / 128][256]
@@ -52,53 +66,129 @@ struct MoeArgs {
 };
 
 // ------------------------------------------------------------------ router
-constexpr int kRouterRanks = 8;
+constexpr int kRouterRanks = 4;            // CTAs of a cluster
+constexpr int kRouterWarps = 16;
+constexpr int kRouterThreads = 32 * kRouterWarps;
 
-// 8 products of a router row and x, summed in fp64.  bf16 and fp16 products are
-// exact in fp32; the choice of experts must not hang on the order of a sum, and a
-// conversion and an fp64 addition per product cost a microsecond at most.
-__device__ __forceinline__ double dot8(const MoeArgs& a, const uint4& xv, size_t off) {
-    float x[8];
-    if (a.dtype == X_BF16) {
+// A sum kept as a pair of fp32 (its value and the rounding errors' sum).  The choice of
+// experts must not hang on the batch, so a logit is always summed in the same order,
+// and should hang on rounding as little as it can: eight products at a time are summed
+// in fp32, those sums without loss, which leaves about 2^-28 of the logit.  (fp64
+// additions and conversions run at a 1/64 of the fp32 rate here: 7 us a token; the
+// lossless sum of every product cost 3 us more than this at 64 tokens.)
+struct PairSum {
+    float s = 0.0f, c = 0.0f;
+    __device__ __forceinline__ void add(float p) {      // two-sum (Knuth)
+        const float t = s + p, q = t - s;
+        c += (s - (t - q)) + (p - q);
+        s = t;
+    }
+    // (an infinite sum has no meaningful error term)
+    __device__ __forceinline__ double value() const { return c != c ? (double)s : (double)s + (double)c; }
+};
+
+__device__ __forceinline__ void unpack8(const uint4& v, int dtype, float (&x)[8]) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t u = (&xv.x)[j];
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t u = (&v.x)[j];
+        if (dtype == X_BF16) {
             x[2 * j] = __uint_as_float(u << 16);
             x[2 * j + 1] = __uint_as_float(u & 0xFFFF0000u);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&(&xv.x)[j]));
+        } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
             x[2 * j] = f.x;
             x[2 * j + 1] = f.y;
         }
     }
-    double s = 0.0;
-    if (a.router_dtype == 0) {
-        const float4* r = reinterpret_cast<const float4*>(static_cast<const float*>(a.router) + off);
-        const float4 r0 = r[0], r1 = r[1];
-        const float f[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
+}
+
+// Eight elements of a router row, as stored.
+template <bool F32> struct RouterPiece { uint4 v[F32 ? 2 : 1]; };
+
+template <bool F32>
+__device__ __forceinline__ RouterPiece<F32> load_router(const MoeArgs& a, size_t off) {
+    RouterPiece<F32> p;
+    const uint4* from = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.router) +
+                                                       off * (F32 ? 4 : 2));
+    p.v[0] = __ldg(from);
+    if (F32) p.v[F32] = __ldg(from + 1);
+    return p;
+}
+
+// acc += 8 products of x and a router row.
+template <bool F32>
+__device__ __forceinline__ void dot8(const MoeArgs& a, const float (&x)[8], const RouterPiece<F32>& p,
+                                     PairSum& acc) {
+    float r[8];
+    if (F32) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s = fma((double)x[j], (double)f[j], s);
+        for (int j = 0; j < 8; ++j) r[j] = __uint_as_float((&p.v[F32 ? j >> 2 : 0].x)[j & 3]);
     } else {
-        float r[4];
+        unpack8(p.v[0], a.dtype, r);
+    }
+    float q0 = x[0] * r[0], q1 = x[1] * r[1];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            load4x(a.router, off + 4 * h, a.router_dtype, r);
+    for (int j = 2; j < 8; j += 2) {
+        q0 = fmaf(x[j], r[j], q0);
+        q1 = fmaf(x[j + 1], r[j + 1], q1);
+    }
+    acc.add(q0 + q1);
+}
+
+// Logits of TT tokens (x rows at xr, pitch ldx elements) for experts e0 and, with EE = 2
+// and `two`, e1.  A warp.  The router's rows come from memory, so kBatch pieces of 256
+// columns are asked for before the first is used.
+template <bool F32, int TT, int EE>
+__device__ __forceinline__ void logits(const MoeArgs& a, const uint16_t* xr, int tokens, int e0, int e1,
+                                       bool two, double (&out)[EE][TT]) {
+    constexpr int kBatch = F32 ? 4 : 8;
+    const int lane = threadIdx.x & 31, n = a.D >> 3;
+    PairSum sum[EE][TT];
+    for (int c0 = lane; c0 < n; c0 += 32 * kBatch) {
+        RouterPiece<F32> r[EE][kBatch];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s += (double)(x[4 * h + j] * r[j]);
+        for (int q = 0; q < kBatch; ++q) {
+            const int c = c0 + 32 * q;
+            if (c < n) {
+                r[0][q] = load_router<F32>(a, (size_t)e0 * a.ldr + 8 * c);
+                if (EE == 2 && two) r[EE - 1][q] = load_router<F32>(a, (size_t)e1 * a.ldr + 8 * c);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < TT; ++k) {
+            if (k >= tokens) break;
+            uint4 xv[kBatch];
+#pragma unroll
+            for (int q = 0; q < kBatch; ++q)
+                if (c0 + 32 * q < n)
+                    xv[q] = __ldg(reinterpret_cast<const uint4*>(xr + (size_t)k * a.ldx) + c0 + 32 * q);
+#pragma unroll
+            for (int q = 0; q < kBatch; ++q) {
+                if (c0 + 32 * q < n) {
+                    float x[8];
+                    unpack8(xv[q], a.dtype, x);
+                    dot8<F32>(a, x, r[0][q], sum[0][k]);
+                    if (EE == 2 && two) dot8<F32>(a, x, r[EE - 1][q], sum[EE - 1][k]);
+                }
+            }
         }
     }
-    return s;
+#pragma unroll
+    for (int e = 0; e < EE; ++e)
+#pragma unroll
+        for (int k = 0; k < TT; ++k) {
+            out[e][k] = sum[e][k].value();
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) out[e][k] += __shfl_xor_sync(0xffffffffu, out[e][k], o);
+        }
 }
 
 // An order on fp64 values as integers; NaN counts as largest (its weights are NaN
-// whatever is chosen).
-__device__ __forceinline__ long long order_key(double v) {
-    if (v != v) return 0x7FFFFFFFFFFFFFFFLL;
-    const long long b = __double_as_longlong(v == 0.0 ? 0.0 : v);
-    return b < 0 ? b ^ 0x7FFFFFFFFFFFFFFFLL : b;
+// whatever is chosen), -0 as 0.
+__device__ __forceinline__ long long order_key(long long bits) {
+    const long long mag = bits & 0x7FFFFFFFFFFFFFFFLL;
+    if (mag > 0x7FF0000000000000LL) return 0x7FFFFFFFFFFFFFFFLL;
+    return bits < 0 ? -mag : mag;
 }
 
 __device__ __forceinline__ uint32_t peer(const void* p, int rank) {
@@ -108,173 +198,251 @@ __device__ __forceinline__ uint32_t peer(const void* p, int rank) {
     return addr;
 }
 
-// Cluster (8 CTAs) per token.  Its 64 warps share the experts' logits, which go to
-// every CTA; the CTAs share the experts again to find their place in the order (the
+// Cluster (4 CTAs) per TT tokens.  Its 64 warps share the experts' logits, which go to
+// every CTA; the CTAs share the experts again to find their places in the order (the
 // number of larger logits, and of equal ones before); an expert placed below top_k is
-// chosen.  Then all rotate the token for the chosen experts.
-__global__ void __cluster_dims__(kRouterRanks, 1, 1) __launch_bounds__(256)
+// chosen.
+template <bool F32, int TT>
+__global__ void __cluster_dims__(kRouterRanks, 1, 1) __launch_bounds__(kRouterThreads, 1)
 moe_router_kernel(const MoeArgs a) {
-    __shared__ double logit[kMaxExperts];
-    __shared__ int chosen[kMaxTopK];
-    __shared__ float share[kMaxTopK];
+    __shared__ long long logit[TT][kMaxExperts];      // fp64 bits
+    __shared__ int chosen[TT][kMaxTopK];
+    __shared__ float share[TT][kMaxTopK];
+    __shared__ double largest[TT];
+    __shared__ float total[TT];
     pdl_launch();
     cg::cluster_group cl = cg::this_cluster();
     auto started = cl.barrier_arrive();
-    const int rank = cl.block_rank(), token = blockIdx.y, t = threadIdx.x;
-    const int warp = t >> 5, lane = t & 31;
-    const uint4* xr = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) + token * a.ldx);
+    const int rank = cl.block_rank(), token0 = blockIdx.y * TT, t = threadIdx.x;
+    const int warp = t >> 5, lane = t & 31, tokens = min(TT, a.T - token0);
+    const uint16_t* xr = static_cast<const uint16_t*>(a.x) + (size_t)token0 * a.ldx;
+    constexpr int EE = TT == 1 ? 2 : 1, kWarps = kRouterRanks * kRouterWarps;
+    // the experts' table is wanted soon, and has left the cache since the last call
+    for (int i = t * 128; i < 3 * a.E * (int)sizeof(exl3b_expert); i += kRouterThreads * 128)
+        asm volatile("prefetch.global.L2 [%0];" :: "l"(reinterpret_cast<const uint8_t*>(a.experts) + i));
     bool wait = true;
-    for (int e0 = rank * 8 + warp; e0 < a.E; e0 += 16 * kRouterRanks) {
-        const int e1 = e0 + 8 * kRouterRanks;
-        const bool two = e1 < a.E;
-        double s0 = 0.0, s1 = 0.0;
-#pragma unroll 4
-        for (int c = lane; c < a.D / 8; c += 32) {
-            const uint4 xv = xr[c];
-            s0 += dot8(a, xv, (size_t)e0 * a.ldr + 8 * c);
-            if (two) s1 += dot8(a, xv, (size_t)e1 * a.ldr + 8 * c);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            s0 += __shfl_xor_sync(0xffffffffu, s0, o);
-            s1 += __shfl_xor_sync(0xffffffffu, s1, o);
-        }
+    for (int e0 = rank * kRouterWarps + warp; e0 < a.E; e0 += EE * kWarps) {
+        const int e1 = e0 + kWarps;
+        const bool two = EE == 2 && e1 < a.E;
+        double l[EE][TT];
+        logits<F32, TT, EE>(a, xr, tokens, e0, e1, two, l);
         if (wait) { cl.barrier_wait(std::move(started)); wait = false; }   // the others run
         if (lane < kRouterRanks) {
-            asm volatile("st.shared::cluster.f64 [%0], %1;" :: "r"(peer(logit + e0, lane)), "d"(s0) : "memory");
-            if (two)
-                asm volatile("st.shared::cluster.f64 [%0], %1;" :: "r"(peer(logit + e1, lane)), "d"(s1) : "memory");
+#pragma unroll
+            for (int k = 0; k < TT; ++k) {
+                asm volatile("st.shared::cluster.f64 [%0], %1;"
+                             :: "r"(peer(&logit[k][e0], lane)), "d"(l[0][k]) : "memory");
+                if (two)
+                    asm volatile("st.shared::cluster.f64 [%0], %1;"
+                                 :: "r"(peer(&logit[k][e1], lane)), "d"(l[EE - 1][k]) : "memory");
+            }
         }
     }
     if (wait) cl.barrier_wait(std::move(started));
     cl.sync();
-    // largest logit and softmax sum, in every warp
-    double m = -INFINITY;
-    for (int e = lane; e < a.E; e += 32) m = fmax(m, logit[e]);
+    if (warp < tokens) {       // largest logit and softmax sum
+        double m = -INFINITY;
+        for (int e = lane; e < a.E; e += 32) m = fmax(m, __longlong_as_double(logit[warp][e]));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float sum = 0.0f;
-    for (int e = lane; e < a.E; e += 32) sum += expf((float)(logit[e] - m));
+        for (int o = 16; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
+        float sum = 0.0f;
+        for (int e = lane; e < a.E; e += 32)
+            sum += expf((float)(__longlong_as_double(logit[warp][e]) - m));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    // 8 lanes count for one expert
-    for (int e = rank * 32 + (t >> 3); e - (t >> 3) < a.E; e += 32 * kRouterRanks) {
-        int place = 0;
-        if (e < a.E) {
-            const long long mine = order_key(logit[e]);
-            for (int o = t & 7; o < a.E; o += 8) {
-                const long long k = order_key(logit[o]);
-                place += k > mine || (k == mine && o < e);
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) { largest[warp] = m; total[warp] = sum; }
+    }
+    // 16 lanes count for one expert
+    const int q = t & 15, shared = (a.E + kRouterRanks - 1) / kRouterRanks;
+    for (int k = 0; k < tokens; ++k) {
+        for (int i0 = 0; i0 < shared; i0 += 2 * kRouterWarps) {
+            const int e = (i0 + (t >> 4)) * kRouterRanks + rank;
+            int place = 0;
+            if (e < a.E) {
+                const long long mine = order_key(logit[k][e]);
+                for (int o = q; o < a.E; o += 16) {
+                    const long long key = order_key(logit[k][o]);
+                    place += key > mine || (key == mine && o < e);
+                }
             }
-        }
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
-        if (e < a.E && place < a.top_k) {
-            const float p = expf((float)(logit[e] - m)) / sum;
-            asm volatile("st.shared::cluster.s32 [%0], %1;" :: "r"(peer(chosen + place, t & 7)), "r"(e) : "memory");
-            asm volatile("st.shared::cluster.f32 [%0], %1;" :: "r"(peer(share + place, t & 7)), "f"(p) : "memory");
+            for (int o = 1; o < 16; o <<= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+            if (e < a.E && place < a.top_k && q < kRouterRanks)
+                asm volatile("st.shared::cluster.s32 [%0], %1;"
+                             :: "r"(peer(&chosen[k][place], q)), "r"(e) : "memory");
         }
     }
     cl.sync();
-    if (rank == 0 && t < a.top_k) {
-        float all = 0.0f;
-        for (int j = 0; j < a.top_k; ++j) all += share[j];
-        a.ids[token * a.top_k + t] = chosen[t];
-        a.wts[token * a.top_k + t] = a.normalize ? share[t] / all : share[t];
-    }
-    // rotate the token for gate and up of every chosen expert
-    const int kd = a.D >> 7, P = a.T * a.top_k;
-#pragma unroll 2
-    for (int i = rank * 8 + warp; i < 2 * a.top_k * kd; i += 8 * kRouterRanks) {
-        const int m2 = i & 1, j = (i >> 1) % a.top_k, b = (i >> 1) / a.top_k, k = b * 128 + 4 * lane;
-        const exl3b_expert* w = a.experts + (size_t)m2 * a.E + chosen[j];
-        float v[4], s[4];
-        load4x(a.x, (size_t)token * a.ldx + k, a.dtype, v);
-        load4(static_cast<const __half*>(w->suh) + k, s);
+    // what is kept of token `rank`: a warp
+    for (int k = rank; k < tokens; k += kRouterRanks) {
+        if (warp != k / kRouterRanks || lane >= a.top_k) continue;
+        const int e = chosen[k][lane], to = (token0 + k) * a.top_k + lane;
+        Chosen c;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) v[c] *= s[c];
-        const size_t to = ((size_t)m2 * P + token * a.top_k + j) * kd + b;
-        few_put_block(v, a.xh1 + to * kRowBytes, a.inv1 + to, lane, 0);
+        for (int m = 0; m < 3; ++m) {
+            const exl3b_expert w = a.experts[(size_t)m * a.E + e];
+            c.tiles[m] = static_cast<const uint8_t*>(w.trellis);
+            c.svh[m] = static_cast<const __half*>(w.svh);
+            c.suh[m] = static_cast<const __half*>(w.suh);
+            c.K[m] = min(max(w.K, 2), a.Kmax[m]);
+        }
+        c.expert = e;
+        a.chosen[to] = c;
+        const float p = expf((float)(__longlong_as_double(logit[k][e]) - largest[k])) / total[k];
+        float sum = p;
+        if (a.normalize) {
+            share[k][lane] = p;
+            __syncwarp(a.top_k == 32 ? 0xffffffffu : (1u << a.top_k) - 1);
+            sum = 0.0f;
+            for (int j = 0; j < a.top_k; ++j) sum += share[k][j];
+        }
+        a.wts[to] = a.normalize ? p / sum : p;
     }
 }
 
 // ------------------------------------------------------------------ experts
 // The chosen experts in ascending order, each cut into slots of up to 8 G of its
 // (token, choice) pairs, which are in ascending order too; with the tensors of the
-// slots' experts, so that the product need not fetch them.
-struct Plan {
-    int* pair;                 // [P]
-    int2* slot;                // {expert, first pair << 8 | rows}
-    const uint8_t** tiles;     // [kinds][slots]
-    int* K;                    // [kinds][slots]
+// slots' experts.  Made once, in device memory; the products copy it to shared memory.
+struct PlanHead {
+    FewJoin join[2];           // the products' runs
     int slots;
 };
 
-__host__ __device__ inline int plan_bytes(int P, int slots_max, int kinds) {
-    return (P * 4 + 7) / 8 * 8 + slots_max * (8 + 12 * kinds);
+struct Plan {
+    const PlanHead* head;
+    int* pair;                 // [P]
+    int2* slot;                // [slots_max] {expert, first pair << 8 | rows}
+    const uint8_t** tiles;     // [3][slots_max + 1]
+    int* K;                    // [3][slots_max + 1]
+};
+
+__host__ __device__ inline int up16(int b) { return (b + 15) & ~15; }
+__host__ __device__ inline int plan_bytes(int P, int slots_max) {
+    return up16(sizeof(PlanHead)) + up16(P * 4) + up16(slots_max * 8) + up16(36 * (slots_max + 1));
+}
+__device__ __forceinline__ Plan plan_at(uint8_t* where, int P, int slots_max) {
+    Plan p;
+    p.head = reinterpret_cast<const PlanHead*>(where);
+    where += up16(sizeof(PlanHead));
+    p.pair = reinterpret_cast<int*>(where);
+    where += up16(P * 4);
+    p.slot = reinterpret_cast<int2*>(where);
+    where += up16(slots_max * 8);
+    p.tiles = reinterpret_cast<const uint8_t**>(where);
+    p.K = reinterpret_cast<int*>(where + 24 * (slots_max + 1));
+    return p;
 }
 
-// For tensors `first` .. first + kinds - 1 of every expert.  `tmp`: room for P + E ints.
-// `place`: where to note the pairs' slots (nullable).  All threads.
+constexpr int kPlanThreads = 512;
+
+// One CTA of kPlanThreads; `tmp`: 2 (P + E) ints of shared memory.
 template <int G>
-__device__ __forceinline__ Plan make_plan(const MoeArgs& a, int first, int kinds, uint8_t* where,
-                                          int* tmp, int* place) {
-    __shared__ int nslots;
-    const int t = threadIdx.x, P = a.T * a.top_k;
-    Plan p;
-    p.pair = reinterpret_cast<int*>(where);
-    p.slot = reinterpret_cast<int2*>(where + (P * 4 + 7) / 8 * 8);
-    p.tiles = reinterpret_cast<const uint8_t**>(p.slot + a.slots_max);
-    p.K = reinterpret_cast<int*>(p.tiles + kinds * a.slots_max);
-    int* count = tmp + P;
-    for (int i = t; i < P; i += blockDim.x) tmp[i] = a.ids[i];
+__device__ __forceinline__ void make_plan(const MoeArgs& a, int* tmp) {
+    __shared__ int totals[kPlanThreads / 32];
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31, P = a.T * a.top_k;
+    const Plan p = plan_at(a.plan, P, a.slots_max);
+    int* rank = tmp + P;       // [P] a pair's place among its expert's
+    int* count = rank + P;     // [E] pairs of an expert
+    int* from = count + a.E;   // [E] its first pair and slot
+    for (int e = t; e < a.E; e += kPlanThreads) count[e] = 0;
+    for (int i = t; i < P; i += kPlanThreads) tmp[i] = a.chosen[i].expert;
     __syncthreads();
-    for (int e = t; e < a.E; e += blockDim.x) {
-        int c = 0;
-        for (int i = 0; i < P; ++i) c += tmp[i] == e;
-        count[e] = c;
+    // in order, 32 pairs at a time
+    if (warp == 0) {
+        for (int base = 0; base < P; base += 32) {
+            const bool in = base + lane < P;
+            const int e = in ? tmp[base + lane] : -1;
+            const uint32_t same = __match_any_sync(0xffffffffu, e);
+            const int r = in ? count[e] + __popc(same & ((1u << lane) - 1)) : 0;
+            __syncwarp();
+            if (in) {
+                rank[base + lane] = r;
+                if ((same >> lane) == 1) count[e] = r + 1;      // the last of them
+            }
+            __syncwarp();
+        }
     }
     __syncthreads();
-    if (t < 32) {              // running sums of pairs (low half) and slots (high half)
-        int sum = 0;
-        for (int base = 0; base < a.E; base += 32) {
-            const int c = base + t < a.E ? count[base + t] : 0;
-            const int mine = c | ((c + 8 * G - 1) / (8 * G)) << 16;
-            int run = mine;
+    // running sums over two experts a thread: pairs in the low half, slots in the high
+    const int e0 = 2 * t, c0 = e0 < a.E ? count[e0] : 0, c1 = e0 + 1 < a.E ? count[e0 + 1] : 0;
+    const int m0 = c0 | (c0 + 8 * G - 1) / (8 * G) << 16, m1 = c1 | (c1 + 8 * G - 1) / (8 * G) << 16;
+    int sum = m0 + m1;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int up = __shfl_up_sync(0xffffffffu, run, o);
-                if (t >= o) run += up;
-            }
-            if (base + t < a.E) count[base + t] = sum + run - mine;
-            sum += __shfl_sync(0xffffffffu, run, 31);
-        }
-        if (t == 0) {
-            nslots = sum >> 16;
-            if (place) place[0] = nslots;
-        }
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += up;
+    }
+    if (lane == 31) totals[warp] = sum;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / 32; ++w) {
+        const int x = totals[w];
+        if (w < warp) before += x;
+        all += x;
+    }
+    const int slots = all >> 16, at0 = before + sum - m0 - m1;
+    if (e0 < a.E) from[e0] = at0;
+    if (e0 + 1 < a.E) from[e0 + 1] = at0 + m0;
+    if (t == kPlanThreads - 1) {
+        PlanHead* h = const_cast<PlanHead*>(p.head);
+        h->slots = slots;
+        h->join[0] = FewJoin(FewRun(a.kd, 2 * slots * (int)a.kf.d, a.ctas1));
+        h->join[1] = FewJoin(FewRun(a.kf, slots * (int)a.kd.d, a.ctas2));
     }
     __syncthreads();
-    p.slots = nslots;
-    for (int e = t; e < a.E; e += blockDim.x) {
-        const int from = count[e] & 0xFFFF;
-        int at = from, slot = count[e] >> 16;
-        for (int i = 0; i < P; ++i)
-            if (tmp[i] == e) {
-                if (place) place[1 + i] = (slot + (at - from) / (8 * G)) << 8 | (at - from) % (8 * G);
-                p.pair[at++] = i;
-            }
-        for (int r = from; r < at; r += 8 * G, ++slot) {
-            p.slot[slot] = make_int2(e, r << 8 | min(8 * G, at - r));
-            for (int m = 0; m < kinds; ++m) {
-                const exl3b_expert* w = a.experts + (size_t)(first + m) * a.E + e;
-                p.tiles[m * p.slots + slot] = static_cast<const uint8_t*>(w->trellis);
-                p.K[m * p.slots + slot] = min(max(w->K, 2), a.Kmax[first + m]);
-            }
+    for (int i = t; i < P; i += kPlanThreads) {
+        const int e = tmp[i], f = from[e], r = rank[i], slot = (f >> 16) + r / (8 * G);
+        p.pair[(f & 0xFFFF) + r] = i;
+        a.place[i] = slot << 8 | r % (8 * G);
+        if (r % (8 * G)) continue;
+        p.slot[slot] = make_int2(e, ((f & 0xFFFF) + r) << 8 | min(8 * G, count[e] - r));
+#pragma unroll
+        for (int m = 0; m < 3; ++m) {
+            p.tiles[m * (a.slots_max + 1) + slot] = a.chosen[i].tiles[m];
+            p.K[m * (a.slots_max + 1) + slot] = a.chosen[i].K[m];
         }
     }
+}
+
+// Rotate the tokens for gate and up of every chosen expert (a warp a block); the last
+// CTA makes the plan.
+template <int G>
+__global__ void __launch_bounds__(kPlanThreads) moe_rotate_kernel(const MoeArgs a, const FastDiv top_k) {
+    extern __shared__ __align__(16) uint8_t sm[];
+    pdl_wait();
+    pdl_launch();
+    if (blockIdx.x == gridDim.x - 1) {
+        make_plan<G>(a, reinterpret_cast<int*>(sm));
+        return;
+    }
+    const int lane = threadIdx.x & 31, P = a.T * a.top_k, kd = (int)a.kd.d;
+    const int i = blockIdx.x * (kPlanThreads / 32) + (threadIdx.x >> 5);      // (pair, block)
+    int pair;
+    const int b = a.kd.mod(i, pair), k = b * 128 + 4 * lane;
+    if (pair >= P) return;
+    float x[4], s[2][4];
+    load4x(a.x, (size_t)top_k.div(pair) * a.ldx + k, a.dtype, x);
+    load4(a.chosen[pair].suh[0] + k, s[0]);
+    load4(a.chosen[pair].suh[1] + k, s[1]);
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        float v[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c] = x[c] * s[m][c];
+        const size_t to = ((size_t)m * P + pair) * kd + b;
+        few_put_block(v, a.xh1 + to * kRowBytes, a.inv1 + to, lane, 0);
+    }
+}
+
+// The plan, copied to shared memory at `where`.  All threads.
+__device__ __forceinline__ Plan copy_plan(const MoeArgs& a, uint8_t* where) {
+    const int P = a.T * a.top_k, n = plan_bytes(P, a.slots_max) / 16;
+    const uint4* from = reinterpret_cast<const uint4*>(a.plan);
+    for (int i = threadIdx.x; i < n; i += blockDim.x) reinterpret_cast<uint4*>(where)[i] = __ldcg(from + i);
     __syncthreads();
-    return p;
+    return plan_at(where, P, a.slots_max);
 }
 
 // Units: (tensor, slot, column block); rows: rotated rows of the pairs.
@@ -285,72 +453,99 @@ struct ExpertJob {
     const Plan& p;
     const uint8_t* x;          // [kinds][P][kb][256]
     const float* s;
-    int kb, cols;              // blocks of a row, column blocks
+    int kb;                    // blocks of a row
+    const FastDiv& cols;       // column blocks
     bool early;                // the rows are there already
-    __device__ __forceinline__ FewUnit unit(int u) const {
-        const int v = u / cols, K = p.K[v];
-        return {p.tiles[v] + (size_t)(u - v * cols) * 256 * K, (uint32_t)cols * 256 * K, K};
+    int first, slots;          // the first unit's tensor; slots of each
+    struct Cursor {
+        const uint8_t* tiles;
+        uint32_t kt_bytes;
+        int K, m, s, left;         // tensor, slot; column blocks from here to the last
+    };
+    __device__ __forceinline__ void load(Cursor& c) const {
+        const int v = c.m * (a.slots_max + 1) + c.s;
+        c.K = p.K[v];
+        c.tiles = p.tiles[v];
+        c.kt_bytes = cols.d * 256 * c.K;
+        c.left = (int)cols.d;
     }
-    __device__ __forceinline__ int rows(int u) const { return p.slot[u / cols % p.slots].y & 0xFF; }
-    __device__ __forceinline__ size_t row(int u, int r, int b) const {
-        const int v = u / cols, m = v / p.slots;
-        return ((size_t)m * a.T * a.top_k + p.pair[(p.slot[v - m * p.slots].y >> 8) + r]) * kb + b;
+    __device__ __forceinline__ Cursor cursor(int u) const {
+        Cursor c;
+        int v;
+        const int nb = cols.mod(u, v);
+        c.m = first + (v >= slots);
+        c.s = v >= slots ? v - slots : v;
+        load(c);
+        c.tiles += (size_t)nb * 256 * c.K;
+        c.left -= nb;
+        return c;
     }
+    __device__ __forceinline__ void next(Cursor& c) const {
+        c.tiles += 256 * c.K;
+        if (--c.left == 0) {
+            if (++c.s == slots) { c.s = 0; ++c.m; }
+            if (c.m < 3) load(c);      // else past the last: not used
+        }
+    }
+    __device__ __forceinline__ int rows(int u) const {
+        const int v = cols.div(u);
+        return p.slot[v >= slots ? v - slots : v].y & 0xFF;
+    }
+    __device__ __forceinline__ size_t row(int u, int r) const {
+        const int v = cols.div(u), m = v >= slots;
+        return ((size_t)m * a.T * a.top_k + p.pair[(p.slot[m ? v - slots : v].y >> 8) + r]) * kb;
+    }
+    __device__ __forceinline__ int row_step() const { return 1; }
     __device__ __forceinline__ const uint8_t* xh() const { return x; }
     __device__ __forceinline__ const float* inv() const { return s; }
     __device__ __forceinline__ void wait() const { if (!early) pdl_wait(); }
 };
 
 template <int CODE, int G>
-__global__ void __launch_bounds__(32 * kFewWarps, 1) moe_gate_up_kernel(const MoeArgs a) {
+__global__ void __launch_bounds__(32 * kFewWarps, 1) moe_gate_up_kernel(const MoeArgs a, int plan) {
     extern __shared__ __align__(16) uint8_t sm[];
-    const int Kmax = max(a.Kmax[0], a.Kmax[1]);
     pdl_wait();
-    pdl_launch();              // from here on the router's results are there for everyone
-    const Plan p = make_plan<G>(a, 0, 2, sm + few_smem(Kmax), reinterpret_cast<int*>(sm),
-                                blockIdx.x == 0 ? a.place : nullptr);
-    const FewRun run(a.D >> 7, 2 * p.slots * (a.F >> 7), gridDim.x);
+    pdl_launch();              // from here on the plan is there for everyone
+    const Plan p = copy_plan(a, sm + plan);
+    const FewRun run = p.head->join[0].run;
     if (blockIdx.x >= run.ctas) return;
-    const ExpertJob<G> job = {a, p, a.xh1, a.inv1, a.D >> 7, a.F >> 7, true};
-    few_run<CODE, G>(job, run, Kmax, sm, a.park);
+    const ExpertJob<G> job = {a, p, a.xh1, a.inv1, (int)a.kd.d, a.kf, true, 0, p.head->slots};
+    few_run<CODE, G>(job, run, max(a.Kmax[0], a.Kmax[1]), sm, a.park);
 }
 
 template <int CODE, int G>
-__global__ void __launch_bounds__(32 * kFewWarps, 1) moe_down_kernel(const MoeArgs a) {
+__global__ void __launch_bounds__(32 * kFewWarps, 1) moe_down_kernel(const MoeArgs a, int plan) {
     extern __shared__ __align__(16) uint8_t sm[];
     pdl_launch();
-    const Plan p = make_plan<G>(a, 2, 1, sm + few_smem(a.Kmax[2]), reinterpret_cast<int*>(sm), nullptr);
-    const FewRun run(a.F >> 7, p.slots * (a.D >> 7), gridDim.x);
+    const Plan p = copy_plan(a, sm + plan);
+    const FewRun run = p.head->join[1].run;
     if (blockIdx.x >= run.ctas) return;
-    const ExpertJob<G> job = {a, p, a.xh2, a.inv2, a.F >> 7, a.D >> 7, false};
+    const ExpertJob<G> job = {a, p, a.xh2, a.inv2, (int)a.kf.d, a.kd, false, 2, p.head->slots};
     few_run<CODE, G>(job, run, a.Kmax[2], sm, a.park);
 }
 
 // h = silu(gate) * up of a (pair, column block of F), and the down projection's rotated
-// row: a CTA each; two warps add the gate's parked sums, two those of up.
+// row: a warp each.
 template <int G>
-__global__ void __launch_bounds__(128) moe_gate_up_finish_kernel(const MoeArgs a, int ctas) {
-    __shared__ float4 sum[3][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int fb = blockIdx.x, pair = blockIdx.y, f = fb * 128 + 4 * lane, fbn = gridDim.x;
+__global__ void __launch_bounds__(128) moe_gate_up_finish_kernel(const MoeArgs a) {
+    const int lane = threadIdx.x & 31, i = blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int fbn = (int)a.kf.d;
+    int pair;
+    const int fb = a.kf.mod(i, pair), f = fb * 128 + 4 * lane;
     pdl_wait();
     pdl_launch();
-    const int e = a.ids[pair], slots = a.place[0], at = a.place[1 + pair];
-    float sg[4], su[4], sd[4], v[4];
-    if (warp == 0) {
-        load4(static_cast<const __half*>(a.experts[e].svh) + f, sg);
-        load4(static_cast<const __half*>(a.experts[a.E + e].svh) + f, su);
-        load4(static_cast<const __half*>(a.experts[2 * a.E + e].suh) + f, sd);
-    }
-    const FewRun run(a.D >> 7, 2 * slots * fbn, ctas);
-    few_sum<G>(a.park, run, ((warp >> 1) * slots + (at >> 8)) * fbn + fb, at & 0xFF, lane, warp & 1, 2, v);
-    if (warp) sum[warp - 1][lane] = make_float4(v[0], v[1], v[2], v[3]);
-    __syncthreads();
-    if (warp) return;
-    add4(v, sum[0][lane]);
-    float h[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    add4(h, sum[1][lane]);
-    add4(h, sum[2][lane]);
+    if (pair >= a.T * a.top_k) return;
+    const Chosen c = a.chosen[pair];
+    const int at = a.place[pair];
+    const FewJoin join = reinterpret_cast<const PlanHead*>(a.plan)->join[0];
+    float sg[4], su[4], sd[4], v[4], h[4];
+    load4(c.svh[0] + f, sg);
+    load4(c.svh[1] + f, su);
+    load4(c.suh[2] + f, sd);
+    const int ug = (at >> 8) * fbn + fb, uu = ug + join.run.units / 2;
+    const FewParts pg(join, ug), pu(join, uu);
+    few_sum<G>(a.park, join, pg, ug, at & 0xFF, lane, 0, 1, v);
+    few_sum<G>(a.park, join, pu, uu, at & 0xFF, lane, 0, 1, h);
     few_rotate_back(v, lane);
     few_rotate_back(h, lane);
 #pragma unroll
@@ -362,20 +557,21 @@ __global__ void __launch_bounds__(128) moe_gate_up_finish_kernel(const MoeArgs a
 // Weighted sum over a token's experts of one column block, and the residual: a CTA
 // each, whose four warps take every fourth expert in the order of choice.
 template <int G>
-__global__ void __launch_bounds__(128) moe_down_finish_kernel(const MoeArgs a, int ctas) {
+__global__ void __launch_bounds__(128) moe_down_finish_kernel(const MoeArgs a) {
     __shared__ float4 sum[3][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int nb = blockIdx.x, token = blockIdx.y, n = nb * 128 + 4 * lane, nbn = gridDim.x;
     float res[4] = {0.0f, 0.0f, 0.0f, 0.0f}, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (warp == 0 && a.residual) load4x(a.residual, (size_t)token * a.ldres + n, a.dtype, res);
     pdl_wait();
-    const FewRun run(a.F >> 7, a.place[0] * nbn, ctas);
+    const FewJoin join = reinterpret_cast<const PlanHead*>(a.plan)->join[1];
     for (int j = warp; j < a.top_k; j += 4) {
-        const int pair = token * a.top_k + j, at = a.place[1 + pair];
+        const int pair = token * a.top_k + j, at = a.place[pair], u = (at >> 8) * nbn + nb;
         float v[4], s[4];
-        load4(static_cast<const __half*>(a.experts[2 * a.E + a.ids[pair]].svh) + n, s);
+        load4(a.chosen[pair].svh[2] + n, s);
         const float wt = a.wts[pair];
-        few_sum<G>(a.park, run, (at >> 8) * nbn + nb, at & 0xFF, lane, 0, 1, v);
+        const FewParts parts(join, u);
+        few_sum<G>(a.park, join, parts, u, at & 0xFF, lane, 0, 1, v);
         few_rotate_back(v, lane);
 #pragma unroll
         for (int c = 0; c < 4; ++c) y[c] = fmaf(v[c], s[c] * wt, y[c]);
@@ -410,9 +606,10 @@ static size_t moe_layout(MoeArgs* a, int T, int D, int F, int E, int top_k, int 
     auto take = [&](size_t bytes) { const size_t o = off; off += up256(bytes); return ws + o; };
     const size_t park1 = few_park_bytes((int)(2 * slots * kf), sms, G);
     const size_t park2 = few_park_bytes((int)(slots * kd), sms, G);
-    uint8_t* ids = take(P * 4);
+    uint8_t* chosen = take(P * sizeof(Chosen));
     uint8_t* wts = take(P * 4);
-    uint8_t* place = take((1 + P) * 4);
+    uint8_t* place = take(P * 4);
+    uint8_t* plan = take(plan_bytes((int)P, slots));
     uint8_t* xh1 = take(2 * P * kd * kRowBytes);
     uint8_t* inv1 = take(2 * P * kd * 4);
     uint8_t* xh2 = take(P * kf * kRowBytes);
@@ -420,9 +617,13 @@ static size_t moe_layout(MoeArgs* a, int T, int D, int F, int E, int top_k, int 
     uint8_t* park = take(park1 > park2 ? park1 : park2);
     if (a) {
         a->slots_max = slots;
-        a->ids = reinterpret_cast<int*>(ids);
+        a->chosen = reinterpret_cast<Chosen*>(chosen);
         a->wts = reinterpret_cast<float*>(wts);
         a->place = reinterpret_cast<int*>(place);
+        a->plan = plan;
+        const long long t1 = 2LL * slots * kd * kf, t2 = t1 / 2;
+        a->ctas1 = (int)(t1 < sms ? t1 : sms);
+        a->ctas2 = (int)(t2 < sms ? t2 : sms);
         a->xh1 = xh1;
         a->inv1 = reinterpret_cast<float*>(inv1);
         a->xh2 = xh2;
@@ -434,24 +635,34 @@ static size_t moe_layout(MoeArgs* a, int T, int D, int F, int E, int top_k, int 
 
 template <int CODE, int G>
 static int moe_run(const MoeArgs& a, int sms, cudaStream_t stream) {
-    int rc = launch_kernel(moe_router_kernel, "moe_router launch", dim3(kRouterRanks, a.T), 256, 0, false,
-                           stream, a);
-    if (rc) return rc;
     const int P = a.T * a.top_k, kd = a.D >> 7, kf = a.F >> 7;
-    const int K1 = a.Kmax[0] > a.Kmax[1] ? a.Kmax[0] : a.Kmax[1];
-    const long long t1 = 2LL * a.slots_max * kf * kd, t2 = t1 / 2;
-    const int c1 = (int)(t1 < sms ? t1 : sms), c2 = (int)(t2 < sms ? t2 : sms);
-    rc = launch_kernel(moe_gate_up_kernel<CODE, G>, "moe_gate_up launch", dim3(c1), 32 * kFewWarps,
-                       few_smem(K1) + plan_bytes(P, a.slots_max, 2), true, stream, a);
+    // tokens of a cluster: as many as it takes for all clusters to run at once
+    const int most = sms / kRouterRanks, tt = a.T <= most ? 1 : a.T <= 2 * most ? 2 : 4;
+    auto router = a.router_dtype == 0 ? (tt == 1 ? moe_router_kernel<true, 1> :
+                                         tt == 2 ? moe_router_kernel<true, 2> : moe_router_kernel<true, 4>)
+                                      : (tt == 1 ? moe_router_kernel<false, 1> :
+                                         tt == 2 ? moe_router_kernel<false, 2> : moe_router_kernel<false, 4>);
+    int rc = launch_kernel(router, "moe_router launch", dim3(kRouterRanks, (a.T + tt - 1) / tt),
+                           kRouterThreads, 0, false, stream, a);
     if (rc) return rc;
-    rc = launch_kernel(moe_gate_up_finish_kernel<G>, "moe_gate_up_finish launch", dim3(kf, P), 128, 0,
-                       true, stream, a, c1);
+    constexpr int kWarps = kPlanThreads / 32;
+    rc = launch_kernel(moe_rotate_kernel<G>, "moe_rotate launch", dim3((P * kd + kWarps - 1) / kWarps + 1),
+                       kPlanThreads, 8 * (P + a.E), true, stream, a, FastDiv(a.top_k));
     if (rc) return rc;
-    rc = launch_kernel(moe_down_kernel<CODE, G>, "moe_down launch", dim3(c2), 32 * kFewWarps,
-                       few_smem(a.Kmax[2]) + plan_bytes(P, a.slots_max, 1), true, stream, a);
+    const int K1 = a.Kmax[0] > a.Kmax[1] ? a.Kmax[0] : a.Kmax[1], plan = plan_bytes(P, a.slots_max);
+    const int at1 = up16(few_smem(K1, G, kFewGroups * kRowStages));
+    const int at2 = up16(few_smem(a.Kmax[2], G, kFewGroups * kRowStages));
+    rc = launch_kernel(moe_gate_up_kernel<CODE, G>, "moe_gate_up launch", dim3(a.ctas1), 32 * kFewWarps,
+                       at1 + plan, true, stream, a, at1);
+    if (rc) return rc;
+    rc = launch_kernel(moe_gate_up_finish_kernel<G>, "moe_gate_up_finish launch", dim3((P * kf + 3) / 4),
+                       128, 0, true, stream, a);
+    if (rc) return rc;
+    rc = launch_kernel(moe_down_kernel<CODE, G>, "moe_down launch", dim3(a.ctas2), 32 * kFewWarps,
+                       at2 + plan, true, stream, a, at2);
     if (rc) return rc;
     return launch_kernel(moe_down_finish_kernel<G>, "moe_down_finish launch", dim3(kd, a.T), 128, 0, true,
-                         stream, a, c2);
+                         stream, a);
 }
 
 }  // namespace exl3b
@@ -520,7 +731,10 @@ int exl3b_moe(const void* dX, int dtype, int64_t ldx, int T, int D, int F, int E
         set_error("moe: workspace %zu < %zu bytes or misaligned", ws_bytes, need);
         return RC_WORKSPACE;
     }
-    MoeArgs a = {};
+    MoeArgs a;
+    memset(&a, 0, sizeof(a));
+    a.kd = FastDiv(D / 128);
+    a.kf = FastDiv(F / 128);
     a.x = dX; a.ldx = ldx; a.dtype = dtype;
     a.T = T; a.D = D; a.F = F; a.E = E; a.top_k = top_k; a.normalize = normalize;
     a.router = dRouter; a.ldr = ldr; a.router_dtype = router_dtype;

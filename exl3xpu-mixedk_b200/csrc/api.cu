@@ -131,6 +131,10 @@ static int init_device_locked(int dev, DeviceState* st) {
                        "cudaMemcpy(lut32)"))
             return RC_DEVICE_ERROR;
     }
+    if (check_cuda(cudaHostAlloc(&st->fwd_err, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable),
+                   "cudaHostAlloc(status)"))
+        return RC_ALLOC;
+    *st->fwd_err = 0;
     st->ready = true;
     return RC_OK;
 }

@@ -27,6 +27,9 @@ struct DeviceState {
     // block LDL lookahead: a high-priority helper stream and fork / join events
     cudaStream_t side = nullptr;
     cudaEvent_t ev_fork = nullptr, ev_join = nullptr;
+    // set by a forward kernel whose bounded wait ran out (pinned host memory, mapped:
+    // the kernels are asynchronous, so the next forward call reports it)
+    int* fwd_err = nullptr;
 };
 
 // Kernel-launch accounting (exl3b_launch_count) and optional per-launch

@@ -5,7 +5,7 @@
 // weights, so the weight is only ever read as its trellis (K / 8 bytes per weight).
 
 #include "exl3b_internal.h"
-#include "forward_few.cuh"
+#include "forward_mid.cuh"
 #include "../../include/exl3b200.h"
 
 namespace exl3b {
@@ -133,10 +133,10 @@ linear_finish_kernel(const LinearArgs a, const FewScratch w, const FewJoin join)
     LinearEpilogue ep;
     if (warp == 0) ep.load(a, row, col);
     const int u = row / (8 * G) * gridDim.x + nb;
-    const FewParts parts(join, u);
+    const FewParts<kFewGroups> parts(join, u);
     pdl_wait();
     float v[4];
-    few_sum<G>(w.park, join, parts, u, row % (8 * G), lane, warp, 4, v);
+    few_sum(w.park, join, parts, u, 8 * G, row % (8 * G), lane, warp, 4, v);
     if (warp) sum[warp - 1][lane] = make_float4(v[0], v[1], v[2], v[3]);
     __syncthreads();
     if (warp) return;
@@ -207,6 +207,181 @@ static int few_dispatch(const LinearArgs& a, int sms, uint8_t* ws, cudaStream_t 
 #undef EXL3B_FEW
 }
 
+// ------------------------------------------------------------------ more rows
+// suh, rotation and rounding of whole rows, a CTA each: fp16 [M][k] in the order of k,
+// times one power of two a row (its reciprocal in inv [M]), since the matrix unit sums
+// over all of k.  The largest magnitude of the row sets it as in block_scale: entries
+// 2^-25 of it and below lose bits, which is below the rounding of the sum.
+__global__ void __launch_bounds__(256) linear_rotate_rows_kernel(const LinearArgs a, __half* xh, float* inv) {
+    __shared__ float part[8];
+    pdl_launch();
+    const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kb = a.k >> 7;
+    const size_t at = (size_t)row * a.ldx + 4 * lane;
+    float m = 0.0f;
+    for (int b = warp; b < kb; b += 8) {
+        float v[4], s[4];
+        load4x(a.x, at + b * 128, a.dtype, v);
+        load4(a.suh + b * 128 + 4 * lane, s);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m = fmaxf(m, fabsf(v[j] * s[j]));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) part[warp] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) m = fmaxf(m, part[w]);
+    float back;
+    const float scale = block_scale(m, back) * kInvSqrt128;
+    if (threadIdx.x == 0) inv[row] = back;
+    for (int b = warp; b < kb; b += 8) {
+        float v[4], s[4];
+        load4x(a.x, at + b * 128, a.dtype, v);
+        load4(a.suh + b * 128 + 4 * lane, s);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = v[j] * s[j] * scale;
+        had128_warp(v, lane);
+        store4(xh + (size_t)row * a.k + b * 128 + 4 * lane, v);
+    }
+}
+
+// Sum of a unit's parked sums of one row, output rotation and epilogue: a warp each.
+__global__ void __launch_bounds__(128)
+linear_mid_finish_kernel(const LinearArgs a, const MidArgs w, const FewJoin join, const float* inv) {
+    const int lane = threadIdx.x & 31, nb = blockIdx.x, row = blockIdx.y * 4 + (threadIdx.x >> 5);
+    if (row >= a.M) return;
+    const int col = nb * 128 + 4 * lane, pass = row / w.N, u = pass * w.nbn + nb;
+    LinearEpilogue ep;
+    ep.load(a, row, col);
+    const FewParts<1> parts(join, u);
+    pdl_wait();
+    float v[4];
+    few_sum(w.park, join, parts, u, w.N, row - pass * w.N, lane, 0, 1, v);
+    const float f = inv[row];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] *= f;
+    few_rotate_back(v, lane);
+    ep.finish(a, row, col, v);
+}
+
+// cuTensorMapEncodeTiled is a driver-API entry point, resolved at run time through the
+// runtime: the library has no link dependency on libcuda.
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                CUtensorMapFloatOOBfill);
+
+// Boxes of 64 x box_rows of a row-major fp16 matrix [rows][k], 128-byte swizzle.
+static int encode_rows(CUtensorMap* map, const void* base, int k, int rows, int box_rows) {
+    static EncodeTiled fn = nullptr;
+    if (!fn) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess) {
+            set_error("cuTensorMapEncodeTiled unavailable from the driver");
+            return RC_DEVICE_ERROR;
+        }
+        fn = reinterpret_cast<EncodeTiled>(p);
+    }
+    const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)k * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, one[2] = {1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box,
+                          one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("cuTensorMapEncodeTiled failed (%d)", (int)r);
+        return RC_DEVICE_ERROR;
+    }
+    return RC_OK;
+}
+
+struct MidScratch {
+    __half* xh;                // [M][k]
+    float* inv;                // [M]
+    float* park;
+};
+
+// Passes of equal size, rows rounded up to what the matrix unit takes.
+static int mid_rows(int M) {
+    const int passes = (M + kMidRows - 1) / kMidRows;
+    return ((M + passes - 1) / passes + 15) / 16 * 16;
+}
+
+static FewRun mid_run(int M, int k, int n, int sms) {
+    const int N = mid_rows(M);
+    return FewRun(FastDiv(k >> 7), (n >> 7) * ((M + N - 1) / N), sms);
+}
+
+static size_t mid_layout(MidScratch* w, int M, int k, int n, int sms, uint8_t* ws) {
+    const FewRun run = mid_run(M, k, n, sms);
+    size_t off = 0;
+    auto take = [&](size_t bytes) { const size_t o = off; off += up256(bytes); return ws + o; };
+    w->xh = reinterpret_cast<__half*>(take((size_t)M * k * 2));
+    w->inv = reinterpret_cast<float*>(take((size_t)M * 4));
+    w->park = reinterpret_cast<float*>(take((size_t)(run.units + run.ctas) * mid_rows(M) * 512));
+    return off;
+}
+
+template <int CODE>
+static int mid_launch(const LinearArgs& a, DeviceState* st, uint8_t* ws, cudaStream_t stream) {
+    MidScratch w;
+    mid_layout(&w, a.M, a.k, a.n, st->sms, ws);
+    MidArgs m;
+    m.trellis = a.trellis;
+    m.K = a.K;
+    m.nbn = a.n >> 7;
+    m.M = a.M;
+    m.N = mid_rows(a.M);
+    m.run = mid_run(a.M, a.k, a.n, st->sms);
+    m.park = w.park;
+    m.err = st->fwd_err;
+    const int fit = (kFewRoom - mid_smem(a.K, m.N, 0)) / (m.N * 256);
+    m.stages = fit < 4 ? fit : 4;
+    CUtensorMap rows;
+    int rc = encode_rows(&rows, w.xh, a.k, a.M, m.N);
+    if (rc) return rc;
+    rc = launch_kernel(linear_rotate_rows_kernel, "linear_rotate_rows launch", dim3(a.M), 256, 0, false,
+                       stream, a, w.xh, w.inv);
+    if (rc) return rc;
+    rc = launch_kernel(linear_mid_kernel<CODE>, "linear_mid launch", dim3(m.run.ctas), kMidThreads,
+                       mid_smem(a.K, m.N, m.stages), true, stream, rows, m);
+    if (rc) return rc;
+    return launch_kernel(linear_mid_finish_kernel, "linear_mid_finish launch",
+                         dim3(m.nbn, (a.M + 3) / 4), 128, 0, true, stream, a, m, FewJoin(m.run),
+                         (const float*)w.inv);
+}
+
+// ------------------------------------------------------------------ which path
+constexpr int kFewMost = 16;
+
+static size_t linear_bytes(int M, int k, int n, int sms) {
+    if (M <= kFewMost) {
+        FewScratch w;
+        return few_layout(&w, M, k, n, few_groups(M), sms, nullptr);
+    }
+    MidScratch w;
+    return mid_layout(&w, M, k, n, sms, nullptr);
+}
+
+static int linear_run_all(const LinearArgs& a, DeviceState* st, uint8_t* ws, cudaStream_t stream) {
+    if (a.M <= kFewMost) return few_dispatch(a, st->sms, ws, stream);
+    switch (a.code) {
+        case CODE_MUL1: return mid_launch<CODE_MUL1>(a, st, ws, stream);
+        case CODE_3INST: return mid_launch<CODE_3INST>(a, st, ws, stream);
+        default: return mid_launch<CODE_MCG>(a, st, ws, stream);
+    }
+}
+
+// A forward kernel's bounded wait ran out in an earlier call.
+int forward_status(DeviceState* st) {
+    volatile int* e = st->fwd_err;
+    if (*e == 0) return RC_OK;
+    *e = 0;
+    set_error("a wait inside an earlier forward kernel ran out; its results are not valid");
+    return RC_DEVICE_ERROR;
+}
+
 }  // namespace exl3b
 
 using namespace exl3b;
@@ -233,8 +408,7 @@ size_t exl3b_linear_workspace_bytes(int M, int k, int n) {
     if (M <= 0 || k <= 0 || n <= 0 || k % 128 || n % 128) return 0;
     const int sms = device_sms();
     if (sms <= 0) return 0;
-    FewScratch w;
-    return few_layout(&w, M, k, n, few_groups(M), sms, nullptr);
+    return linear_bytes(M, k, n, sms);
 }
 
 int exl3b_linear(const void* dX, int dtype, int64_t ldx, int M, int k, int n,
@@ -272,7 +446,9 @@ int exl3b_linear(const void* dX, int dtype, int64_t ldx, int M, int k, int n,
     LinearArgs a = {dX, ldx, dtype, M, k, n, reinterpret_cast<const uint8_t*>(dTrellis), K, code,
                     static_cast<const __half*>(d_suh_f16), static_cast<const __half*>(d_svh_f16),
                     d_bias, act, d_mul, ldmul, d_residual, ldres, dOut, ldo};
-    return few_dispatch(a, st->sms, static_cast<uint8_t*>(ws), static_cast<cudaStream_t>(stream));
+    const int rc = forward_status(st);
+    if (rc) return rc;
+    return linear_run_all(a, st, static_cast<uint8_t*>(ws), static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -434,33 +434,39 @@ __device__ __forceinline__ void few_run(const Job& job, const FewRun& run, int K
     }
 }
 
-// Sum of unit u's parked sums of row r, elements 4 lane .. 4 lane + 3: the ones at
-// `part`, part + parts, ... in the order of the CTAs and their groups.  A warp.
+// The parked sums of unit u: GROUPS per CTA of its run.
+template <int GROUPS>
 struct FewParts {
     int lo, hi, c0, n;
     __device__ __forceinline__ FewParts(const FewJoin& j, int u) {
         lo = u * (int)j.run.kb.d;
         hi = lo + (int)j.run.kb.d;
         c0 = j.owner(lo);
-        n = (j.owner(hi - 1) - c0 + 1) * kFewGroups;
+        n = (j.owner(hi - 1) - c0 + 1) * GROUPS;
     }
 };
 
-template <int G>
-__device__ __forceinline__ void few_sum(const float* park, const FewJoin& join, const FewParts& p, int u,
-                                        int r, int lane, int part, int parts, float (&v)[4]) {
-    const float* from = park + (size_t)(u + p.c0) * kFewGroups * 8 * G * 128 + r * 128 + 4 * lane;
+// Sum of unit u's parked sums of row r (of `rows` a slot), elements 4 lane ..
+// 4 lane + 3: the ones at `part`, part + parts, ... in the order of the CTAs and their
+// groups.  A warp.
+template <int GROUPS>
+__device__ __forceinline__ void few_sum(const float* park, const FewJoin& join, const FewParts<GROUPS>& p,
+                                        int u, int rows, int r, int lane, int part, int parts,
+                                        float (&v)[4]) {
+    const size_t slot = (size_t)rows * 128;
+    const float* from = park + (size_t)(u + p.c0) * GROUPS * slot + r * 128 + 4 * lane;
     v[0] = v[1] = v[2] = v[3] = 0.0f;
 #pragma unroll 4
     for (int i = part; i < p.n; i += parts) {
-        const int c = p.c0 + i / kFewGroups, g = i % kFewGroups;
-        const int s = join.run.start(c), e = join.run.start(c + 1);
-        const int f = s > p.lo ? s : p.lo, l = e < p.hi ? e : p.hi;      // the CTA's blocks of u
-        // a group takes every other block of the run: none of a single one, maybe
-        if (l - f >= kFewGroups || ((f - s) & 1) == g) {
-            const float4 q = __ldcg(reinterpret_cast<const float4*>(from + (size_t)i * 8 * G * 128));
-            v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
+        if (GROUPS > 1) {
+            const int c = p.c0 + i / GROUPS, g = i % GROUPS;
+            const int s = join.run.start(c), e = join.run.start(c + 1);
+            const int f = s > p.lo ? s : p.lo, l = e < p.hi ? e : p.hi;      // the CTA's blocks of u
+            // a group takes every other block of the run: none of a single one, maybe
+            if (l - f < GROUPS && ((f - s) & 1) != g) continue;
         }
+        const float4 q = __ldcg(reinterpret_cast<const float4*>(from + i * slot));
+        v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
     }
 }
 

@@ -543,9 +543,9 @@ __global__ void __launch_bounds__(128) moe_gate_up_finish_kernel(const MoeArgs a
     load4(c.svh[1] + f, su);
     load4(c.suh[2] + f, sd);
     const int ug = (at >> 8) * fbn + fb, uu = ug + join.run.units / 2;
-    const FewParts pg(join, ug), pu(join, uu);
-    few_sum<G>(a.park, join, pg, ug, at & 0xFF, lane, 0, 1, v);
-    few_sum<G>(a.park, join, pu, uu, at & 0xFF, lane, 0, 1, h);
+    const FewParts<kFewGroups> pg(join, ug), pu(join, uu);
+    few_sum(a.park, join, pg, ug, 8 * G, at & 0xFF, lane, 0, 1, v);
+    few_sum(a.park, join, pu, uu, 8 * G, at & 0xFF, lane, 0, 1, h);
     few_rotate_back(v, lane);
     few_rotate_back(h, lane);
 #pragma unroll
@@ -570,8 +570,8 @@ __global__ void __launch_bounds__(128) moe_down_finish_kernel(const MoeArgs a) {
         float v[4], s[4];
         load4(a.chosen[pair].svh[2] + n, s);
         const float wt = a.wts[pair];
-        const FewParts parts(join, u);
-        few_sum<G>(a.park, join, parts, u, at & 0xFF, lane, 0, 1, v);
+        const FewParts<kFewGroups> parts(join, u);
+        few_sum(a.park, join, parts, u, 8 * G, at & 0xFF, lane, 0, 1, v);
         few_rotate_back(v, lane);
 #pragma unroll
         for (int c = 0; c < 4; ++c) y[c] = fmaf(v[c], s[c] * wt, y[c]);

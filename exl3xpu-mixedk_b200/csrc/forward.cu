@@ -5,7 +5,7 @@
 // weights, so the weight is only ever read as its trellis (K / 8 bytes per weight).
 
 #include "exl3b_internal.h"
-#include "forward_mid.cuh"
+#include "forward_gemm.cuh"
 #include "../../include/exl3b200.h"
 
 namespace exl3b {
@@ -208,10 +208,11 @@ static int few_dispatch(const LinearArgs& a, int sms, uint8_t* ws, cudaStream_t 
 }
 
 // ------------------------------------------------------------------ more rows
-// suh, rotation and rounding of whole rows, a CTA each: fp16 [M][k] in the order of k,
-// times one power of two a row (its reciprocal in inv [M]), since the matrix unit sums
+// suh, rotation and rounding of whole rows, a CTA each: fp16 [M][k] in the order of k
+// (PAIRED: each 32 k in few_put_block's order, as linear_expand_kernel's), times one power of two a row (its reciprocal in inv [M]), since the matrix unit sums
 // over all of k.  The largest magnitude of the row sets it as in block_scale: entries
 // 2^-25 of it and below lose bits, which is below the rounding of the sum.
+template <bool PAIRED>
 __global__ void __launch_bounds__(256) linear_rotate_rows_kernel(const LinearArgs a, __half* xh, float* inv) {
     __shared__ float part[8];
     pdl_launch();
@@ -241,7 +242,15 @@ __global__ void __launch_bounds__(256) linear_rotate_rows_kernel(const LinearArg
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = v[j] * s[j] * scale;
         had128_warp(v, lane);
-        store4(xh + (size_t)row * a.k + b * 128 + 4 * lane, v);
+        __half* to = xh + (size_t)row * a.k + b * 128;
+        if (PAIRED) {
+            const int k = 4 * lane;
+            to += (k >> 5) * 32 + ((k & 7) >> 1) * 8 + ((k >> 4) & 1) * 4 + ((k >> 3) & 1) * 2;
+            *reinterpret_cast<__half2*>(to) = __floats2half2_rn(v[0], v[1]);
+            *reinterpret_cast<__half2*>(to + 8) = __floats2half2_rn(v[2], v[3]);
+        } else {
+            store4(to + 4 * lane, v);
+        }
     }
 }
 
@@ -341,7 +350,7 @@ static int mid_launch(const LinearArgs& a, DeviceState* st, uint8_t* ws, cudaStr
     CUtensorMap rows;
     int rc = encode_rows(&rows, w.xh, a.k, a.M, m.N);
     if (rc) return rc;
-    rc = launch_kernel(linear_rotate_rows_kernel, "linear_rotate_rows launch", dim3(a.M), 256, 0, false,
+    rc = launch_kernel(linear_rotate_rows_kernel<false>, "linear_rotate_rows launch", dim3(a.M), 256, 0, false,
                        stream, a, w.xh, w.inv);
     if (rc) return rc;
     rc = launch_kernel(linear_mid_kernel<CODE>, "linear_mid launch", dim3(m.run.ctas), kMidThreads,
@@ -352,25 +361,132 @@ static int mid_launch(const LinearArgs& a, DeviceState* st, uint8_t* ws, cudaStr
                          (const float*)w.inv);
 }
 
+// ------------------------------------------------------------------ long prompts
+struct LinearRows {
+    LinearArgs a;
+    bool wide;                 // rows of mul, residual and out on 16-byte boundaries
+    // 128 columns of a row held by a thread: scale, svh, epilogue.
+    __device__ __forceinline__ void finish128(int row, int col, float f, float (&v)[128]) const {
+        const uint16_t* mul = a.mul ? static_cast<const uint16_t*>(a.mul) + (size_t)row * a.ldmul + col : nullptr;
+        const uint16_t* res =
+            a.residual ? static_cast<const uint16_t*>(a.residual) + (size_t)row * a.ldres + col : nullptr;
+        uint16_t* out = static_cast<uint16_t*>(a.out) + (size_t)row * a.ldo + col;
+#pragma unroll
+        for (int i = 0; i < 128; i += 8) {
+            float s[8], t[8];
+            load4(a.svh + col + i, *reinterpret_cast<float(*)[4]>(s));
+            load4(a.svh + col + i + 4, *reinterpret_cast<float(*)[4]>(s + 4));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s[j] *= v[i + j] * f;
+            if (a.bias) {
+                load4x(a.bias, col + i, a.dtype, *reinterpret_cast<float(*)[4]>(t));
+                load4x(a.bias, col + i + 4, a.dtype, *reinterpret_cast<float(*)[4]>(t + 4));
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s[j] += t[j];
+            }
+            if (a.act != ACT_NONE) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s[j] = activate(s[j], a.act);
+            }
+            if (mul) {
+                const uint4 u = load8_raw(mul + i, wide);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float x, y;
+                    unpack2((&u.x)[j], a.dtype, x, y);
+                    s[2 * j] *= x;
+                    s[2 * j + 1] *= y;
+                }
+            }
+            if (res) {
+                const uint4 u = load8_raw(res + i, wide);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float x, y;
+                    unpack2((&u.x)[j], a.dtype, x, y);
+                    s[2 * j] += x;
+                    s[2 * j + 1] += y;
+                }
+            }
+            uint4 u;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) (&u.x)[j] = pack2(s[2 * j], s[2 * j + 1], a.dtype);
+            if (wide) {
+                *reinterpret_cast<uint4*>(out + i) = u;
+            } else {
+                reinterpret_cast<uint2*>(out + i)[0] = make_uint2(u.x, u.y);
+                reinterpret_cast<uint2*>(out + i)[1] = make_uint2(u.z, u.w);
+            }
+        }
+    }
+};
+
+struct GemmScratch {
+    __half* xh;                // [M][k]
+    float* inv;                // [M]
+    __half* w;                 // [n][k]
+};
+
+static size_t gemm_layout(GemmScratch* w, int M, int k, int n, uint8_t* ws) {
+    size_t off = 0;
+    auto take = [&](size_t bytes) { const size_t o = off; off += up256(bytes); return ws + o; };
+    w->xh = reinterpret_cast<__half*>(take((size_t)M * k * 2));
+    w->inv = reinterpret_cast<float*>(take((size_t)M * 4));
+    w->w = reinterpret_cast<__half*>(take((size_t)n * k * 2));
+    return off;
+}
+
+template <int CODE>
+static int gemm_launch(const LinearArgs& a, DeviceState* st, uint8_t* ws, cudaStream_t stream) {
+    GemmScratch w;
+    gemm_layout(&w, a.M, a.k, a.n, ws);
+    CUtensorMap rows, cols;
+    int rc = encode_rows(&rows, w.xh, a.k, a.M, 128);
+    if (!rc) rc = encode_rows(&cols, w.w, a.k, a.n, 128);
+    if (rc) return rc;
+    rc = launch_kernel(linear_rotate_rows_kernel<true>, "linear_rotate_rows launch", dim3(a.M), 256, 0, false,
+                       stream, a, w.xh, w.inv);
+    if (rc) return rc;
+    rc = launch_kernel(linear_expand_kernel<CODE>, "linear_expand launch", dim3(a.n >> 7, a.k >> 7), 256, 0,
+                       false, stream, a.trellis, a.K, a.k, a.n, w.w);
+    if (rc) return rc;
+    LinearRows e;
+    e.a = a;
+    auto wide = [](const void* p, int64_t ld) { return !p || (((uintptr_t)p & 15) == 0 && ld % 8 == 0); };
+    e.wide = wide(a.mul, a.ldmul) && wide(a.residual, a.ldres) && wide(a.out, a.ldo);
+    const GemmArgs g = {a.M, a.k, a.n, w.inv, st->fwd_err};
+    const int tiles = ((a.M + kGemmTile - 1) / kGemmTile) * ((a.n + kGemmTile - 1) / kGemmTile);
+    const int pairs = tiles < st->sms / 2 ? tiles : st->sms / 2;
+    return launch_kernel(linear_gemm_kernel<LinearRows>, "linear_gemm launch", dim3(2 * pairs),
+                         kGemmThreadsAll, kGemmBytes, true, stream, rows, cols, g, e);
+}
+
 // ------------------------------------------------------------------ which path
-constexpr int kFewMost = 16;
+constexpr int kFewMost = 16, kMidMost = 767;
 
 static size_t linear_bytes(int M, int k, int n, int sms) {
     if (M <= kFewMost) {
         FewScratch w;
         return few_layout(&w, M, k, n, few_groups(M), sms, nullptr);
     }
-    MidScratch w;
-    return mid_layout(&w, M, k, n, sms, nullptr);
+    if (M <= kMidMost) {
+        MidScratch w;
+        return mid_layout(&w, M, k, n, sms, nullptr);
+    }
+    GemmScratch w;
+    return gemm_layout(&w, M, k, n, nullptr);
 }
 
 static int linear_run_all(const LinearArgs& a, DeviceState* st, uint8_t* ws, cudaStream_t stream) {
     if (a.M <= kFewMost) return few_dispatch(a, st->sms, ws, stream);
+    const bool mid = a.M <= kMidMost;
+#define EXL3B_ROWS(C) (mid ? mid_launch<C>(a, st, ws, stream) : gemm_launch<C>(a, st, ws, stream))
     switch (a.code) {
-        case CODE_MUL1: return mid_launch<CODE_MUL1>(a, st, ws, stream);
-        case CODE_3INST: return mid_launch<CODE_3INST>(a, st, ws, stream);
-        default: return mid_launch<CODE_MCG>(a, st, ws, stream);
+        case CODE_MUL1: return EXL3B_ROWS(CODE_MUL1);
+        case CODE_3INST: return EXL3B_ROWS(CODE_3INST);
+        default: return EXL3B_ROWS(CODE_MCG);
     }
+#undef EXL3B_ROWS
 }
 
 // A forward kernel's bounded wait ran out in an earlier call.

@@ -1,0 +1,277 @@
+// forward_gemm.cuh -- the product for long prompts: the weight is decoded once into
+// fp16 (its code values are fp16 numbers, so nothing is lost) and multiplied by a
+// tcgen05 GEMM whose epilogue rotates the sums back in registers.
+//
+// A pair of CTAs (cta_group::2) owns 256 rows x 256 columns of the output: each loads
+// its 128 rows and 128 of the columns, and holds its rows' 256 sums in tensor memory,
+// twice, so that the epilogue of a tile overlaps the next one's MMAs.  In tensor memory
+// a lane is a row, so a thread has all 128 columns of a Hadamard block in registers
+// and no lane needs another's.  Decoding in the product instead (forward_mid.cuh) reads the
+// rows' operand once per 128 columns rather than per 256 and is bound by that: 700 us
+// against 480 at 4096 rows of 5120 x 17408, before the parked sums' way to memory and back.
+#pragma once
+#include "forward_mid.cuh"
+
+namespace exl3b {
+
+constexpr int kGemmTile = 256;                      // rows and columns of a pair's tile
+constexpr int kGemmBox = 128 * 128;                 // 128 rows of 64 k: 16 KB
+constexpr int kGemmStages = 6;
+constexpr int kGemmStage = 2 * kGemmBox;            // rows | columns
+constexpr int kGemmBytes = kGemmStages * kGemmStage + 256 + 1024;
+constexpr int kGemmThreadsAll = 192;                // loader, MMA, four epilogue warps
+
+// W_inner^T as fp16 [n][k]; the k of a pair of tiles in few_put_block's order, in which
+// a lane's values of two tiles are 16 bytes of a row.  A warp per tile column and 128 k.
+template <int K, int CODE>
+__device__ __forceinline__ void expand_block(const uint8_t* src, size_t kt_bytes, __half* out, int k,
+                                             int lane) {
+    const LaneWindow<K> lw(lane);
+    uint8_t* to = reinterpret_cast<uint8_t*>(out + (size_t)(lane >> 2) * k) + (lane & 3) * 16;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        uint32_t a[4], b[4];
+        decode_tile<K, CODE>(reinterpret_cast<const uint32_t*>(src + (2 * p) * kt_bytes), lw, a);
+        decode_tile<K, CODE>(reinterpret_cast<const uint32_t*>(src + (2 * p + 1) * kt_bytes), lw, b);
+        *reinterpret_cast<uint4*>(to + 64 * p) = make_uint4(a[0], a[2], b[0], b[2]);
+        *reinterpret_cast<uint4*>(to + 64 * p + (size_t)16 * k) = make_uint4(a[1], a[3], b[1], b[3]);
+    }
+}
+
+template <int CODE>
+__global__ void __launch_bounds__(256)
+linear_expand_kernel(const uint8_t* trellis, int K, int k, int n, __half* w) {
+    const int lane = threadIdx.x & 31, col = blockIdx.x * 8 + (threadIdx.x >> 5), b = blockIdx.y;
+    pdl_launch();
+    const size_t kt_bytes = (size_t)(n >> 4) * 32 * K;
+    const uint8_t* src = trellis + (size_t)b * 8 * kt_bytes + (size_t)col * 32 * K;
+    __half* out = w + (size_t)col * 16 * k + b * 128;
+    with_bits(K, [&](auto bits) {
+        expand_block<decltype(bits)::value, CODE>(src, kt_bytes, out, k, lane);
+    });
+}
+
+struct GemmArgs {
+    int M, k, n;
+    const float* inv;          // [M] reciprocal row scales
+    int* err;
+};
+
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y,
+                                              uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3}], [%4];"
+        :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+
+// Arrive at `bar` of both CTAs of the pair when every MMA issued so far is done.
+__device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+        :: "r"(bar), "h"((uint16_t)3) : "memory");
+}
+
+// 128-point Hadamard transform of a thread's values, not normalised.
+__device__ __forceinline__ void had128_thread(float (&v)[128]) {
+#pragma unroll
+    for (int h = 1; h < 128; h <<= 1)
+#pragma unroll
+        for (int i = 0; i < 128; ++i)
+            if (!(i & h)) {
+                const float a = v[i], b = v[i + h];
+                v[i] = a + b;
+                v[i + h] = a - b;
+            }
+}
+
+// Eight elements of a row (8-byte aligned, 16 if `wide`).
+__device__ __forceinline__ uint4 load8_raw(const void* p, bool wide) {
+    if (wide) return *reinterpret_cast<const uint4*>(p);
+    const uint2 a = reinterpret_cast<const uint2*>(p)[0], b = reinterpret_cast<const uint2*>(p)[1];
+    return make_uint4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ void unpack2(uint32_t u, int dtype, float& a, float& b) {
+    if (dtype == X_BF16) {
+        a = __uint_as_float(u << 16);
+        b = __uint_as_float(u & 0xFFFF0000u);
+    } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
+        a = f.x;
+        b = f.y;
+    }
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, int dtype) {
+    if (dtype == X_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Tile t: groups of up to 16 row tiles, columns slowest inside a group, so that the
+// tiles in flight share their operands in L2.
+__device__ __forceinline__ void gemm_place(int t, int mt, int nt, int& m, int& n) {
+    const int per = 16 * nt, g = t / per, first = g * 16, rows = min(16, mt - first), in = t - g * per;
+    n = in / rows;
+    m = first + in - n * rows;
+}
+
+template <typename Linear>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreadsAll, 1)
+linear_gemm_kernel(const __grid_constant__ CUtensorMap rows, const __grid_constant__ CUtensorMap cols,
+                   const GemmArgs g, const Linear a) {
+    extern __shared__ __align__(1024) uint8_t sm_raw[];
+    __shared__ int fail;
+    __shared__ uint32_t tmem_slot;
+    uint8_t* sm = (uint8_t*)(((uintptr_t)sm_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + kGemmStages * kGemmStage);
+    const uint32_t full = shared_addr(bars), empty = full + 8 * kGemmStages,
+                   afull = empty + 8 * kGemmStages, aempty = afull + 16, done = aempty + 16;
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+    const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int mt = (g.M + kGemmTile - 1) / kGemmTile, nt = (g.n + kGemmTile - 1) / kGemmTile;
+    const int tiles = mt * nt, chunks = g.k >> 6;
+    if (t == 0) {
+        for (int i = 0; i < kGemmStages; ++i) {
+            bar_init(full + 8 * i, 1);
+            bar_init(empty + 8 * i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            bar_init(afull + 8 * i, 1);
+            bar_init(aempty + 8 * i, 8);       // the epilogue warps of both CTAs
+        }
+        bar_init(done, 1);
+        fail = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;"
+                     :: "r"(shared_addr(&tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    pdl_wait();
+
+    if (t == 0) {
+        // loader: this CTA's rows and columns of every chunk, counted at the leader
+        asm volatile("fence.proxy.async.global;" ::: "memory");
+        int s = 0, r = 0, issued = 0;
+        bool ok = true;
+        for (int tile = pair; tile < tiles && ok; tile += pairs) {
+            int m, n;
+            gemm_place(tile, mt, nt, m, n);
+            for (int c = 0; c < chunks; ++c) {
+                if (r > 0) ok = bar_wait(empty + 8 * s, (r - 1) & 1, &fail);
+                if (!ok) break;
+                const uint32_t dst = shared_addr(sm) + s * kGemmStage, bar = cluster_addr(full + 8 * s, 0);
+                if (rank == 0) bar_expect(full + 8 * s, 2 * kGemmStage);
+                tma_load_pair(dst, &rows, c * 64, m * kGemmTile + rank * 128, bar);
+                tma_load_pair(dst + kGemmBox, &cols, c * 64, n * kGemmTile + rank * 128, bar);
+                ++issued;
+                if (++s == kGemmStages) { s = 0; ++r; }
+            }
+        }
+        if (!ok) atomicExch(&fail, 1);
+        // both CTAs' loads land before either's shared memory is released (the pair
+        // meets at the end)
+        if (rank == 0) {
+            const int never = 0;
+            for (int i = max(0, issued - kGemmStages); i < issued; ++i)
+                bar_wait(full + 8 * (i % kGemmStages), (i / kGemmStages) & 1, &never);
+        }
+    } else if (t == 32) {
+        if (rank == 0) {
+            const uint32_t idesc = mma_desc_f16(256, 256);
+            int s = 0, r = 0, lt = 0;
+            bool ok = true;
+            for (int tile = pair; tile < tiles && ok; tile += pairs, ++lt) {
+                const int acc = lt & 1, use = lt >> 1;
+                if (use > 0) ok = bar_wait(aempty + 8 * acc, (use - 1) & 1, &fail);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t d = tmem + acc * 256;
+                for (int c = 0; c < chunks; ++c) {
+                    ok = bar_wait(full + 8 * s, r & 1, &fail);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t base = shared_addr(sm) + s * kGemmStage;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        asm volatile(
+                            "{\n\t.reg .pred p;\n\t"
+                            "setp.ne.b32 p, %4, 0;\n\t"
+                            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                            :: "r"(d), "l"(operand_desc(base + 32 * q)),
+                               "l"(operand_desc(base + kGemmBox + 32 * q)), "r"(idesc),
+                               "r"((uint32_t)(c > 0 || q > 0)) : "memory");
+                    tc_commit_pair(empty + 8 * s);
+                    if (++s == kGemmStages) { s = 0; ++r; }
+                }
+                if (ok) tc_commit_pair(afull + 8 * acc);
+            }
+            if (!ok) atomicExch(&fail, 1);
+            tc_commit_pair(done);
+        }
+    } else if (warp >= 2) {
+        // epilogue: lane = row
+        const int quad = warp & 3;
+        int lt = 0;
+        for (int tile = pair; tile < tiles; tile += pairs, ++lt) {
+            const int acc = lt & 1, use = lt >> 1;
+            const bool ok = __all_sync(0xffffffffu, bar_wait(afull + 8 * acc, use & 1, &fail));
+            if (!ok) {
+                if (lane == 0) atomicExch(&fail, 1);
+                break;
+            }
+            tc_fence_after();
+            int m, n;
+            gemm_place(tile, mt, nt, m, n);
+            const int row = m * kGemmTile + rank * 128 + 32 * quad + lane;
+            const float f = row < g.M ? g.inv[row] * kInvSqrt128 : 0.0f;
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+                const int col = n * kGemmTile + h * 128;
+                float v[128];
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    tc_load32(tmem + ((uint32_t)(32 * quad) << 16) + acc * 256 + h * 128 + c * 32,
+                              *reinterpret_cast<uint32_t(*)[32]>(&v[c * 32]));
+                tc_wait_ld();
+                if (h == 1) {                  // read out: the leader may use it again
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0)
+                        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];"
+                                     :: "r"(cluster_addr(aempty + 8 * acc, 0)) : "memory");
+                }
+                if (row < g.M && col < g.n) {
+                    had128_thread(v);
+                    a.finish128(row, col, f, v);
+                }
+            }
+        }
+    }
+    const int never = 0;
+    const bool ok = bar_wait(done, 0, &never);
+    if (__syncthreads_or(!ok || fail)) {
+        if (t == 0) *(volatile int*)g.err = 1;
+    }
+    tc_fence_before();
+    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" :: "r"(tmem) : "memory");
+}
+
+}  // namespace exl3b

@@ -261,6 +261,53 @@ def test_linear_refuses_gradients_and_devices(fw, oracle):
         fw.linear(x.detach().cpu(), w)
 
 
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("M,k,n,K", [(768, 128, 128, 2), (769, 256, 384, 3), (1100, 640, 256, 4),
+                                     (2050, 128, 640, 5), (1280, 1152, 128, 6), (900, 384, 256, 7)])
+def test_linear_long(fw, oracle, M, k, n, K, code):
+    prob = Problem(oracle, k, n, K, code, seed=M)
+    w = prob.weight(fw)
+    dt = torch.float16 if K % 2 else torch.bfloat16
+    x, bias = rnd((M, k), dt, 1), rnd((n,), dt, 2)
+    x[5] = 0
+    x[7] *= 1e-4
+    mul, res = rnd((M, n), dt, 3), rnd((M, n), dt, 4)
+    check(fw.linear(x, w), *expect(prob, x))
+    kw = {"bias": bias, "mul": mul, "residual": res}
+    ref = fw.linear(x, w, activation="silu", **kw)
+    check(ref, *expect(prob, x, act="silu", **kw))
+    # rows on 8-byte boundaries only, and in place on the residual
+    buf = torch.zeros(M, n + 4, dtype=dt, device="cuda")
+    o = buf[:, 4:]
+    o.copy_(res)
+    fw.linear(x, w, bias=bias, activation="silu", mul=mul, residual=o, out=o)
+    assert torch.equal(o, ref)
+    assert not buf[:, :4].any()
+    x[9, 3] = float("nan")
+    got = fw.linear(x, w, activation="silu", **kw)
+    assert torch.isnan(got[9]).all()
+    keep = [i for i in range(M) if i != 9]
+    assert torch.equal(got[keep], ref[keep])
+
+
+def test_linear_long_graphs(fw, oracle):
+    prob = Problem(oracle, 256, 384, 4, seed=21)
+    w = prob.weight(fw)
+    x = rnd((1000, 256), torch.bfloat16, 1)
+    ref = fw.linear(x, w)
+    outs, graphs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(fw.linear(x, w))
+        graphs.append(g)
+    for _ in range(2):
+        for g, o in zip(graphs, outs):
+            o.zero_()
+            g.replay()
+            assert torch.equal(o, ref)
+
+
 @pytest.mark.parametrize("channel_scales", [False, True])
 def test_linear_of_a_quantized_layer(fw, tmp_path, channel_scales):
     """quantize_linear_fused -> stored fields -> linear: the forward product equals

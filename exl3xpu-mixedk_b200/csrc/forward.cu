@@ -362,61 +362,80 @@ static int mid_launch(const LinearArgs& a, DeviceState* st, uint8_t* ws, cudaStr
 }
 
 // ------------------------------------------------------------------ long prompts
+__device__ __forceinline__ void widen4(uint2 u, int dtype, float (&v)[4]) {
+    if (dtype == X_BF16) {
+        v[0] = __uint_as_float(u.x << 16); v[1] = __uint_as_float(u.x & 0xFFFF0000u);
+        v[2] = __uint_as_float(u.y << 16); v[3] = __uint_as_float(u.y & 0xFFFF0000u);
+    } else {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+        v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+    }
+}
+
+// The GEMM's epilogue on 32 columns from `col` of `rows` rows from row0, whose scaled
+// and rotated sums are in `patch` (kGemmPitch floats a row).  A warp, eight lanes a row.
 struct LinearRows {
     LinearArgs a;
-    bool wide;                 // rows of mul, residual and out on 16-byte boundaries
-    // 128 columns of a row held by a thread: scale, svh, epilogue.
-    __device__ __forceinline__ void finish128(int row, int col, float f, float (&v)[128]) const {
-        const uint16_t* mul = a.mul ? static_cast<const uint16_t*>(a.mul) + (size_t)row * a.ldmul + col : nullptr;
-        const uint16_t* res =
-            a.residual ? static_cast<const uint16_t*>(a.residual) + (size_t)row * a.ldres + col : nullptr;
-        uint16_t* out = static_cast<uint16_t*>(a.out) + (size_t)row * a.ldo + col;
+    struct Operands { uint2 mul[8], res[8], svh, bias; };
+    __device__ __forceinline__ static uint2 piece(const void* p, size_t i) {
+        return *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+    }
+    __device__ __forceinline__ void fetch(Operands& o, int row0, int rows, int col, int lane) const {
+        const int c = col + (lane & 7) * 4;
+        o.svh = piece(a.svh, c);
+        if (a.bias) o.bias = piece(a.bias, c);
+        if (a.mul) {
 #pragma unroll
-        for (int i = 0; i < 128; i += 8) {
-            float s[8], t[8];
-            load4(a.svh + col + i, *reinterpret_cast<float(*)[4]>(s));
-            load4(a.svh + col + i + 4, *reinterpret_cast<float(*)[4]>(s + 4));
+            for (int i = 0; i < 8; ++i)
+                if (4 * i + (lane >> 3) < rows)
+                    o.mul[i] = piece(a.mul, (size_t)(row0 + 4 * i + (lane >> 3)) * a.ldmul + c);
+        }
+        if (a.residual) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s[j] *= v[i + j] * f;
-            if (a.bias) {
-                load4x(a.bias, col + i, a.dtype, *reinterpret_cast<float(*)[4]>(t));
-                load4x(a.bias, col + i + 4, a.dtype, *reinterpret_cast<float(*)[4]>(t + 4));
-#pragma unroll
-                for (int j = 0; j < 8; ++j) s[j] += t[j];
+            for (int i = 0; i < 8; ++i)
+                if (4 * i + (lane >> 3) < rows)
+                    o.res[i] = piece(a.residual, (size_t)(row0 + 4 * i + (lane >> 3)) * a.ldres + c);
+        }
+    }
+    __device__ __forceinline__ void finish(const Operands& o, int row0, int rows, int col, float* patch,
+                                           int lane) const {
+        const int c = col + (lane & 7) * 4;
+        float4* at = reinterpret_cast<float4*>(patch + (lane >> 3) * kGemmPitch + (lane & 7) * 4);
+        constexpr int kStep = kGemmPitch;          // float4 between a lane's rows
+        float svh[4], bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        widen4(o.svh, X_FP16, svh);
+        if (a.bias) widen4(o.bias, a.dtype, bias);
+        if (a.act != ACT_NONE) {                   // a loop of its own: its code is long
+#pragma unroll 1
+            for (int i = 0; i < 8; ++i) {
+                const float4 q = at[i * kStep];
+                at[i * kStep] = make_float4(activate(fmaf(q.x, svh[0], bias[0]), a.act),
+                                            activate(fmaf(q.y, svh[1], bias[1]), a.act),
+                                            activate(fmaf(q.z, svh[2], bias[2]), a.act),
+                                            activate(fmaf(q.w, svh[3], bias[3]), a.act));
             }
-            if (a.act != ACT_NONE) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) s[j] = activate(s[j], a.act);
-            }
-            if (mul) {
-                const uint4 u = load8_raw(mul + i, wide);
+            for (int j = 0; j < 4; ++j) { svh[j] = 1.0f; bias[j] = 0.0f; }
+        }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float x, y;
-                    unpack2((&u.x)[j], a.dtype, x, y);
-                    s[2 * j] *= x;
-                    s[2 * j + 1] *= y;
-                }
-            }
-            if (res) {
-                const uint4 u = load8_raw(res + i, wide);
+        for (int i = 0; i < 8; ++i) {
+            const int r = 4 * i + (lane >> 3);
+            if (r >= rows) break;
+            const float4 q = at[i * kStep];
+            float v[4] = {fmaf(q.x, svh[0], bias[0]), fmaf(q.y, svh[1], bias[1]),
+                          fmaf(q.z, svh[2], bias[2]), fmaf(q.w, svh[3], bias[3])}, t[4];
+            if (a.mul) {
+                widen4(o.mul[i], a.dtype, t);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float x, y;
-                    unpack2((&u.x)[j], a.dtype, x, y);
-                    s[2 * j] += x;
-                    s[2 * j + 1] += y;
-                }
+                for (int j = 0; j < 4; ++j) v[j] *= t[j];
             }
-            uint4 u;
+            if (a.residual) {
+                widen4(o.res[i], a.dtype, t);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) (&u.x)[j] = pack2(s[2 * j], s[2 * j + 1], a.dtype);
-            if (wide) {
-                *reinterpret_cast<uint4*>(out + i) = u;
-            } else {
-                reinterpret_cast<uint2*>(out + i)[0] = make_uint2(u.x, u.y);
-                reinterpret_cast<uint2*>(out + i)[1] = make_uint2(u.z, u.w);
+                for (int j = 0; j < 4; ++j) v[j] += t[j];
             }
+            store4x(a.out, (size_t)(row0 + r) * a.ldo + c, a.dtype, v);
         }
     }
 };
@@ -448,12 +467,9 @@ static int gemm_launch(const LinearArgs& a, DeviceState* st, uint8_t* ws, cudaSt
                        stream, a, w.xh, w.inv);
     if (rc) return rc;
     rc = launch_kernel(linear_expand_kernel<CODE>, "linear_expand launch", dim3(a.n >> 7, a.k >> 7), 256, 0,
-                       false, stream, a.trellis, a.K, a.k, a.n, w.w);
+                       true, stream, a.trellis, a.K, a.k, a.n, w.w);
     if (rc) return rc;
-    LinearRows e;
-    e.a = a;
-    auto wide = [](const void* p, int64_t ld) { return !p || (((uintptr_t)p & 15) == 0 && ld % 8 == 0); };
-    e.wide = wide(a.mul, a.ldmul) && wide(a.residual, a.ldres) && wide(a.out, a.ldo);
+    const LinearRows e = {a};
     const GemmArgs g = {a.M, a.k, a.n, w.inv, st->fwd_err};
     const int tiles = ((a.M + kGemmTile - 1) / kGemmTile) * ((a.n + kGemmTile - 1) / kGemmTile);
     const int pairs = tiles < st->sms / 2 ? tiles : st->sms / 2;

@@ -16,10 +16,13 @@ namespace exl3b {
 
 constexpr int kGemmTile = 256;                      // rows and columns of a pair's tile
 constexpr int kGemmBox = 128 * 128;                 // 128 rows of 64 k: 16 KB
-constexpr int kGemmStages = 6;
 constexpr int kGemmStage = 2 * kGemmBox;            // rows | columns
-constexpr int kGemmBytes = kGemmStages * kGemmStage + 256 + 1024;
-constexpr int kGemmThreadsAll = 192;                // loader, MMA, four epilogue warps
+constexpr int kGemmPitch = 36;                      // floats: 32 columns of a row in the epilogue
+constexpr int kGemmPatch = 32 * kGemmPitch * 4;     // a warp's 32 rows of them
+constexpr int kGemmEpilogue = 8;                    // warps: a quarter of the rows, a half of the columns
+constexpr int kGemmStages = 5;
+constexpr int kGemmBytes = kGemmStages * kGemmStage + kGemmEpilogue * kGemmPatch + 256 + 1024;
+constexpr int kGemmThreadsAll = 64 + 32 * kGemmEpilogue;      // loader, MMA, epilogue
 
 // W_inner^T as fp16 [n][k]; the k of a pair of tiles in few_put_block's order, in which
 // a lane's values of two tiles are 16 bytes of a row.  A warp per tile column and 128 k.
@@ -49,6 +52,7 @@ linear_expand_kernel(const uint8_t* trellis, int K, int k, int n, __half* w) {
     with_bits(K, [&](auto bits) {
         expand_block<decltype(bits)::value, CODE>(src, kt_bytes, out, k, lane);
     });
+    pdl_wait();                // this kernel's end stands for the rotation's, too
 }
 
 struct GemmArgs {
@@ -91,31 +95,6 @@ __device__ __forceinline__ void had128_thread(float (&v)[128]) {
             }
 }
 
-// Eight elements of a row (8-byte aligned, 16 if `wide`).
-__device__ __forceinline__ uint4 load8_raw(const void* p, bool wide) {
-    if (wide) return *reinterpret_cast<const uint4*>(p);
-    const uint2 a = reinterpret_cast<const uint2*>(p)[0], b = reinterpret_cast<const uint2*>(p)[1];
-    return make_uint4(a.x, a.y, b.x, b.y);
-}
-__device__ __forceinline__ void unpack2(uint32_t u, int dtype, float& a, float& b) {
-    if (dtype == X_BF16) {
-        a = __uint_as_float(u << 16);
-        b = __uint_as_float(u & 0xFFFF0000u);
-    } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
-        a = f.x;
-        b = f.y;
-    }
-}
-__device__ __forceinline__ uint32_t pack2(float a, float b, int dtype) {
-    if (dtype == X_BF16) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 // Tile t: groups of up to 16 row tiles, columns slowest inside a group, so that the
 // tiles in flight share their operands in L2.
 __device__ __forceinline__ void gemm_place(int t, int mt, int nt, int& m, int& n) {
@@ -124,15 +103,15 @@ __device__ __forceinline__ void gemm_place(int t, int mt, int nt, int& m, int& n
     m = first + in - n * rows;
 }
 
-template <typename Linear>
+template <typename Epilogue>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreadsAll, 1)
 linear_gemm_kernel(const __grid_constant__ CUtensorMap rows, const __grid_constant__ CUtensorMap cols,
-                   const GemmArgs g, const Linear a) {
+                   const GemmArgs g, const Epilogue ep) {
     extern __shared__ __align__(1024) uint8_t sm_raw[];
     __shared__ int fail;
     __shared__ uint32_t tmem_slot;
     uint8_t* sm = (uint8_t*)(((uintptr_t)sm_raw + 1023) & ~(uintptr_t)1023);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + kGemmStages * kGemmStage);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + kGemmStages * kGemmStage + kGemmEpilogue * kGemmPatch);
     const uint32_t full = shared_addr(bars), empty = full + 8 * kGemmStages,
                    afull = empty + 8 * kGemmStages, aempty = afull + 16, done = aempty + 16;
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
@@ -146,7 +125,7 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap rows, const __grid_consta
         }
         for (int i = 0; i < 2; ++i) {
             bar_init(afull + 8 * i, 1);
-            bar_init(aempty + 8 * i, 8);       // the epilogue warps of both CTAs
+            bar_init(aempty + 8 * i, 2 * kGemmEpilogue);
         }
         bar_init(done, 1);
         fail = 0;
@@ -225,41 +204,56 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap rows, const __grid_consta
             tc_commit_pair(done);
         }
     } else if (warp >= 2) {
-        // epilogue: lane = row
-        const int quad = warp & 3;
+        // epilogue: lane = row up to the rotation; then, 32 columns at a time through
+        // shared memory, eight lanes a row, so that global memory sees 64-byte pieces and
+        // the code stays small (unrolled over a thread's 128 columns it missed the
+        // instruction cache: 1.74 ms with silu).  Operands are asked for before the
+        // exchange: a warp has little else to hide their latency.
+        const int quad = warp & 3, half = (warp - 2) >> 2;
+        float* patch = reinterpret_cast<float*>(sm + kGemmStages * kGemmStage + (warp - 2) * kGemmPatch);
         int lt = 0;
         for (int tile = pair; tile < tiles; tile += pairs, ++lt) {
             const int acc = lt & 1, use = lt >> 1;
+            int m, n;
+            gemm_place(tile, mt, nt, m, n);
+            const int row0 = m * kGemmTile + rank * 128 + 32 * quad, row = row0 + lane;
+            const int col = n * kGemmTile + half * 128, have = col < g.n ? min(32, g.M - row0) : 0;
+            const float f = row < g.M ? g.inv[row] * kInvSqrt128 : 0.0f;
             const bool ok = __all_sync(0xffffffffu, bar_wait(afull + 8 * acc, use & 1, &fail));
             if (!ok) {
                 if (lane == 0) atomicExch(&fail, 1);
                 break;
             }
             tc_fence_after();
-            int m, n;
-            gemm_place(tile, mt, nt, m, n);
-            const int row = m * kGemmTile + rank * 128 + 32 * quad + lane;
-            const float f = row < g.M ? g.inv[row] * kInvSqrt128 : 0.0f;
-#pragma unroll 1
-            for (int h = 0; h < 2; ++h) {
-                const int col = n * kGemmTile + h * 128;
-                float v[128];
+            float v[128];
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    tc_load32(tmem + ((uint32_t)(32 * quad) << 16) + acc * 256 + h * 128 + c * 32,
-                              *reinterpret_cast<uint32_t(*)[32]>(&v[c * 32]));
-                tc_wait_ld();
-                if (h == 1) {                  // read out: the leader may use it again
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0)
-                        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];"
-                                     :: "r"(cluster_addr(aempty + 8 * acc, 0)) : "memory");
-                }
-                if (row < g.M && col < g.n) {
-                    had128_thread(v);
-                    a.finish128(row, col, f, v);
-                }
+            for (int c = 0; c < 4; ++c)
+                tc_load32(tmem + ((uint32_t)(32 * quad) << 16) + acc * 256 + half * 128 + c * 32,
+                          *reinterpret_cast<uint32_t(*)[32]>(&v[c * 32]));
+            tc_wait_ld();
+            tc_fence_before();                 // read out: the leader may use it again
+            __syncwarp();
+            if (lane == 0)
+                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];"
+                             :: "r"(cluster_addr(aempty + 8 * acc, 0)) : "memory");
+            if (have <= 0) continue;
+            had128_thread(v);
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+                typename Epilogue::Operands op;
+                ep.fetch(op, row0, have, col + c * 32, lane);
+                float4* to = reinterpret_cast<float4*>(patch + lane * kGemmPitch);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (e == c) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            to[j] = make_float4(v[e * 32 + 4 * j] * f, v[e * 32 + 4 * j + 1] * f,
+                                                v[e * 32 + 4 * j + 2] * f, v[e * 32 + 4 * j + 3] * f);
+                    }
+                __syncwarp();
+                ep.finish(op, row0, have, col + c * 32, patch, lane);
+                __syncwarp();
             }
         }
     }

@@ -215,16 +215,34 @@ static int few_dispatch(const LinearArgs& a, int sms, uint8_t* ws, cudaStream_t 
 template <bool PAIRED>
 __global__ void __launch_bounds__(256) linear_rotate_rows_kernel(const LinearArgs a, __half* xh, float* inv) {
     __shared__ float part[8];
+    constexpr int kHold = 6;                  // blocks a warp keeps in registers; others are read twice
     pdl_launch();
     const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kb = a.k >> 7;
     const size_t at = (size_t)row * a.ldx + 4 * lane;
-    float m = 0.0f;
-    for (int b = warp; b < kb; b += 8) {
-        float v[4], s[4];
+    auto load = [&](int b, float (&v)[4]) {
+        float s[4];
         load4x(a.x, at + b * 128, a.dtype, v);
         load4(a.suh + b * 128 + 4 * lane, s);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) m = fmaxf(m, fabsf(v[j] * s[j]));
+        for (int j = 0; j < 4; ++j) v[j] *= s[j];
+    };
+    float held[kHold][4], m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kHold; ++i) {
+        const int b = warp + 8 * i;
+        if (b < kb) load(b, held[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kHold; ++i)
+        if (warp + 8 * i < kb)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) m = fmaxf(m, fabsf(held[i][j]));
+#pragma unroll 4
+    for (int b = warp + 8 * kHold; b < kb; b += 8) {
+        float v[4];
+        load(b, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m = fmaxf(m, fabsf(v[j]));
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -235,12 +253,9 @@ __global__ void __launch_bounds__(256) linear_rotate_rows_kernel(const LinearArg
     float back;
     const float scale = block_scale(m, back) * kInvSqrt128;
     if (threadIdx.x == 0) inv[row] = back;
-    for (int b = warp; b < kb; b += 8) {
-        float v[4], s[4];
-        load4x(a.x, at + b * 128, a.dtype, v);
-        load4(a.suh + b * 128 + 4 * lane, s);
+    auto store = [&](int b, float (&v)[4]) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = v[j] * s[j] * scale;
+        for (int j = 0; j < 4; ++j) v[j] *= scale;
         had128_warp(v, lane);
         __half* to = xh + (size_t)row * a.k + b * 128;
         if (PAIRED) {
@@ -251,6 +266,17 @@ __global__ void __launch_bounds__(256) linear_rotate_rows_kernel(const LinearArg
         } else {
             store4(to + 4 * lane, v);
         }
+    };
+#pragma unroll
+    for (int i = 0; i < kHold; ++i) {
+        const int b = warp + 8 * i;
+        if (b < kb) store(b, held[i]);
+    }
+#pragma unroll 4
+    for (int b = warp + 8 * kHold; b < kb; b += 8) {
+        float v[4];
+        load(b, v);
+        store(b, v);
     }
 }
 
@@ -478,14 +504,32 @@ static int gemm_launch(const LinearArgs& a, DeviceState* st, uint8_t* ws, cudaSt
 }
 
 // ------------------------------------------------------------------ which path
-constexpr int kFewMost = 16, kMidMost = 767;
+constexpr int kFewMost = 16;
+
+// Up to 16 rows mma.sync (one decode serves them); beyond, tensor memory.  There the
+// product that decodes as it goes repeats the decode per 256 rows and parks its sums,
+// and the decoded copy costs its way to memory and back but leaves a plain GEMM of whole
+// 256 x 256 tiles.  The estimates are fits in microseconds, without the rotation that
+// both need.  Measured, decoding against copying (in x out, rows): 5120 x 5120, 512 45 /
+// 52, 1024 79 / 84, 1536 110 / 90; 5120 x 17408, 512 115 / 122, 768 167 / 155, 4096 913 /
+// 605; 17408 x 5120, 1024 203 / 261, 2048 436 / 388; 5120 x 1024, 2048 49 / 55.
+static bool copy_pays(int M, int k, int n, int sms) {
+    const double kb = k >> 7, nb = n >> 7;
+    const int N = mid_rows(M), passes = (M + N - 1) / N;
+    const double mid = 13.0 + 1.15 * passes * nb * kb / sms * (N > 160 ? N : 160) / 256.0 +
+                       3.3e-6 * M * (double)n;
+    const int tiles = ((M + kGemmTile - 1) / kGemmTile) * ((n + kGemmTile - 1) / kGemmTile);
+    const int waves = (tiles + sms / 2 - 1) / (sms / 2);
+    const double wave = 0.62 * kb + 2.0;               // at least its epilogue, 11 us
+    return 10.0 + 5.2e-7 * k * (double)n + waves * (wave > 11.0 ? wave : 11.0) < mid;
+}
 
 static size_t linear_bytes(int M, int k, int n, int sms) {
     if (M <= kFewMost) {
         FewScratch w;
         return few_layout(&w, M, k, n, few_groups(M), sms, nullptr);
     }
-    if (M <= kMidMost) {
+    if (!copy_pays(M, k, n, sms)) {
         MidScratch w;
         return mid_layout(&w, M, k, n, sms, nullptr);
     }
@@ -495,7 +539,7 @@ static size_t linear_bytes(int M, int k, int n, int sms) {
 
 static int linear_run_all(const LinearArgs& a, DeviceState* st, uint8_t* ws, cudaStream_t stream) {
     if (a.M <= kFewMost) return few_dispatch(a, st->sms, ws, stream);
-    const bool mid = a.M <= kMidMost;
+    const bool mid = !copy_pays(a.M, a.k, a.n, st->sms);
 #define EXL3B_ROWS(C) (mid ? mid_launch<C>(a, st, ws, stream) : gemm_launch<C>(a, st, ws, stream))
     switch (a.code) {
         case CODE_MUL1: return EXL3B_ROWS(CODE_MUL1);

@@ -61,27 +61,6 @@ struct GemmArgs {
     int* err;
 };
 
-__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, int rank) {
-    uint32_t r;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
-
-__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y,
-                                              uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3}], [%4];"
-        :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
-}
-
-// Arrive at `bar` of both CTAs of the pair when every MMA issued so far is done.
-__device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
-    asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-        :: "r"(bar), "h"((uint16_t)3) : "memory");
-}
-
 // 128-point Hadamard transform of a thread's values, not normalised.
 __device__ __forceinline__ void had128_thread(float (&v)[128]) {
 #pragma unroll
@@ -131,14 +110,10 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap rows, const __grid_consta
         fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;"
-                     :: "r"(shared_addr(&tmem_slot)) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    }
+    if (warp == 1) tc_alloc_pair(shared_addr(&tmem_slot));
     tc_fence_before();
     __syncthreads();
-    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+    cluster_meet();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     pdl_wait();
@@ -233,9 +208,7 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap rows, const __grid_consta
             tc_wait_ld();
             tc_fence_before();                 // read out: the leader may use it again
             __syncwarp();
-            if (lane == 0)
-                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];"
-                             :: "r"(cluster_addr(aempty + 8 * acc, 0)) : "memory");
+            if (lane == 0) bar_arrive_cluster(cluster_addr(aempty + 8 * acc, 0));
             if (have <= 0) continue;
             had128_thread(v);
 #pragma unroll 1
@@ -263,9 +236,8 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap rows, const __grid_consta
         if (t == 0) *(volatile int*)g.err = 1;
     }
     tc_fence_before();
-    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-    if (warp == 1)
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" :: "r"(tmem) : "memory");
+    cluster_meet();
+    if (warp == 1) tc_free_pair(tmem);
 }
 
 }  // namespace exl3b

@@ -177,20 +177,20 @@ static int few_launch(const LinearArgs& a, int sms, uint8_t* ws, cudaStream_t st
         // one or two rows are rotated where they are used, cheaper than a launch (5120 x
         // 5120, K = 4: 12.2 us against 12.9), if a CTA's share of them fits
         if (a.M <= 2 && few_smem(a.K, G, most) <= kFewRoom) {
-            rc = launch_kernel(linear_few_kernel<CODE, G, true>, "linear_few launch", dim3(run.ctas),
+            rc = launch_kernel<linear_few_kernel<CODE, G, true>>("linear_few launch", dim3(run.ctas),
                                32 * kFewWarps, few_smem(a.K, G, most), false, stream, a, w, run, nbn);
             done = true;
         }
     }
     if (!done) {
-        rc = launch_kernel(linear_rotate_kernel, "linear_rotate launch",
+        rc = launch_kernel<linear_rotate_kernel>("linear_rotate launch",
                            dim3(((a.k >> 7) * a.M + 3) / 4), 128, 0, false, stream, a, w);
         if (rc) return rc;
-        rc = launch_kernel(linear_few_kernel<CODE, G, false>, "linear_few launch", dim3(run.ctas),
+        rc = launch_kernel<linear_few_kernel<CODE, G, false>>("linear_few launch", dim3(run.ctas),
                            32 * kFewWarps, few_smem(a.K, G, ring), true, stream, a, w, run, nbn);
     }
     if (rc) return rc;
-    return launch_kernel(linear_finish_kernel<G>, "linear_finish launch", fin, 128, 0, true, stream, a,
+    return launch_kernel<linear_finish_kernel<G>>("linear_finish launch", fin, 128, 0, true, stream, a,
                          w, FewJoin(run));
 }
 
@@ -376,13 +376,13 @@ static int mid_launch(const LinearArgs& a, DeviceState* st, uint8_t* ws, cudaStr
     CUtensorMap rows;
     int rc = encode_rows(&rows, w.xh, a.k, a.M, m.N);
     if (rc) return rc;
-    rc = launch_kernel(linear_rotate_rows_kernel<false>, "linear_rotate_rows launch", dim3(a.M), 256, 0, false,
+    rc = launch_kernel<linear_rotate_rows_kernel<false>>("linear_rotate_rows launch", dim3(a.M), 256, 0, false,
                        stream, a, w.xh, w.inv);
     if (rc) return rc;
-    rc = launch_kernel(linear_mid_kernel<CODE>, "linear_mid launch", dim3(m.run.ctas), kMidThreads,
+    rc = launch_kernel<linear_mid_kernel<CODE>>("linear_mid launch", dim3(m.run.ctas), kMidThreads,
                        mid_smem(a.K, m.N, m.stages), true, stream, rows, m);
     if (rc) return rc;
-    return launch_kernel(linear_mid_finish_kernel, "linear_mid_finish launch",
+    return launch_kernel<linear_mid_finish_kernel>("linear_mid_finish launch",
                          dim3(m.nbn, (a.M + 3) / 4), 128, 0, true, stream, a, m, FewJoin(m.run),
                          (const float*)w.inv);
 }
@@ -489,17 +489,17 @@ static int gemm_launch(const LinearArgs& a, DeviceState* st, uint8_t* ws, cudaSt
     int rc = encode_rows(&rows, w.xh, a.k, a.M, 128);
     if (!rc) rc = encode_rows(&cols, w.w, a.k, a.n, 128);
     if (rc) return rc;
-    rc = launch_kernel(linear_rotate_rows_kernel<true>, "linear_rotate_rows launch", dim3(a.M), 256, 0, false,
+    rc = launch_kernel<linear_rotate_rows_kernel<true>>("linear_rotate_rows launch", dim3(a.M), 256, 0, false,
                        stream, a, w.xh, w.inv);
     if (rc) return rc;
-    rc = launch_kernel(linear_expand_kernel<CODE>, "linear_expand launch", dim3(a.n >> 7, a.k >> 7), 256, 0,
+    rc = launch_kernel<linear_expand_kernel<CODE>>("linear_expand launch", dim3(a.n >> 7, a.k >> 7), 256, 0,
                        true, stream, a.trellis, a.K, a.k, a.n, w.w);
     if (rc) return rc;
     const LinearRows e = {a};
     const GemmArgs g = {a.M, a.k, a.n, w.inv, st->fwd_err};
     const int tiles = ((a.M + kGemmTile - 1) / kGemmTile) * ((a.n + kGemmTile - 1) / kGemmTile);
     const int pairs = tiles < st->sms / 2 ? tiles : st->sms / 2;
-    return launch_kernel(linear_gemm_kernel<LinearRows>, "linear_gemm launch", dim3(2 * pairs),
+    return launch_kernel<linear_gemm_kernel<LinearRows>>("linear_gemm launch", dim3(2 * pairs),
                          kGemmThreadsAll, kGemmBytes, true, stream, rows, cols, g, e);
 }
 

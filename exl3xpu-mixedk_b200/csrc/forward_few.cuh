@@ -9,6 +9,8 @@
 // matrix unit, and mma.sync takes the decoded operand from the registers it was
 // decoded into, without the trip through tensor memory that tcgen05 would need.
 #pragma once
+#include <atomic>
+
 #include "exl3b_internal.h"
 #include "trellis_mma.cuh"
 
@@ -215,7 +217,7 @@ struct FewJoin {
     FewRun run;
     FastDiv least, more;       // by the blocks of the short runs and of the longer ones
     __host__ __device__ FewJoin() {}
-    __host__ __device__ explicit FewJoin(const FewRun& r)
+    __host__ explicit FewJoin(const FewRun& r)
         : run(r), least(r.least ? r.least : 1), more(r.least + 1) {}
     __device__ __forceinline__ int owner(int g) const {
         const int head = run.longer * (run.least + 1);
@@ -481,18 +483,31 @@ __device__ __forceinline__ void few_rotate_back(float (&v)[4], int lane) {
     had128_warp(v, lane);
 }
 
-template <typename... P, typename... A>
-int launch_kernel(void (*kern)(P...), const char* what, dim3 grid, int threads, size_t smem, bool pdl,
-                  cudaStream_t stream, A... args) {
-    if (smem > 48 * 1024 &&
-        check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
-                   what))
-        return RC_DEVICE_ERROR;
-    // the same split of L1 for all: a kernel that wants another waits for the SM to empty
-    if (smem <= 48 * 1024 &&
+// The kernel attributes of a launch, set once per kernel and device: shared memory up to
+// what a CTA may have, and the same split of L1 for all, since a kernel that wants
+// another waits for the SM to empty.  (Setting them again is harmless: two threads may.)
+template <typename... P>
+int prepare_kernel(void (*kern)(P...), const char* what, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    if (check_cuda(cudaGetDevice(&dev), what)) return RC_DEVICE_ERROR;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_acquire) & bit) return RC_OK;
+    cudaFuncAttributes fa;
+    if (check_cuda(cudaFuncGetAttributes(&fa, kern), what) ||
+        check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        227 * 1024 - (int)fa.sharedSizeBytes), what) ||
         check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout,
                                         cudaSharedmemCarveoutMaxShared), what))
         return RC_DEVICE_ERROR;
+    done.fetch_or(bit, std::memory_order_release);
+    return RC_OK;
+}
+
+template <auto Kern, typename... A>
+int launch_kernel(const char* what, dim3 grid, int threads, size_t smem, bool pdl, cudaStream_t stream,
+                  A... args) {
+    static std::atomic<uint64_t> done{0};
+    if (prepare_kernel(Kern, what, done)) return RC_DEVICE_ERROR;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
@@ -503,7 +518,7 @@ int launch_kernel(void (*kern)(P...), const char* what, dim3 grid, int threads, 
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = pdl ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, Kern, args...);
     note_launch();
     return check_cuda(e, what) ? RC_DEVICE_ERROR : RC_OK;
 }

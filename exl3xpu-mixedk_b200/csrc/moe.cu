@@ -336,37 +336,54 @@ __device__ __forceinline__ Plan plan_at(uint8_t* where, int P, int slots_max) {
 
 constexpr int kPlanThreads = 512;
 
-// One CTA of kPlanThreads; `tmp`: 2 (P + E) ints of shared memory.
+__host__ __device__ inline int plan_scratch(int P, int E) {
+    return up16(P * 4) + up16(E * 8) + (P + 31) / 32 * E;
+}
+
+// One CTA of kPlanThreads; `tmp`: plan_scratch bytes of shared memory.
 template <int G>
-__device__ __forceinline__ void make_plan(const MoeArgs& a, int* tmp) {
+__device__ __forceinline__ void make_plan(const MoeArgs& a, uint8_t* tmp) {
     __shared__ int totals[kPlanThreads / 32];
-    const int t = threadIdx.x, warp = t >> 5, lane = t & 31, P = a.T * a.top_k;
+    constexpr int kWarps = kPlanThreads / 32;
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31, P = a.T * a.top_k, chunks = (P + 31) / 32;
     const Plan p = plan_at(a.plan, P, a.slots_max);
-    int* rank = tmp + P;       // [P] a pair's place among its expert's
-    int* count = rank + P;     // [E] pairs of an expert
-    int* from = count + a.E;   // [E] its first pair and slot
-    for (int e = t; e < a.E; e += kPlanThreads) count[e] = 0;
-    for (int i = t; i < P; i += kPlanThreads) tmp[i] = a.chosen[i].expert;
+    int* where = reinterpret_cast<int*>(tmp);                   // [P] expert << 8 | place in its chunk
+    int* from = reinterpret_cast<int*>(tmp + up16(P * 4));      // [E] an expert's first pair and slot
+    int* count = from + a.E;                                    // [E] its pairs
+    uint8_t* before = tmp + up16(P * 4) + up16(a.E * 8);        // [chunks][E] then running
+    Chosen own;
+    if (t < P) own = a.chosen[t];
+    for (int i = t; i < (chunks * a.E + 3) / 4; i += kPlanThreads) reinterpret_cast<uint32_t*>(before)[i] = 0;
     __syncthreads();
-    // in order, 32 pairs at a time
-    if (warp == 0) {
-        for (int base = 0; base < P; base += 32) {
-            const bool in = base + lane < P;
-            const int e = in ? tmp[base + lane] : -1;
-            const uint32_t same = __match_any_sync(0xffffffffu, e);
-            const int r = in ? count[e] + __popc(same & ((1u << lane) - 1)) : 0;
-            __syncwarp();
-            if (in) {
-                rank[base + lane] = r;
-                if ((same >> lane) == 1) count[e] = r + 1;      // the last of them
-            }
-            __syncwarp();
+    // 32 pairs a warp: how many of the same expert come before a pair there
+    for (int c = warp; c < chunks; c += kWarps) {
+        const int i = c * 32 + lane;
+        const int e = i >= P ? -1 : i == t ? own.expert : a.chosen[i].expert;
+        const uint32_t same = __match_any_sync(0xffffffffu, e);
+        if (e >= 0) {
+            where[i] = e << 8 | __popc(same & ((1u << lane) - 1));
+            if ((same >> lane) == 1) before[c * a.E + e] = (uint8_t)__popc(same);
         }
     }
     __syncthreads();
+    // and how many in the chunks before; a count of more than 255 lies in the last sum
+    // only, since an expert has at most T pairs, T <= 256, and the last chunk's is not added
+    const int e0 = 2 * t;
+    int c2[2] = {0, 0};
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        if (e0 + h < a.E) {
+            int sum = 0;
+            for (int c = 0; c < chunks; ++c) {
+                const int x = before[c * a.E + e0 + h];
+                before[c * a.E + e0 + h] = (uint8_t)sum;
+                sum += x;
+            }
+            c2[h] = sum;
+            count[e0 + h] = sum;
+        }
     // running sums over two experts a thread: pairs in the low half, slots in the high
-    const int e0 = 2 * t, c0 = e0 < a.E ? count[e0] : 0, c1 = e0 + 1 < a.E ? count[e0 + 1] : 0;
-    const int m0 = c0 | (c0 + 8 * G - 1) / (8 * G) << 16, m1 = c1 | (c1 + 8 * G - 1) / (8 * G) << 16;
+    const int m0 = c2[0] | (c2[0] + 8 * G - 1) / (8 * G) << 16, m1 = c2[1] | (c2[1] + 8 * G - 1) / (8 * G) << 16;
     int sum = m0 + m1;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -375,46 +392,59 @@ __device__ __forceinline__ void make_plan(const MoeArgs& a, int* tmp) {
     }
     if (lane == 31) totals[warp] = sum;
     __syncthreads();
-    int before = 0, all = 0;
+    int base = 0, all = 0;
 #pragma unroll
-    for (int w = 0; w < kPlanThreads / 32; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
         const int x = totals[w];
-        if (w < warp) before += x;
+        if (w < warp) base += x;
         all += x;
     }
-    const int slots = all >> 16, at0 = before + sum - m0 - m1;
+    const int slots = all >> 16, at0 = base + sum - m0 - m1;
     if (e0 < a.E) from[e0] = at0;
     if (e0 + 1 < a.E) from[e0 + 1] = at0 + m0;
-    if (t == kPlanThreads - 1) {
+    if (warp == kWarps - 1 && lane < 4) {      // the products' runs: a divisor a lane
+        const bool down = lane >= 2;
+        const FewRun run = down ? FewRun(a.kf, slots * (int)a.kd.d, a.ctas2)
+                                : FewRun(a.kd, 2 * slots * (int)a.kf.d, a.ctas1);
+        const FastDiv d(lane & 1 ? run.least + 1 : run.least);
         PlanHead* h = const_cast<PlanHead*>(p.head);
-        h->slots = slots;
-        h->join[0] = FewJoin(FewRun(a.kd, 2 * slots * (int)a.kf.d, a.ctas1));
-        h->join[1] = FewJoin(FewRun(a.kf, slots * (int)a.kd.d, a.ctas2));
+        FewJoin* join = h->join + (down ? 1 : 0);
+        if (lane & 1) join->more = d;
+        else { join->run = run; join->least = d; }
+        if (lane == 0) h->slots = slots;
     }
     __syncthreads();
     for (int i = t; i < P; i += kPlanThreads) {
-        const int e = tmp[i], f = from[e], r = rank[i], slot = (f >> 16) + r / (8 * G);
+        const int e = where[i] >> 8, f = from[e], r = before[(i >> 5) * a.E + e] + (where[i] & 0xFF);
+        const int slot = (f >> 16) + r / (8 * G);
         p.pair[(f & 0xFFFF) + r] = i;
         a.place[i] = slot << 8 | r % (8 * G);
         if (r % (8 * G)) continue;
         p.slot[slot] = make_int2(e, ((f & 0xFFFF) + r) << 8 | min(8 * G, count[e] - r));
 #pragma unroll
         for (int m = 0; m < 3; ++m) {
-            p.tiles[m * (a.slots_max + 1) + slot] = a.chosen[i].tiles[m];
-            p.K[m * (a.slots_max + 1) + slot] = a.chosen[i].K[m];
+            p.tiles[m * (a.slots_max + 1) + slot] = i == t ? own.tiles[m] : a.chosen[i].tiles[m];
+            p.K[m * (a.slots_max + 1) + slot] = i == t ? own.K[m] : a.chosen[i].K[m];
         }
     }
 }
 
+__device__ __forceinline__ void prefetch_bytes(const void* p, uint32_t bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" :: "l"(p), "r"(bytes) : "memory");
+}
+
 // Rotate the tokens for gate and up of every chosen expert (a warp a block); the last
-// CTA makes the plan.
+// CTA makes the plan.  What the joins will want of the experts is brought into L2
+// meanwhile.  (Bringing the tensors, too, delayed the rotation itself: one token 35 -> 43
+// us, nine tokens through large experts 104 -> 140.)
 template <int G>
-__global__ void __launch_bounds__(kPlanThreads) moe_rotate_kernel(const MoeArgs a, const FastDiv top_k) {
+__global__ void __launch_bounds__(kPlanThreads)
+moe_rotate_kernel(const MoeArgs a, const FastDiv top_k) {
     extern __shared__ __align__(16) uint8_t sm[];
     pdl_wait();
     pdl_launch();
     if (blockIdx.x == gridDim.x - 1) {
-        make_plan<G>(a, reinterpret_cast<int*>(sm));
+        make_plan<G>(a, sm);
         return;
     }
     const int lane = threadIdx.x & 31, P = a.T * a.top_k, kd = (int)a.kd.d;
@@ -422,10 +452,16 @@ __global__ void __launch_bounds__(kPlanThreads) moe_rotate_kernel(const MoeArgs 
     int pair;
     const int b = a.kd.mod(i, pair), k = b * 128 + 4 * lane;
     if (pair >= P) return;
+    const Chosen& ch = a.chosen[pair];
     float x[4], s[2][4];
     load4x(a.x, (size_t)top_k.div(pair) * a.ldx + k, a.dtype, x);
-    load4(a.chosen[pair].suh[0] + k, s[0]);
-    load4(a.chosen[pair].suh[1] + k, s[1]);
+    load4(ch.suh[0] + k, s[0]);
+    load4(ch.suh[1] + k, s[1]);
+    if (lane < 4) {            // block b of svh down; the others of F are shared out
+        const __half* v = lane == 0 ? ch.svh[2] : lane == 1 ? ch.svh[0] : lane == 2 ? ch.svh[1] : ch.suh[2];
+        const int n = lane == 0 ? kd : (int)a.kf.d;
+        for (int f = b; f < n; f += kd) prefetch_bytes(v + f * 128, 256);
+    }
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
         float v[4];
@@ -633,35 +669,40 @@ static size_t moe_layout(MoeArgs* a, int T, int D, int F, int E, int top_k, int 
     return off;
 }
 
+template <bool F32, int TT>
+static int router_launch(const MoeArgs& a, cudaStream_t stream) {
+    return launch_kernel<moe_router_kernel<F32, TT>>("moe_router launch", dim3(kRouterRanks, (a.T + TT - 1) / TT),
+                                                     kRouterThreads, 0, false, stream, a);
+}
+
 template <int CODE, int G>
 static int moe_run(const MoeArgs& a, int sms, cudaStream_t stream) {
     const int P = a.T * a.top_k, kd = a.D >> 7, kf = a.F >> 7;
     // tokens of a cluster: as many as it takes for all clusters to run at once
     const int most = sms / kRouterRanks, tt = a.T <= most ? 1 : a.T <= 2 * most ? 2 : 4;
-    auto router = a.router_dtype == 0 ? (tt == 1 ? moe_router_kernel<true, 1> :
-                                         tt == 2 ? moe_router_kernel<true, 2> : moe_router_kernel<true, 4>)
-                                      : (tt == 1 ? moe_router_kernel<false, 1> :
-                                         tt == 2 ? moe_router_kernel<false, 2> : moe_router_kernel<false, 4>);
-    int rc = launch_kernel(router, "moe_router launch", dim3(kRouterRanks, (a.T + tt - 1) / tt),
-                           kRouterThreads, 0, false, stream, a);
+    int rc = a.router_dtype == 0
+                 ? (tt == 1 ? router_launch<true, 1>(a, stream) :
+                    tt == 2 ? router_launch<true, 2>(a, stream) : router_launch<true, 4>(a, stream))
+                 : (tt == 1 ? router_launch<false, 1>(a, stream) :
+                    tt == 2 ? router_launch<false, 2>(a, stream) : router_launch<false, 4>(a, stream));
     if (rc) return rc;
     constexpr int kWarps = kPlanThreads / 32;
-    rc = launch_kernel(moe_rotate_kernel<G>, "moe_rotate launch", dim3((P * kd + kWarps - 1) / kWarps + 1),
-                       kPlanThreads, 8 * (P + a.E), true, stream, a, FastDiv(a.top_k));
+    rc = launch_kernel<moe_rotate_kernel<G>>("moe_rotate launch", dim3((P * kd + kWarps - 1) / kWarps + 1),
+                       kPlanThreads, plan_scratch(P, a.E), true, stream, a, FastDiv(a.top_k));
     if (rc) return rc;
     const int K1 = a.Kmax[0] > a.Kmax[1] ? a.Kmax[0] : a.Kmax[1], plan = plan_bytes(P, a.slots_max);
     const int at1 = up16(few_smem(K1, G, kFewGroups * kRowStages));
     const int at2 = up16(few_smem(a.Kmax[2], G, kFewGroups * kRowStages));
-    rc = launch_kernel(moe_gate_up_kernel<CODE, G>, "moe_gate_up launch", dim3(a.ctas1), 32 * kFewWarps,
+    rc = launch_kernel<moe_gate_up_kernel<CODE, G>>("moe_gate_up launch", dim3(a.ctas1), 32 * kFewWarps,
                        at1 + plan, true, stream, a, at1);
     if (rc) return rc;
-    rc = launch_kernel(moe_gate_up_finish_kernel<G>, "moe_gate_up_finish launch", dim3((P * kf + 3) / 4),
+    rc = launch_kernel<moe_gate_up_finish_kernel<G>>("moe_gate_up_finish launch", dim3((P * kf + 3) / 4),
                        128, 0, true, stream, a);
     if (rc) return rc;
-    rc = launch_kernel(moe_down_kernel<CODE, G>, "moe_down launch", dim3(a.ctas2), 32 * kFewWarps,
+    rc = launch_kernel<moe_down_kernel<CODE, G>>("moe_down launch", dim3(a.ctas2), 32 * kFewWarps,
                        at2 + plan, true, stream, a, at2);
     if (rc) return rc;
-    return launch_kernel(moe_down_finish_kernel<G>, "moe_down_finish launch", dim3(kd, a.T), 128, 0, true,
+    return launch_kernel<moe_down_finish_kernel<G>>("moe_down_finish launch", dim3(kd, a.T), 128, 0, true,
                          stream, a);
 }
 

@@ -22,7 +22,7 @@ from pathlib import Path
 import torch
 
 from . import ops
-from .native import call, lib
+from .native import check, lib
 
 DTYPE_IDS = {torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
@@ -58,9 +58,14 @@ class TrellisWeight:
             raise ValueError("trellis, suh and svh must be on one CUDA device")
         self.k, self.n, self.K, self.code = k, n, K, code
         self.device = trellis.device
+        self.index = trellis.device.index       # of the device
+        self._bytes = {}                        # rows -> workspace bytes of linear
         self.trellis = _aligned(trellis.detach(), 16)
         self.suh = _aligned(suh.detach().half(), 8)
         self.svh = _aligned(svh.detach().half(), 8)
+        # trellis, K, code, suh, svh as the C ABI takes them
+        self._args = (self.trellis.data_ptr(), K, self.code_id, self.suh.data_ptr(),
+                      self.svh.data_ptr())
         with torch.cuda.device(self.device):
             ops.select_device(self.trellis)
 
@@ -95,36 +100,40 @@ class TrellisWeight:
 
 # ------------------------------------------------------------------ arguments
 def _no_grad(op: str, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{op} has no gradient: call it under torch.no_grad() or on detached "
-                         "tensors")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{op} has no gradient: call it under torch.no_grad() or on "
+                                 "detached tensors")
 
 
-def _check_input(op: str, what: str, t: torch.Tensor, shape, dtype, device):
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != device:
-        raise ValueError(f"{op}: {what} must be {tuple(shape)} {dtype} on {device}, got "
+def _check_input(op: str, what: str, t: torch.Tensor, shape, dtype, index: int):
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != index:
+        raise ValueError(f"{op}: {what} must be {tuple(shape)} {dtype} on device {index}, got "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
 
 
-def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
-    """t as [rows, cols] the kernels can read: unit inner stride, rows on 8-byte
-    boundaries (a copy where it is not so already)."""
-    t = t.reshape(-1, cols)
-    if t.stride(1) == 1 and t.data_ptr() % 8 == 0 and \
-            (t.shape[0] <= 1 or (t.stride(0) >= cols and t.stride(0) % 4 == 0)):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
-
-
-def _ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _rows(t: torch.Tensor, cols: int, align: int = 8):
+    """(t as [rows, cols], its row pitch) as the kernels can read it: unit inner
+    stride, rows on `align`-byte boundaries of 2-byte elements (a copy where it is not
+    so already)."""
+    if t.dim() != 2:
+        t = t.reshape(-1, cols)
+    ld, inner = t.stride()
+    if inner == 1 and ld >= cols and ld % (align // 2) == 0 and t.data_ptr() % align == 0:
+        return t, ld
+    if t.shape[0] <= 1 and inner == 1 and t.data_ptr() % align == 0:
+        return t, cols
+    return t.clone(memory_format=torch.contiguous_format), cols
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two [rows, cols] views of 2-byte elements share memory."""
     if a.numel() == 0 or b.numel() == 0:
         return False
-    pa, pb, la, lb = a.data_ptr(), b.data_ptr(), _ld(a), _ld(b)
+    la = a.stride(0) if a.shape[0] > 1 else a.shape[1]
+    lb = b.stride(0) if b.shape[0] > 1 else b.shape[1]
+    pa, pb = a.data_ptr(), b.data_ptr()
     if pa >= pb + 2 * ((b.shape[0] - 1) * lb + b.shape[1]) or \
             pb >= pa + 2 * ((a.shape[0] - 1) * la + a.shape[1]):
         return False
@@ -134,36 +143,63 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return True
 
 
-def _out_rows(op: str, out, lead, cols: int, x: torch.Tensor, sources) -> torch.Tensor:
-    """The [rows, cols] view to write: a new tensor, or the caller's `out`.  The
-    kernel reads `sources` ([rows, cols], element by element where it writes) and
-    x (as a whole): out may be one of the sources, and nothing else of them."""
-    if out is None:
-        return torch.empty(*lead, cols, dtype=x.dtype, device=x.device).view(-1, cols)
-    _check_input(op, "out", out, (*lead, cols), x.dtype, x.device)
+def _out_rows(op: str, out: torch.Tensor, shape, x: torch.Tensor, index: int, sources):
+    """([rows, cols] view of the caller's `out`, its pitch).  The kernels read `sources`
+    ([rows, cols], element by element where they write) and x (as a whole): out may
+    be one of the sources, and nothing else of them."""
+    cols = shape[-1]
+    _check_input(op, "out", out, shape, x.dtype, index)
     try:
         o = out.view(-1, cols)
     except RuntimeError:
         raise ValueError(f"{op}: out {tuple(out.shape)} with strides {out.stride()} is not "
                          "a matrix of rows") from None
+    many = o.shape[0] > 1
     if o.numel() and (o.stride(1) != 1 or o.data_ptr() % 8 or
-                      (o.shape[0] > 1 and (o.stride(0) < cols or o.stride(0) % 4))):
+                      (many and (o.stride(0) < cols or o.stride(0) % 4))):
         raise ValueError(f"{op}: out must have unit inner stride and rows on 8-byte boundaries")
     if _overlap(o, x):
         raise ValueError(f"{op}: out overlaps x")
     for s in sources:
         if s is not None and _overlap(o, s) and not (
-                s.data_ptr() == o.data_ptr() and s.shape == o.shape and _ld(s) == _ld(o)):
+                s.data_ptr() == o.data_ptr() and s.shape == o.shape and
+                (not many or s.stride(0) == o.stride(0))):
             raise ValueError(f"{op}: out overlaps an input it is not equal to")
-    return o
+    return o, (o.stride(0) if many else cols)
 
 
-def _workspace(nbytes: int, device):
-    """(tensor or None, pointer) of stream-ordered scratch."""
-    if not nbytes:
-        return None, 0
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return ws, ws.data_ptr()
+_functions: dict = {}
+# the current stream's handle, without a Stream object where torch offers that
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _call(name: str, index: int, args):
+    """A C ABI entry point on torch's current stream of device `index`, which is made
+    current in the library (it has its own CUDA runtime) and, where it is not, in torch."""
+    f = _functions.get(name)
+    if f is None:
+        f = _functions[name] = getattr(lib(), name)
+        _functions["select"] = None if torch.cuda.device_count() == 1 else lib().exl3b_device_init
+    select = _functions["select"]
+    if select is not None:              # with one device it is always the current one
+        if torch.cuda.current_device() != index:
+            with torch.cuda.device(index):
+                return _call(name, index, args)
+        check("exl3b_device_init", select(index))
+    check(name, f(*args, _raw_stream(index)))
+
+
+def _scratch(cache: dict, key, index: int, size, *args) -> int:
+    """size(*args) bytes of workspace, remembered for a few keys."""
+    nbytes = cache.get(key)
+    if nbytes is None:
+        with torch.cuda.device(index):
+            check("exl3b_device_init", lib().exl3b_device_init(index))
+            nbytes = size(*args)
+        if len(cache) < 64:
+            cache[key] = nbytes
+    return nbytes
 
 
 # ------------------------------------------------------------------ linear
@@ -178,39 +214,48 @@ def linear(x: torch.Tensor, w: TrellisWeight, bias: torch.Tensor | None = None,
     activation: None, "relu", "silu", "gelu" (erf) or "gelu_tanh".  Returns
     [..., n] in x's dtype, or writes `out`, which may be `mul` or `residual`
     themselves.  The sums and the epilogue are fp32, rounded once."""
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"activation {activation!r}: one of {sorted(map(str, ACTIVATIONS))}")
-    if x.dtype not in DTYPE_IDS:
+    dt, k, n, index = DTYPE_IDS.get(x.dtype), w.k, w.n, w.index
+    if dt is None:
         raise ValueError(f"x must be bf16 or fp16, got {x.dtype}")
-    if x.device != w.device:
+    if x.get_device() != index:
         raise ValueError(f"x is on {x.device}, the weight on {w.device}")
-    if x.dim() < 1 or x.shape[-1] != w.k:
-        raise ValueError(f"x {tuple(x.shape)} for a weight with in = {w.k}")
+    shape = x.shape
+    if not shape or shape[-1] != k:
+        raise ValueError(f"x {tuple(shape)} for a weight with in = {k}")
     _no_grad("linear", x, bias, mul, residual)
-    lead = x.shape[:-1]
+    shape = (*shape[:-1], n)
+    bias_ptr = mul_ptr = res_ptr = ldm = ldr = 0
+    mr = rr = None
     if bias is not None:
-        _check_input("linear", "bias", bias, (w.n,), x.dtype, x.device)
+        _check_input("linear", "bias", bias, (n,), x.dtype, index)
         bias = _aligned(bias, 8)
-    for what, t in (("mul", mul), ("residual", residual)):
-        if t is not None:
-            _check_input("linear", what, t, (*lead, w.n), x.dtype, x.device)
-    xr = _rows(x, w.k)
-    mr = None if mul is None else _rows(mul, w.n)
-    rr = None if residual is None else _rows(residual, w.n)
-    o = _out_rows("linear", out, lead, w.n, xr, (mr, rr))
+        bias_ptr = bias.data_ptr()
+    if mul is not None:
+        _check_input("linear", "mul", mul, shape, x.dtype, index)
+        mr, ldm = _rows(mul, n)
+        mul_ptr = mr.data_ptr()
+    if residual is not None:
+        _check_input("linear", "residual", residual, shape, x.dtype, index)
+        rr, ldr = _rows(residual, n)
+        res_ptr = rr.data_ptr()
+    xr, ldx = _rows(x, k)
+    if out is None:
+        y = o = x.new_empty(shape)
+        ldo = n
+    else:
+        y = out
+        o, ldo = _out_rows("linear", out, shape, xr, index, (mr, rr))
     M = xr.shape[0]
     if M:
-        with torch.cuda.device(x.device):
-            dev = ops.select_device(xr)
-            nbytes = lib().exl3b_linear_workspace_bytes(M, w.k, w.n)
-            ws, ws_ptr = _workspace(nbytes, x.device)
-            call("exl3b_linear", xr.data_ptr(), DTYPE_IDS[x.dtype], _ld(xr), M, w.k, w.n,
-                 w.trellis.data_ptr(), w.K, w.code_id, w.suh.data_ptr(), w.svh.data_ptr(),
-                 0 if bias is None else bias.data_ptr(), ACTIVATIONS[activation],
-                 0 if mr is None else mr.data_ptr(), 0 if mr is None else _ld(mr),
-                 0 if rr is None else rr.data_ptr(), 0 if rr is None else _ld(rr),
-                 o.data_ptr(), _ld(o), ws_ptr, nbytes, ops.stream_handle(dev))
-    return o.view(*lead, w.n) if out is None else out
+        nbytes = _scratch(w._bytes, M, index, lib().exl3b_linear_workspace_bytes, M, k, n)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        _call("exl3b_linear", index,
+              (xr.data_ptr(), dt, ldx, M, k, n, *w._args, bias_ptr, act, mul_ptr, ldm, res_ptr,
+               ldr, o.data_ptr(), ldo, ws.data_ptr(), nbytes))
+    return y
 
 
 # ------------------------------------------------------------------ mixture of experts
@@ -238,22 +283,14 @@ class TrellisExperts:
                 if (w.k, w.n) != shape or w.code != first.code or w.device != first.device:
                     raise ValueError(f"{what} of expert {e} is {w}, expected [{shape[0]}, "
                                      f"{shape[1]}] {first.code} on {first.device}")
-        self.device, self.code_id = first.device, first.code_id
+        self.device, self.index, self.code_id = first.device, first.index, first.code_id
         self.weights = (gate, up, down)
+        self._bytes = {}                        # (tokens, top_k) -> workspace bytes of moe
         self.Kmax = tuple(max(w.K for w in ws) for ws in self.weights)
         table = b"".join(struct.pack("<QQQii", w.trellis.data_ptr(), w.suh.data_ptr(),
                                      w.svh.data_ptr(), w.K, 0)
                          for ws in self.weights for w in ws)
         self.table = torch.frombuffer(bytearray(table), dtype=torch.uint8).to(self.device)
-
-
-def _rows16(t: torch.Tensor, cols: int) -> torch.Tensor:
-    """_rows with 16-byte aligned rows (8 elements of 2 bytes, 4 of 4)."""
-    t = t.reshape(-1, cols)
-    if t.stride(1) == 1 and t.data_ptr() % 16 == 0 and \
-            (t.shape[0] <= 1 or (t.stride(0) >= cols and t.stride(0) % 8 == 0)):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
 
 
 def moe(x: torch.Tensor, router: torch.Tensor, experts: TrellisExperts, top_k: int,
@@ -270,39 +307,47 @@ def moe(x: torch.Tensor, router: torch.Tensor, experts: TrellisExperts, top_k: i
     (or 2048 choices) are taken in pieces of that many; a chosen expert is read once
     for 8 or 16 of its tokens, so long prompts are better served by linear per
     expert."""
-    if x.dtype not in DTYPE_IDS:
+    dt, D, index = DTYPE_IDS.get(x.dtype), experts.D, experts.index
+    if dt is None:
         raise ValueError(f"x must be bf16 or fp16, got {x.dtype}")
-    if x.device != experts.device:
+    if x.get_device() != index:
         raise ValueError(f"x is on {x.device}, the experts on {experts.device}")
-    if x.dim() < 1 or x.shape[-1] != experts.D:
-        raise ValueError(f"x {tuple(x.shape)} for experts with in = {experts.D}")
+    shape = x.shape
+    if not shape or shape[-1] != D:
+        raise ValueError(f"x {tuple(shape)} for experts with in = {D}")
     top_k = int(top_k)
     if not 1 <= top_k <= min(experts.E, MOE_TOP_K):
         raise ValueError(f"top_k={top_k} with {experts.E} experts (at most {MOE_TOP_K})")
-    if router.dtype not in (x.dtype, torch.float32):
+    if router.dtype is not x.dtype and router.dtype is not torch.float32:
         raise ValueError(f"router must be {x.dtype} or float32, got {router.dtype}")
-    _check_input("moe", "router", router, (experts.E, experts.D), router.dtype, x.device)
+    _check_input("moe", "router", router, (experts.E, D), router.dtype, index)
     _no_grad("moe", x, router, residual)
-    lead, D = x.shape[:-1], experts.D
+    rr, res_ptr, ldr = None, 0, 0
     if residual is not None:
-        _check_input("moe", "residual", residual, (*lead, D), x.dtype, x.device)
-    xr = _rows16(x, D)
-    rt = _rows16(router, D)
-    rr = None if residual is None else _rows(residual, D)
-    o = _out_rows("moe", out, lead, D, xr, (rr,))
+        _check_input("moe", "residual", residual, shape, x.dtype, index)
+        rr, ldr = _rows(residual, D)
+        res_ptr = rr.data_ptr()
+    xr, ldx = _rows(x, D, 16)
+    rt, ldt = _rows(router, D, 16)
+    if out is None:
+        y = o = x.new_empty(shape)
+        ldo = D
+    else:
+        y = out
+        o, ldo = _out_rows("moe", out, shape, xr, index, (rr,))
     T = xr.shape[0]
     if T:
-        with torch.cuda.device(x.device):
-            dev = ops.select_device(xr)
-            most = min(MOE_TOKENS, MOE_PAIRS // top_k)
-            nbytes = lib().exl3b_moe_workspace_bytes(min(T, most), D, experts.F, experts.E, top_k)
-            ws, ws_ptr = _workspace(nbytes, x.device)
-            for t in range(0, T, most):
-                n = min(most, T - t)
-                call("exl3b_moe", xr[t:].data_ptr(), DTYPE_IDS[x.dtype], _ld(xr), n, D, experts.F,
-                     experts.E, top_k, int(bool(normalize)), rt.data_ptr(),
-                     0 if router.dtype == torch.float32 else DTYPE_IDS[x.dtype], _ld(rt),
-                     experts.table.data_ptr(), *experts.Kmax, experts.code_id,
-                     0 if rr is None else rr[t:].data_ptr(), 0 if rr is None else _ld(rr),
-                     o[t:].data_ptr(), _ld(o), ws_ptr, nbytes, ops.stream_handle(dev))
-    return o.view(*lead, D) if out is None else out
+        most = min(MOE_TOKENS, MOE_PAIRS // top_k)
+        nbytes = _scratch(experts._bytes, (min(T, most), top_k), index,
+                          lib().exl3b_moe_workspace_bytes, min(T, most), D, experts.F, experts.E,
+                          top_k)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        rdt = 0 if router.dtype is torch.float32 else dt
+        for t in range(0, T, most):
+            _call("exl3b_moe", index,
+                  (xr.data_ptr() + 2 * t * ldx, dt, ldx, min(most, T - t), D, experts.F, experts.E,
+                   top_k, 1 if normalize else 0, rt.data_ptr(), rdt, ldt,
+                   experts.table.data_ptr(), *experts.Kmax, experts.code_id,
+                   res_ptr + 2 * t * ldr if res_ptr else 0, ldr, o.data_ptr() + 2 * t * ldo, ldo,
+                   ws.data_ptr(), nbytes))
+    return y

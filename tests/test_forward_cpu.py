@@ -58,7 +58,7 @@ def test_weight_refuses():
 class _Weight:
     """Stands for a weight where a call must be refused before any kernel."""
     k, n, K, code_id = 256, 128, 4, 0
-    device = torch.device("cpu")
+    device, index = torch.device("cpu"), -1            # what CPU tensors answer
 
 
 def test_linear_refuses():
@@ -160,7 +160,7 @@ def test_experts_and_moe_refuse():
     class W:
         def __init__(self, k, n, code="exl3_mul1"):
             self.k, self.n, self.K, self.code, self.code_id = k, n, 4, code, 0
-            self.device = torch.device("cpu")
+            self.device, self.index = torch.device("cpu"), -1
             self.trellis = self.suh = self.svh = torch.zeros(1)
     g, d = W(256, 128), W(128, 256)
     for args, msg in [(([], [], []), "one of each"), (([g], [g, g], [d]), "one of each"),

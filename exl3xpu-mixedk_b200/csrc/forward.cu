@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(128) linear_rotate_kernel(const LinearArgs a, 
 // Units: (group of 8 G rows, column block).
 template <int G, bool ROTATE>
 struct LinearJob {
-    static constexpr bool kRotate = ROTATE;
+    static constexpr bool kRotate = ROTATE, kLo = false;
     const LinearArgs& a;
     const FewScratch& w;
     const FastDiv& nbn;

@@ -92,9 +92,12 @@ __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;"
 // two (block_scale; its reciprocal goes to *inv_scale).  The 16 k of a tile are
 // stored so that a lane's four values, and those of the next tile, are 16 bytes.
 // Rounding to fp16 (2^-11 relative at most) matches the weights' type, which a
-// matrix instruction needs; bf16 would cost three bits of the activations.
+// matrix instruction needs; bf16 would cost three bits of the activations.  With LO,
+// what the rounding left is stored as well, at dst + lo, rounded to fp16 itself: the
+// pair holds 22 bits of the values (to 2^-25 of the block's largest).
+template <bool LO = false>
 __device__ __forceinline__ void few_put_block(float (&v)[4], uint8_t* dst, float* inv_scale,
-                                              int lane, int swz) {
+                                              int lane, int swz, size_t lo = 0) {
     float m = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -109,12 +112,19 @@ __device__ __forceinline__ void few_put_block(float (&v)[4], uint8_t* dst, float
     const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
     *reinterpret_cast<__half2*>(dst + ((2 * off) ^ swz)) = a;
     *reinterpret_cast<__half2*>(dst + ((2 * off + 16) ^ swz)) = b;
+    if constexpr (LO) {
+        const float2 fa = __half22float2(a), fb = __half22float2(b);
+        *reinterpret_cast<__half2*>(dst + lo + ((2 * off) ^ swz)) =
+            __floats2half2_rn(v[0] - fa.x, v[1] - fa.y);
+        *reinterpret_cast<__half2*>(dst + lo + ((2 * off + 16) ^ swz)) =
+            __floats2half2_rn(v[2] - fb.x, v[3] - fb.y);
+    }
     if (lane == 0) *inv_scale = inv;
 }
 
 // acc[g][..] += one k block: the warp's eight tiles at `tiles`, rows 8 g .. 8 g + 7 of
-// the block at `xh`, reciprocal scales inv [8 G].
-template <int K, int CODE, int G>
+// the block at `xh` (with LO, their remainders 8 G rows on), reciprocal scales inv [8 G].
+template <int K, int CODE, int G, bool LO>
 __device__ __forceinline__ void few_block(const LaneWindow<K>& lw, const uint8_t* tiles_,
                                           const uint8_t* xh, const float* inv, float (&acc)[G][4],
                                           int lane) {
@@ -127,17 +137,18 @@ __device__ __forceinline__ void few_block(const LaneWindow<K>& lw, const uint8_t
     for (int g = 0; g < G; ++g) blk[g][0] = blk[g][1] = blk[g][2] = blk[g][3] = 0.0f;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
-        uint4 x[G];
+        constexpr int N = LO ? 2 * G : G;
+        uint4 x[N];
 #pragma unroll
-        for (int g = 0; g < G; ++g)
+        for (int g = 0; g < N; ++g)
             x[g] = *reinterpret_cast<const uint4*>((p & 1 ? odd : even) + g * 8 * kRowBytes + p * 64);
         uint32_t a[4];
         decode_tile<K, CODE>(tiles + (2 * p) * 8 * K, lw, a);
 #pragma unroll
-        for (int g = 0; g < G; ++g) mma_16816(blk[g], a, x[g].x, x[g].y);
+        for (int g = 0; g < N; ++g) mma_16816(blk[g % G], a, x[g].x, x[g].y);
         decode_tile<K, CODE>(tiles + (2 * p + 1) * 8 * K, lw, a);
 #pragma unroll
-        for (int g = 0; g < G; ++g) mma_16816(blk[g], a, x[g].z, x[g].w);
+        for (int g = 0; g < N; ++g) mma_16816(blk[g % G], a, x[g].z, x[g].w);
     }
 #pragma unroll
     for (int g = 0; g < G; ++g) {
@@ -234,8 +245,8 @@ __host__ __device__ inline size_t few_park_bytes(int units, int ctas, int G) {
 // Shared memory of the product: weight rings, then the rows -- rings of kRowStages
 // blocks per group, or (rotated in place) all `blocks` of the run.
 constexpr int kFewRoom = 222 * 1024;      // of the 227 KB a CTA may have
-__host__ __device__ inline int few_smem(int Kmax, int G, int blocks) {
-    return kFewWarps * few_ring_bytes(Kmax) + blocks * 8 * G * (kRowBytes + 4);
+__host__ __device__ inline int few_smem(int Kmax, int G, int blocks, bool lo = false) {
+    return kFewWarps * few_ring_bytes(Kmax) + blocks * 8 * G * ((lo ? 2 : 1) * kRowBytes + 4);
 }
 
 // A job tells what the units are.  Its Cursor stands at one unit: tiles (first tile of
@@ -245,6 +256,7 @@ __host__ __device__ inline int few_smem(int Kmax, int G, int blocks) {
 // and, unless kRotate,
 //   row(u, r) -> index of block 0 of the unit's row r among the rotated blocks (256
 //                bytes each at xh(), reciprocal scales at inv()); block b is b * kRowStep on
+//   lo()      with kLo, bytes from a rotated block to its remainders
 //   wait()    -> returns once the rows are there
 // or, with kRotate (every unit has the same rows),
 //   rotate(r, b, dst, inv, swz)   puts block b of row r itself (a warp)
@@ -264,8 +276,11 @@ __device__ __forceinline__ void few_run(const Job& job, const FewRun& run, int K
     const int kb = (int)run.kb.d;
     uint8_t* ring = sm + warp * few_ring_bytes(Kmax);
     const int blocks = Job::kRotate ? count : kFewGroups * kRowStages;
+    constexpr bool LO = Job::kLo;
+    constexpr int kBlockBytes = 8 * G * (LO ? 2 : 1) * kRowBytes;
+    static_assert(!(LO && Job::kRotate), "rows rotated in place have no remainders");
     uint8_t* xh = sm + kFewWarps * few_ring_bytes(Kmax);
-    float* inv = reinterpret_cast<float*>(xh + blocks * 8 * G * kRowBytes);
+    float* inv = reinterpret_cast<float*>(xh + blocks * kBlockBytes);
     const int mine = Job::kRotate ? 0 : grp * kRowStages;      // the group's first row stage
     int u0;
     const int b0 = run.kb.mod(g0, u0);
@@ -278,10 +293,12 @@ __device__ __forceinline__ void few_run(const Job& job, const FewRun& run, int K
     u += u0;
     auto at = job.cursor(u);
     bool waited = false;
-    // this warp's rows of a block: G, sixteen lanes each
+    // this warp's rows of a block: G, sixteen lanes each; a single row's remainders by
+    // the other sixteen
+    constexpr bool kHalves = LO && G == 1;
     const int rr = G == 1 ? col : 2 * col + (lane >> 4);
-    const uint32_t rdst = (uint32_t)__cvta_generic_to_shared(xh) + mine * 8 * G * kRowBytes +
-                          rr * kRowBytes + few_swizzle(rr, 16 * (lane & 15));
+    const uint32_t rdst = (uint32_t)__cvta_generic_to_shared(xh) + mine * kBlockBytes + rr * kRowBytes +
+                          few_swizzle(rr, 16 * (lane & 15)) + (kHalves ? (lane >> 4) * 8 * kRowBytes : 0);
     const uint32_t idst = (uint32_t)__cvta_generic_to_shared(inv) + 4 * (mine * 8 * G + rr);
     // Stretches of equal bit width: the weight ring restarts where it changes.
     while (i < count) {
@@ -302,10 +319,11 @@ __device__ __forceinline__ void few_run(const Job& job, const FewRun& run, int K
                 st.seek(to.tiles + (size_t)ib * 8 * to.kt_bytes + (size_t)col * 32 * K, to.kt_bytes);
                 step = (size_t)kFewGroups * 8 * to.kt_bytes;
                 if constexpr (!Job::kRotate) {
-                    has = rr < job.rows(iu) && (G == 2 || lane < 16);
+                    has = rr < job.rows(iu) && (G == 2 || LO || lane < 16);
                     if (has) {
                         const size_t from = job.row(iu, rr) + (size_t)ib * job.row_step();
                         xsrc = job.xh() + from * kRowBytes + 16 * (lane & 15);
+                        if constexpr (kHalves) xsrc += lane < 16 ? 0 : job.lo();
                         isrc = job.inv() + from;
                     }
                     xstep = (size_t)kFewGroups * job.row_step();
@@ -317,8 +335,12 @@ __device__ __forceinline__ void few_run(const Job& job, const FewRun& run, int K
                 if constexpr (!Job::kRotate) {
                     if (has) {
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
-                                     :: "r"(rdst + stage * 8 * G * kRowBytes), "l"(xsrc) : "memory");
-                        if ((lane & 15) == 0)
+                                     :: "r"(rdst + stage * kBlockBytes), "l"(xsrc) : "memory");
+                        if constexpr (LO && G == 2)
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                                         :: "r"(rdst + stage * kBlockBytes + 8 * G * kRowBytes),
+                                            "l"(xsrc + job.lo()) : "memory");
+                        if (kHalves ? lane == 0 : (lane & 15) == 0)
                             asm volatile("cp.async.ca.shared.global [%0], [%1], 4;"
                                          :: "r"(idst + stage * 32 * G), "l"(isrc) : "memory");
                         xsrc += xstep * kRowBytes;
@@ -374,7 +396,7 @@ __device__ __forceinline__ void few_run(const Job& job, const FewRun& run, int K
                 const bool feed = left > 0;
                 if (feed) n = min(n, left);
                 const int from = Job::kRotate ? i : mine;
-                const uint8_t* x = xh + from * 8 * G * kRowBytes;
+                const uint8_t* x = xh + from * kBlockBytes;
                 const float* f = inv + from * 8 * G;
 #pragma unroll 1
                 for (int j = 0; j < n; ++j) {
@@ -387,14 +409,14 @@ __device__ __forceinline__ void few_run(const Job& job, const FewRun& run, int K
                     cp_wait<kFewStages - 1>();
                     if constexpr (Job::kRotate) {
                         __syncwarp();
-                        few_block<K, CODE, G>(lw, ring + cur * 256 * K, x, f, acc, lane);
-                        x += kFewGroups * 8 * G * kRowBytes;
+                        few_block<K, CODE, G, LO>(lw, ring + cur * 256 * K, x, f, acc, lane);
+                        x += kFewGroups * kBlockBytes;
                         f += kFewGroups * 8 * G;
                         __syncwarp();      // every lane has read the stage before it is refilled
                     } else {
                         asm volatile("bar.sync %0, 256;" :: "r"(1 + grp) : "memory");
-                        few_block<K, CODE, G>(lw, ring + cur * 256 * K, x + rcur * 8 * G * kRowBytes,
-                                              f + rcur * 8 * G, acc, lane);
+                        few_block<K, CODE, G, LO>(lw, ring + cur * 256 * K, x + rcur * kBlockBytes,
+                                                  f + rcur * 8 * G, acc, lane);
                         rcur = (rcur + 1) & (kRowStages - 1);
                         __syncwarp();
                     }

@@ -58,9 +58,9 @@ struct MoeArgs {
     int* place;                           // [T * top_k] slot << 8 | row of a pair
     uint8_t* plan;                        // PlanHead and arrays
     int ctas1, ctas2;                     // of the products
-    uint8_t* xh1;                         // [2][T * top_k][D / 128][256], few_put_block order
-    float* inv1;
-    uint8_t* xh2;                         // [T * top_k][F / 128][256]
+    uint8_t* xh1;                         // [2][T * top_k][D / 128][256], few_put_block order, and
+    float* inv1;                          //   as much again for the remainders (LO)
+    uint8_t* xh2;                         // [T * top_k][F / 128][256], and the remainders
     float* inv2;
     float* park;
 };
@@ -437,7 +437,7 @@ __device__ __forceinline__ void prefetch_bytes(const void* p, uint32_t bytes) {
 // CTA makes the plan.  What the joins will want of the experts is brought into L2
 // meanwhile.  (Bringing the tensors, too, delayed the rotation itself: one token 35 -> 43
 // us, nine tokens through large experts 104 -> 140.)
-template <int G>
+template <int G, bool LO>
 __global__ void __launch_bounds__(kPlanThreads)
 moe_rotate_kernel(const MoeArgs a, const FastDiv top_k) {
     extern __shared__ __align__(16) uint8_t sm[];
@@ -468,7 +468,7 @@ moe_rotate_kernel(const MoeArgs a, const FastDiv top_k) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) v[c] = x[c] * s[m][c];
         const size_t to = ((size_t)m * P + pair) * kd + b;
-        few_put_block(v, a.xh1 + to * kRowBytes, a.inv1 + to, lane, 0);
+        few_put_block<LO>(v, a.xh1 + to * kRowBytes, a.inv1 + to, lane, 0, (size_t)2 * P * kd * kRowBytes);
     }
 }
 
@@ -482,9 +482,9 @@ __device__ __forceinline__ Plan copy_plan(const MoeArgs& a, uint8_t* where) {
 }
 
 // Units: (tensor, slot, column block); rows: rotated rows of the pairs.
-template <int G>
+template <int G, bool LO>
 struct ExpertJob {
-    static constexpr bool kRotate = false;
+    static constexpr bool kRotate = false, kLo = LO;
     const MoeArgs& a;
     const Plan& p;
     const uint8_t* x;          // [kinds][P][kb][256]
@@ -493,6 +493,7 @@ struct ExpertJob {
     const FastDiv& cols;       // column blocks
     bool early;                // the rows are there already
     int first, slots;          // the first unit's tensor; slots of each
+    size_t remainders;
     struct Cursor {
         const uint8_t* tiles;
         uint32_t kt_bytes;
@@ -534,10 +535,11 @@ struct ExpertJob {
     __device__ __forceinline__ int row_step() const { return 1; }
     __device__ __forceinline__ const uint8_t* xh() const { return x; }
     __device__ __forceinline__ const float* inv() const { return s; }
+    __device__ __forceinline__ size_t lo() const { return remainders; }
     __device__ __forceinline__ void wait() const { if (!early) pdl_wait(); }
 };
 
-template <int CODE, int G>
+template <int CODE, int G, bool LO>
 __global__ void __launch_bounds__(32 * kFewWarps, 1) moe_gate_up_kernel(const MoeArgs a, int plan) {
     extern __shared__ __align__(16) uint8_t sm[];
     pdl_wait();
@@ -545,24 +547,26 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) moe_gate_up_kernel(const Mo
     const Plan p = copy_plan(a, sm + plan);
     const FewRun run = p.head->join[0].run;
     if (blockIdx.x >= run.ctas) return;
-    const ExpertJob<G> job = {a, p, a.xh1, a.inv1, (int)a.kd.d, a.kf, true, 0, p.head->slots};
+    const ExpertJob<G, LO> job = {a, p, a.xh1, a.inv1, (int)a.kd.d, a.kf, true, 0, p.head->slots,
+                                  (size_t)2 * a.T * a.top_k * a.kd.d * kRowBytes};
     few_run<CODE, G>(job, run, max(a.Kmax[0], a.Kmax[1]), sm, a.park);
 }
 
-template <int CODE, int G>
+template <int CODE, int G, bool LO>
 __global__ void __launch_bounds__(32 * kFewWarps, 1) moe_down_kernel(const MoeArgs a, int plan) {
     extern __shared__ __align__(16) uint8_t sm[];
     pdl_launch();
     const Plan p = copy_plan(a, sm + plan);
     const FewRun run = p.head->join[1].run;
     if (blockIdx.x >= run.ctas) return;
-    const ExpertJob<G> job = {a, p, a.xh2, a.inv2, (int)a.kf.d, a.kd, false, 2, p.head->slots};
+    const ExpertJob<G, LO> job = {a, p, a.xh2, a.inv2, (int)a.kf.d, a.kd, false, 2, p.head->slots,
+                                  (size_t)a.T * a.top_k * a.kf.d * kRowBytes};
     few_run<CODE, G>(job, run, a.Kmax[2], sm, a.park);
 }
 
 // h = silu(gate) * up of a (pair, column block of F), and the down projection's rotated
 // row: a warp each.
-template <int G>
+template <int G, bool LO>
 __global__ void __launch_bounds__(128) moe_gate_up_finish_kernel(const MoeArgs a) {
     const int lane = threadIdx.x & 31, i = blockIdx.x * 4 + (threadIdx.x >> 5);
     const int fbn = (int)a.kf.d;
@@ -587,7 +591,8 @@ __global__ void __launch_bounds__(128) moe_gate_up_finish_kernel(const MoeArgs a
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = silu_f(v[j] * sg[j]) * (h[j] * su[j]) * sd[j];
     const size_t to = (size_t)pair * fbn + fb;
-    few_put_block(v, a.xh2 + to * kRowBytes, a.inv2 + to, lane, 0);
+    few_put_block<LO>(v, a.xh2 + to * kRowBytes, a.inv2 + to, lane, 0,
+                      (size_t)a.T * a.top_k * fbn * kRowBytes);
 }
 
 // Weighted sum over a token's experts of one column block, and the residual: a CTA
@@ -646,9 +651,9 @@ static size_t moe_layout(MoeArgs* a, int T, int D, int F, int E, int top_k, int 
     uint8_t* wts = take(P * 4);
     uint8_t* place = take(P * 4);
     uint8_t* plan = take(plan_bytes((int)P, slots));
-    uint8_t* xh1 = take(2 * P * kd * kRowBytes);
+    uint8_t* xh1 = take(4 * P * kd * kRowBytes);       // with the remainders' half
     uint8_t* inv1 = take(2 * P * kd * 4);
-    uint8_t* xh2 = take(P * kf * kRowBytes);
+    uint8_t* xh2 = take(2 * P * kf * kRowBytes);
     uint8_t* inv2 = take(P * kf * 4);
     uint8_t* park = take(park1 > park2 ? park1 : park2);
     if (a) {
@@ -675,7 +680,7 @@ static int router_launch(const MoeArgs& a, cudaStream_t stream) {
                                                      kRouterThreads, 0, false, stream, a);
 }
 
-template <int CODE, int G>
+template <int CODE, int G, bool LO>
 static int moe_run(const MoeArgs& a, int sms, cudaStream_t stream) {
     const int P = a.T * a.top_k, kd = a.D >> 7, kf = a.F >> 7;
     // tokens of a cluster: as many as it takes for all clusters to run at once
@@ -687,19 +692,19 @@ static int moe_run(const MoeArgs& a, int sms, cudaStream_t stream) {
                     tt == 2 ? router_launch<false, 2>(a, stream) : router_launch<false, 4>(a, stream));
     if (rc) return rc;
     constexpr int kWarps = kPlanThreads / 32;
-    rc = launch_kernel<moe_rotate_kernel<G>>("moe_rotate launch", dim3((P * kd + kWarps - 1) / kWarps + 1),
+    rc = launch_kernel<moe_rotate_kernel<G, LO>>("moe_rotate launch", dim3((P * kd + kWarps - 1) / kWarps + 1),
                        kPlanThreads, plan_scratch(P, a.E), true, stream, a, FastDiv(a.top_k));
     if (rc) return rc;
     const int K1 = a.Kmax[0] > a.Kmax[1] ? a.Kmax[0] : a.Kmax[1], plan = plan_bytes(P, a.slots_max);
-    const int at1 = up16(few_smem(K1, G, kFewGroups * kRowStages));
-    const int at2 = up16(few_smem(a.Kmax[2], G, kFewGroups * kRowStages));
-    rc = launch_kernel<moe_gate_up_kernel<CODE, G>>("moe_gate_up launch", dim3(a.ctas1), 32 * kFewWarps,
+    const int at1 = up16(few_smem(K1, G, kFewGroups * kRowStages, LO));
+    const int at2 = up16(few_smem(a.Kmax[2], G, kFewGroups * kRowStages, LO));
+    rc = launch_kernel<moe_gate_up_kernel<CODE, G, LO>>("moe_gate_up launch", dim3(a.ctas1), 32 * kFewWarps,
                        at1 + plan, true, stream, a, at1);
     if (rc) return rc;
-    rc = launch_kernel<moe_gate_up_finish_kernel<G>>("moe_gate_up_finish launch", dim3((P * kf + 3) / 4),
+    rc = launch_kernel<moe_gate_up_finish_kernel<G, LO>>("moe_gate_up_finish launch", dim3((P * kf + 3) / 4),
                        128, 0, true, stream, a);
     if (rc) return rc;
-    rc = launch_kernel<moe_down_kernel<CODE, G>>("moe_down launch", dim3(a.ctas2), 32 * kFewWarps,
+    rc = launch_kernel<moe_down_kernel<CODE, G, LO>>("moe_down launch", dim3(a.ctas2), 32 * kFewWarps,
                        at2 + plan, true, stream, a, at2);
     if (rc) return rc;
     return launch_kernel<moe_down_finish_kernel<G>>("moe_down_finish launch", dim3(kd, a.T), 128, 0, true,
@@ -784,7 +789,11 @@ int exl3b_moe(const void* dX, int dtype, int64_t ldx, int T, int D, int F, int E
     a.residual = d_residual; a.ldres = ldres; a.out = dOut; a.ldo = ldo;
     moe_layout(&a, T, D, F, E, top_k, st->sms, static_cast<uint8_t*>(ws));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-#define EXL3B_MOE(C) (moe_groups(T, E, top_k) == 2 ? moe_run<C, 2>(a, st->sms, s) : moe_run<C, 1>(a, st->sms, s))
+    // fp16: the operands of the products keep what their rounding leaves (LO)
+#define EXL3B_MOE(C) \
+    (moe_groups(T, E, top_k) == 2 \
+         ? dtype == X_FP16 ? moe_run<C, 2, true>(a, st->sms, s) : moe_run<C, 2, false>(a, st->sms, s) \
+         : dtype == X_FP16 ? moe_run<C, 1, true>(a, st->sms, s) : moe_run<C, 1, false>(a, st->sms, s))
     switch (code) {
         case CODE_MUL1: return EXL3B_MOE(CODE_MUL1);
         case CODE_3INST: return EXL3B_MOE(CODE_3INST);

@@ -143,10 +143,11 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return True
 
 
-def _out_rows(op: str, out: torch.Tensor, shape, x: torch.Tensor, index: int, sources):
+def _out_rows(op: str, out: torch.Tensor, shape, x: torch.Tensor, index: int, sources,
+              other: str, o_t: torch.Tensor | None):
     """([rows, cols] view of the caller's `out`, its pitch).  The kernels read `sources`
-    ([rows, cols], element by element where they write) and x (as a whole): out may
-    be one of the sources, and nothing else of them."""
+    ([rows, cols], element by element where they write) and, as a whole, x and `o_t`
+    (named `other`): out may be one of the sources, and nothing else of what is read."""
     cols = shape[-1]
     _check_input(op, "out", out, shape, x.dtype, index)
     try:
@@ -160,6 +161,11 @@ def _out_rows(op: str, out: torch.Tensor, shape, x: torch.Tensor, index: int, so
         raise ValueError(f"{op}: out must have unit inner stride and rows on 8-byte boundaries")
     if _overlap(o, x):
         raise ValueError(f"{op}: out overlaps x")
+    if o_t is not None and o_t.numel() and o.numel():
+        last = sum((d - 1) * st for d, st in zip(o_t.shape, o_t.stride())) + 1
+        end = o.data_ptr() + 2 * ((o.shape[0] - 1) * o.stride(0) + cols)
+        if o_t.data_ptr() < end and o.data_ptr() < o_t.data_ptr() + o_t.element_size() * last:
+            raise ValueError(f"{op}: out overlaps {other}")
     for s in sources:
         if s is not None and _overlap(o, s) and not (
                 s.data_ptr() == o.data_ptr() and s.shape == o.shape and
@@ -247,7 +253,7 @@ def linear(x: torch.Tensor, w: TrellisWeight, bias: torch.Tensor | None = None,
         ldo = n
     else:
         y = out
-        o, ldo = _out_rows("linear", out, shape, xr, index, (mr, rr))
+        o, ldo = _out_rows("linear", out, shape, xr, index, (mr, rr), "bias", bias)
     M = xr.shape[0]
     if M:
         nbytes = _scratch(w._bytes, M, index, lib().exl3b_linear_workspace_bytes, M, k, n)
@@ -334,7 +340,7 @@ def moe(x: torch.Tensor, router: torch.Tensor, experts: TrellisExperts, top_k: i
         ldo = D
     else:
         y = out
-        o, ldo = _out_rows("moe", out, shape, xr, index, (rr,))
+        o, ldo = _out_rows("moe", out, shape, xr, index, (rr,), "router", rt)
     T = xr.shape[0]
     if T:
         most = min(MOE_TOKENS, MOE_PAIRS // top_k)

@@ -514,3 +514,83 @@ def test_block_of_quantized_layers(fw):
     scale = (h.double().abs() @ torch.ones(F, 1, dtype=torch.float64, device="cuda")) / math.sqrt(F)
     assert bool(((y.double() - z.double()).abs()
                  <= 2.0 ** -10 * (z.double().abs() + 4 * scale)).all())
+
+@pytest.mark.parametrize("T,E,top_k", [(64, 4, 2), (64, 16, 2)])
+def test_moe_fp16_keeps_its_precision(fw, oracle, T, E, top_k):
+    """With fp16 tensors the operands of the products hold 22 bits, so that all which
+    is lost is the rounding of the result.  That is uniform within half a step, at most
+    2^-11 of the value: 2^-11 / sqrt(3) of it as a root of mean squares, and 2% more for
+    the operands (2^-22 each), the fp32 sums (2^-20) and the spread of 32768 values."""
+    layer = Layer(oracle, fw, 512, 256, E, [4, 6], seed=40 + E)
+    x, router = rnd((T, 512), torch.float16, 1), rnd((E, 512), torch.float16, 2) / 60
+    want, _ = layer.expect(x, router, top_k)
+    d = f64(fw.moe(x, router, layer.experts, top_k)) - want
+    assert np.sqrt((d ** 2).sum() / (want ** 2).sum()) <= 1.02 * 2.0 ** -11 / math.sqrt(3)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,E,top_k", [(256, 1024, 8), (64, 1024, 32), (256, 9, 8), (255, 3, 3)])
+def test_moe_largest_calls(fw, oracle, T, E, top_k, dtype):
+    """All tokens and choices that one call takes, at the widest tensors, with the
+    experts spread or crowded: every row equals the row computed by itself, and some
+    are checked by value."""
+    layer = Layer(oracle, fw, 256, 128, min(E, 12), [7], seed=50 + E)
+    many = fw.TrellisExperts(*([ws[e % 12] for e in range(E)] for ws in layer.experts.weights))
+    x = rnd((T, 256), dtype, 1)
+    router = rnd((E, 256), torch.float32, 2) / 30
+    got = fw.moe(x, router, many, top_k)
+    for t in (0, 1, T // 2, T - 1):
+        one = fw.moe(x[t:t + 1], router, many, top_k)
+        half = torch.finfo(dtype).eps / 2
+        # the same products in another order of fp32 sums: a step of the result at most
+        assert bool(((one - got[t:t + 1]).abs().double()
+                     <= 2 * half * got[t:t + 1].abs().double() + 2.0 ** -16 * x[t].abs().max().double()).all())
+    if E <= 12:
+        check(got[:8], *layer.expect(x[:8], router, top_k))
+
+
+def test_calls_on_two_streams_at_once(fw, oracle):
+    """Two streams work on the same weights and inputs at the same time, each call with
+    its own workspace; what they give is what one stream gives."""
+    prob = Problem(oracle, 1280, 1024, 4, seed=60)
+    w = prob.weight(fw)
+    layer = Layer(oracle, fw, 512, 256, 6, [4], seed=61)
+    xs = [rnd((M, 1280), torch.bfloat16, M) for M in (1, 6, 40, 300, 1000)]
+    xm, router = rnd((9, 512), torch.bfloat16, 1), rnd((6, 512), torch.bfloat16, 2) / 20
+    calls = [lambda x=x: fw.linear(x, w, activation="silu") for x in xs]
+    calls.append(lambda: fw.moe(xm, router, layer.experts, 2))
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for _ in range(10):
+        for i in range(len(calls)):
+            for s, j in zip(streams, (i, len(calls) - 1 - i)):
+                with torch.cuda.stream(s):
+                    outs.append((j, calls[j]()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[j]) for j, o in outs)
+
+
+def test_first_call_of_a_kernel_may_be_captured(fw, oracle):
+    """No eager call before: what a kernel needs set up once is no work on a stream."""
+    prob = Problem(oracle, 256, 128, 3, "exl3_mcg", seed=70)
+    w = prob.weight(fw)
+    cases = [rnd((M, 256), torch.float16, M) for M in (1, 12, 33, 800)]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = [fw.linear(x, w, activation="gelu") for x in cases]
+    g.replay()
+    for x, o in zip(cases, outs):
+        check(o, *expect(prob, x, act="gelu"))
+
+
+def test_out_must_not_overlap_what_is_read_whole(fw, oracle):
+    prob = Problem(oracle, 128, 128, 4, seed=71)
+    w = prob.weight(fw)
+    buf = torch.zeros(4, 128, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="overlaps bias"):
+        fw.linear(rnd((2, 128), torch.bfloat16, 1), w, bias=buf[1], out=buf[:2])
+    fw.linear(rnd((2, 128), torch.bfloat16, 1), w, bias=buf[0], out=buf[1:3])
+    layer = Layer(oracle, fw, 128, 128, 2, [4], seed=72)
+    with pytest.raises(ValueError, match="overlaps router"):
+        fw.moe(rnd((2, 128), torch.bfloat16, 1), buf[:2], layer.experts, 1, out=buf[1:3])

@@ -5,4 +5,6 @@ Layers:
   ops     torch-tensor wrappers: device pointers + the current CUDA stream
   api     the reference-compatible Python API (quantize_linear, quantize,
           ldlq_viterbi, prepare_incoherence, ...)
+  forward what a layer computes from the finished tensors: linear with its
+          epilogue, mixture-of-experts layers
 """

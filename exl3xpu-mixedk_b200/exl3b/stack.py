@@ -27,6 +27,10 @@ the device as their three stored EXL3 fields and are written to disk by a
 background thread, so the file I/O overlaps the next group's quantization.
 
     torchrun --nproc-per-node 8 -m exl3b.stack --layers 64 --out DIR [--hessians HDIR]
+
+With --probe N every finished tensor is applied to N seeded rows by the forward
+operators, from its stored fields, and compared with the unquantized weight's
+product; the gate, up and down projections also as one block (Probe).
 """
 from __future__ import annotations
 
@@ -112,13 +116,64 @@ def load_hessian(path, dim: int, device):
     return H.to(device=device, dtype=torch.float32)
 
 
+class Probe:
+    """Relative output errors (root of the sums of squares) of one layer's finished
+    tensors on `rows` seeded fp16 rows of normal activations, run from their stored
+    fields as a user of the files would: tensor() of one projection (forward.linear),
+    block() of down(silu(gate x) * up x) once all three are there (forward.moe with
+    one expert).  The unquantized products are fp32."""
+
+    def __init__(self, rows: int, layer: int, device):
+        if rows < 1:
+            raise ValueError(f"{rows} rows to probe with")
+        self.rows, self.layer, self.device = rows, layer, device
+        self.inputs, self.kept = {}, {}
+
+    def x(self, dim: int):
+        import torch
+        if dim not in self.inputs:
+            g = torch.Generator().manual_seed(1000003 * self.layer + dim)
+            self.inputs[dim] = torch.randn(self.rows, dim, generator=g).half().to(self.device)
+        return self.inputs[dim]
+
+    @staticmethod
+    def error(got, want) -> float:
+        d = got.double() - want.double()
+        return float((d.square().sum() / want.double().square().sum()).sqrt())
+
+    def tensor(self, name: str, W, result: dict) -> float:
+        from . import forward
+        w, W = forward.TrellisWeight.from_result(result, self.device), W.float()
+        x = self.x(W.shape[1])
+        want = x.float() @ W.t()
+        if name in ("gate", "up"):
+            self.kept[name] = (w, want)
+        elif name == "down" and len(self.kept) == 2:
+            import torch
+            (gate, g), (up, u) = self.kept.pop("gate"), self.kept.pop("up")
+            self.kept["block"] = ([gate], [up], [w]), (torch.nn.functional.silu(g) * u) @ W.t()
+        return self.error(forward.linear(x, w), want)
+
+    def block(self):
+        """None until gate, up and down have been probed, in this order."""
+        if "block" not in self.kept:
+            return None
+        import torch
+        from . import forward
+        tensors, want = self.kept.pop("block")
+        experts = forward.TrellisExperts(*tensors)
+        router = torch.zeros(1, experts.D, dtype=torch.float16, device=self.device)
+        return self.error(forward.moe(self.x(experts.D), router, experts, 1), want)
+
+
 def quantize_layer(layer: int, device, Ks: dict | None = None, out_root=None,
                    tensors: list | None = None, writer: Writer | None = None,
-                   hessian_dir=None) -> list:
+                   hessian_dir=None, probe: int = 0) -> list:
     """Quantize one layer's tensors on `device`; returns per-tensor stats
     (name, K, weights, Wscale, seconds of quantization, seconds of input
-    synthesis / loading -- each group's time shared by weight).  Writes EXL3
-    files when out_root is given (through `writer` in the background, else
+    synthesis / loading -- each group's time shared by weight; with `probe` rows
+    also "probe_error" and, for down, the gated block's "block_error").  Writes
+    EXL3 files when out_root is given (through `writer` in the background, else
     inline)."""
     import torch
 
@@ -126,6 +181,7 @@ def quantize_layer(layer: int, device, Ks: dict | None = None, out_root=None,
     Ks = dict(synth.SC5_K if Ks is None else Ks)
     stats = []
     s = torch.cuda.current_stream(device)
+    probing = Probe(probe, layer, device) if probe else None
     for group, dim, group_members in synth.STACK_GROUPS:
         members = [m for m in group_members if tensors is None or m in tensors]
         if not members:
@@ -155,6 +211,10 @@ def quantize_layer(layer: int, device, Ks: dict | None = None, out_root=None,
                           "weights": W.numel(), "Wscale": r["Wscale"],
                           "seconds": t_q * W.numel() / tot,
                           "synth_seconds": t_syn * W.numel() / tot})
+            if probing is not None:
+                stats[-1]["probe_error"] = probing.tensor(m, W, r)
+                if m == "down" and (e := probing.block()) is not None:
+                    stats[-1]["block_error"] = e
         del H, Ws, res
     return stats
 
@@ -324,6 +384,18 @@ def quantize_layer_split(layer: int, device, group=None, Ks: dict | None = None,
     return stats
 
 
+def probe_summary(stats: list, rows: int) -> dict:
+    """What main() reports of the probe: the largest output error of any tensor, the
+    mean of them, and the largest of any gated block."""
+    if not rows:
+        return {}
+    e = [s["probe_error"] for s in stats]
+    b = [s["block_error"] for s in stats if "block_error" in s]
+    return {"probe_rows": rows, "probe_error_max": max(e, default=None),
+            "probe_error_mean": sum(e) / len(e) if e else None,
+            "block_error_max": max(b, default=None)}
+
+
 def run_rank(n_layers: int, rank: int, world: int, device, out_root=None,
              quantize=quantize_layer, **kw) -> list:
     """This rank's share of the stack; `quantize(layer, device, ...)` returns
@@ -345,7 +417,12 @@ def main(argv=None) -> int:
     ap.add_argument("--hessians", default=None,
                     help="directory of captured input Grams (L{layer}_{module}.safetensors, "
                          "key H); default: seeded synthetic Hessians")
+    ap.add_argument("--probe", type=int, default=0, metavar="N",
+                    help="apply every finished tensor to N seeded rows and report the output "
+                         "errors (default 0: none)")
     a = ap.parse_args(argv)
+    if a.probe < 0 or (a.probe and a.split_layers):
+        raise SystemExit("--probe takes a number of rows, and whole layers (no --split-layers)")
     import torch
     import torch.distributed as dist
     from datetime import timedelta
@@ -375,7 +452,7 @@ def main(argv=None) -> int:
             st.setdefault("synth_seconds", 0.0)
     else:
         stats = run_rank(a.layers, rank, world, dev, a.out, tensors=tensors, writer=writer,
-                         hessian_dir=a.hessians)
+                         hessian_dir=a.hessians, **({"probe": a.probe} if a.probe else {}))
     if writer is not None:
         writer.close()          # the rank's last files are on disk inside the timing
     ev1.record()
@@ -399,7 +476,8 @@ def main(argv=None) -> int:
                           "seconds_per_layer": float(ms.item()) / 1e3 / max(a.layers, 1),
                           "sharding": "each layer split over all ranks" if a.split_layers
                                       else "whole layers per rank",
-                          "hessians": a.hessians or "synthetic"}))
+                          "hessians": a.hessians or "synthetic",
+                          **probe_summary(stats, a.probe)}))
     return 0
 
 

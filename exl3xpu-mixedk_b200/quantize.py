@@ -1,7 +1,8 @@
 """Drop-in replacement for the reference's ``quantize/quantize.py`` module
 (SergiioB/exl3xpu-mixedk): ``import quantize as xq`` with this directory on
 ``sys.path`` gives the same public API, computed by the B200 CUDA kernels of
-``exl3b`` (see exl3b/api.py)."""
+``exl3b`` (see exl3b/api.py), and beside it the forward operators that apply the
+finished tensors (exl3b/forward.py)."""
 from exl3b.api import (  # noqa: F401
     CODES,
     block_LDL,
@@ -27,4 +28,10 @@ from exl3b.api import (  # noqa: F401
     unpack_states,
     verify_trellis,
     viterbi,
+)
+from exl3b.forward import (  # noqa: F401
+    TrellisExperts,
+    TrellisWeight,
+    linear,
+    moe,
 )

@@ -333,7 +333,11 @@ int exl3b_decode_trellis(const int16_t* dTrellis, int tk, int tn, int K, int cod
  *         multiples of 4); bias, mul and residual may be NULL.  out may be
  *         the same rows as mul or residual, and must not overlap x
  *   act   0 none, 1 relu, 2 silu, 3 gelu (erf), 4 gelu (tanh form)
- * fp32 accumulation; one rounding to dtype at the end.  ws:
+ * x is rotated ((x suh) B) and rounded to fp16 once, each 128 of a row at a power
+ * of two of their own; fp32 accumulation; one rounding to dtype at the end.
+ * From 17 rows on kernels wait for one another's copies, each wait with a limit:
+ * one that runs out (a defect) is told by EXL3B_DEVICE_ERROR from the next call
+ * on the device, since this one has returned by then.  ws:
  * exl3b_linear_workspace_bytes(M, k, n) bytes, 256-byte aligned (NULL when
  * that is 0), in use until the work queued on `stream` has run. */
 size_t exl3b_linear_workspace_bytes(int M, int k, int n);
@@ -363,8 +367,10 @@ typedef struct {
  *   dExperts device table [3][E]: gate [D][F], up [D][F], down [F][D] of every
  *         expert, all of one code; each K in 2..Kmax of its kind
  *   T <= 256, E <= 1024, top_k <= 32, T top_k <= 2048; D and F multiples of 128
- * Logits are summed in fp64, so a token's choice does not depend on the batch;
- * every other sum is fp32 in a fixed order; one rounding to dtype at the end.
+ * Logits are summed in pairs of fp32 in one order whatever the batch, so a token's
+ * choice does not depend on it; every other sum is fp32 in a fixed order.  The
+ * products' operands (x and h = silu * up, rotated) are fp16, with fp16 tensors
+ * and the remainder of that rounding; one rounding to dtype at the end.
  * ws: exl3b_moe_workspace_bytes bytes, 256-byte aligned, in use until the work
  * queued on `stream` has run.  out may be residual's rows; it must not overlap
  * x otherwise. */

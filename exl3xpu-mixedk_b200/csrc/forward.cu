@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(256) linear_rotate_rows_kernel(const LinearArg
 // Sum of a unit's parked sums of one row, output rotation and epilogue: a warp each.
 __global__ void __launch_bounds__(128)
 linear_mid_finish_kernel(const LinearArgs a, const MidArgs w, const FewJoin join, const float* inv) {
-    const int lane = threadIdx.x & 31, nb = blockIdx.x, row = blockIdx.y * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, nb = blockIdx.y, row = blockIdx.x * 4 + (threadIdx.x >> 5);
     if (row >= a.M) return;
     const int col = nb * 128 + 4 * lane, pass = row / w.N, u = pass * w.nbn + nb;
     LinearEpilogue ep;
@@ -383,7 +383,7 @@ static int mid_launch(const LinearArgs& a, DeviceState* st, uint8_t* ws, cudaStr
                        mid_smem(a.K, m.N, m.stages), true, stream, rows, m);
     if (rc) return rc;
     return launch_kernel<linear_mid_finish_kernel>("linear_mid_finish launch",
-                         dim3(m.nbn, (a.M + 3) / 4), 128, 0, true, stream, a, m, FewJoin(m.run),
+                         dim3((a.M + 3) / 4, m.nbn), 128, 0, true, stream, a, m, FewJoin(m.run),
                          (const float*)w.inv);
 }
 
@@ -504,6 +504,13 @@ static int gemm_launch(const LinearArgs& a, DeviceState* st, uint8_t* ws, cudaSt
 }
 
 // ------------------------------------------------------------------ which path
+// Sizes whose tiles, blocks and grids are counted in 32 bits: more than a device holds.
+constexpr int kMostRows = 1 << 24, kMostCols = 1 << 22;
+static bool sizes_fit(int M, int k, int n) {
+    return M <= kMostRows && k <= kMostCols && n <= kMostCols &&
+           (int64_t)M * (k > n ? k : n) <= (int64_t)1 << 38;
+}
+
 constexpr int kFewMost = 16;
 
 // Up to 16 rows mma.sync (one decode serves them); beyond, tensor memory.  There the
@@ -516,6 +523,7 @@ constexpr int kFewMost = 16;
 static bool copy_pays(int M, int k, int n, int sms) {
     const double kb = k >> 7, nb = n >> 7;
     const int N = mid_rows(M), passes = (M + N - 1) / N;
+    if (passes * nb * kb > 1e9) return true;           // blocks are counted in 32 bits
     const double mid = 13.0 + 1.15 * passes * nb * kb / sms * (N > 160 ? N : 160) / 256.0 +
                        3.3e-6 * M * (double)n;
     const int tiles = ((M + kGemmTile - 1) / kGemmTile) * ((n + kGemmTile - 1) / kGemmTile);
@@ -581,7 +589,7 @@ int check_rows(const char* what, const void* p, int64_t ld, int rows, int cols) 
 extern "C" {
 
 size_t exl3b_linear_workspace_bytes(int M, int k, int n) {
-    if (M <= 0 || k <= 0 || n <= 0 || k % 128 || n % 128) return 0;
+    if (M <= 0 || k <= 0 || n <= 0 || k % 128 || n % 128 || !sizes_fit(M, k, n)) return 0;
     const int sms = device_sms();
     if (sms <= 0) return 0;
     return linear_bytes(M, k, n, sms);
@@ -600,6 +608,11 @@ int exl3b_linear(const void* dX, int dtype, int64_t ldx, int M, int k, int n,
     }
     if (M < 0 || k <= 0 || n <= 0 || k % 128 || n % 128) {
         set_error("linear: [%d, %d] x [%d, %d]: in and out must be multiples of 128", M, k, k, n);
+        return RC_BAD_REQUEST;
+    }
+    if (!sizes_fit(M, k, n)) {
+        set_error("linear: [%d, %d] x [%d, %d]: at most %d rows, in and out at most %d, 2^38 elements",
+                  M, k, k, n, kMostRows, kMostCols);
         return RC_BAD_REQUEST;
     }
     if (M == 0) return RC_OK;

@@ -26,6 +26,7 @@ constexpr int kMaxExperts = 1024;
 constexpr int kMaxTokens = 256;
 constexpr int kMaxTopK = 32;
 constexpr int kMaxPairs = 2048;           // (token, choice) pairs of one call
+constexpr int kMaxWidth = 1 << 16;        // D and F: blocks are counted in 32 bits
 
 // What the later kernels need of a chosen expert.
 struct Chosen {
@@ -720,7 +721,8 @@ namespace {
 bool aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
 bool moe_dims(int T, int D, int F, int E, int top_k) {
-    return T >= 0 && T <= kMaxTokens && D > 0 && D % 128 == 0 && F > 0 && F % 128 == 0 && E > 0 &&
+    return T >= 0 && T <= kMaxTokens && D > 0 && D % 128 == 0 && D <= kMaxWidth && F > 0 &&
+           F % 128 == 0 && F <= kMaxWidth && E > 0 &&
            E <= kMaxExperts && top_k > 0 && top_k <= kMaxTopK && top_k <= E && T * top_k <= kMaxPairs;
 }
 
@@ -747,7 +749,7 @@ int exl3b_moe(const void* dX, int dtype, int64_t ldx, int T, int D, int F, int E
         return RC_BAD_REQUEST;
     }
     if (!moe_dims(T, D, F, E, top_k)) {
-        set_error("moe: %d tokens (at most %d), hidden %d and expert width %d (multiples of 128), "
+        set_error("moe: %d tokens (at most %d), hidden %d and expert width %d (multiples of 128, at most 65536), "
                   "%d experts (at most %d), top_k %d (at most %d; tokens x top_k at most %d)", T,
                   kMaxTokens, D, F, E, kMaxExperts, top_k, kMaxTopK, kMaxPairs);
         return RC_BAD_REQUEST;

@@ -327,7 +327,8 @@ int exl3b_decode_trellis(const int16_t* dTrellis, int tk, int tn, int K, int cod
  *   W [k][n] = diag(suh) B W_inner B diag(svh) (from_inner, quantize.py:158-164)
  *         of an EXL3 tensor as stored: dTrellis int16 [k/16][n/16][16 K]
  *         (16-byte aligned), suh fp16 [k] with the tensor's scale folded in
- *         and svh fp16 [n] (8-byte aligned); k and n multiples of 128
+ *         and svh fp16 [n] (8-byte aligned); k and n multiples of 128, at
+ *         most 2^22; M at most 2^24, M k and M n at most 2^38
  *   x [M][k], mul, residual and out [M][n], bias [n]: dtype 1 = bf16 or
  *         2 = fp16, 8-byte aligned, row pitches ld* in elements (>= the row,
  *         multiples of 4); bias, mul and residual may be NULL.  out may be
@@ -366,7 +367,8 @@ typedef struct {
  *         rows; dtype 1 = bf16, 2 = fp16; router_dtype the same, or 0 = fp32
  *   dExperts device table [3][E]: gate [D][F], up [D][F], down [F][D] of every
  *         expert, all of one code; each K in 2..Kmax of its kind
- *   T <= 256, E <= 1024, top_k <= 32, T top_k <= 2048; D and F multiples of 128
+ *   T <= 256, E <= 1024, top_k <= 32, T top_k <= 2048; D and F multiples of 128,
+ *         at most 65536
  * Logits are summed in pairs of fp32 in one order whatever the batch, so a token's
  * choice does not depend on it; every other sum is fp32 in a fixed order.  The
  * products' operands (x and h = silu * up, rotated) are fp16, with fp16 tensors

@@ -31,6 +31,9 @@ def _linear(**kw):
     (dict(ldx=258), 7, "x:"), (dict(out=P + 2), 7, "out:"), (dict(ldo=127), 7, "out:"),
     (dict(mul=P, ldmul=64), 7, "mul:"), (dict(mul=P + 4, ldmul=128), 7, "mul:"),
     (dict(res=P, ldres=130), 7, "residual:"),
+    (dict(M=(1 << 24) + 1), 7, "at most"), (dict(k=(1 << 22) + 128, ldx=1 << 23), 7, "at most"),
+    (dict(n=(1 << 22) + 128, ldo=1 << 23), 7, "at most"),
+    (dict(M=1 << 24, n=1 << 15, ldo=1 << 15), 7, "2^38"),
 ])
 def test_linear_abi_refuses(kw, rc, msg):
     got, text = _linear(**kw)

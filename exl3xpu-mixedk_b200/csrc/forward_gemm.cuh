@@ -7,8 +7,13 @@
 // twice, so that the epilogue of a tile overlaps the next one's MMAs.  In tensor memory
 // a lane is a row, so a thread has all 128 columns of a Hadamard block in registers
 // and no lane needs another's.  Decoding in the product instead (forward_mid.cuh) reads the
-// rows' operand once per 128 columns rather than per 256 and is bound by that: 700 us
-// against 480 at 4096 rows of 5120 x 17408, before the parked sums' way to memory and back.
+// rows' operand once per 128 columns rather than per 256 and is bound by that: 913 us in
+// all against 605 at 4096 rows of 5120 x 17408 without activation.
+//
+// Measured there (K = 5, silu and multiply): 553 to 585 us, the matrix pipe busy 79% of
+// the cycles at 1.41 GHz, to which the power limit takes the clock at once (602 thousand
+// cycles of MMAs); a library GEMM of the same shape, without decode or epilogue, 490.  The
+// time does not depend on a sixth stage (four: 3% more); L2 delivers 13 TB/s.
 #pragma once
 #include "forward_mid.cuh"
 
@@ -26,6 +31,8 @@ constexpr int kGemmThreadsAll = 64 + 32 * kGemmEpilogue;      // loader, MMA, ep
 
 // W_inner^T as fp16 [n][k]; the k of a pair of tiles in few_put_block's order, in which
 // a lane's values of two tiles are 16 bytes of a row.  A warp per tile column and 128 k.
+// 45 us at 5120 x 17408, K = 5, where the bytes read and written take 36; a warp that walks
+// a column with its tiles copied ahead gains nothing.
 template <int K, int CODE>
 __device__ __forceinline__ void expand_block(const uint8_t* src, size_t kt_bytes, __half* out, int k,
                                              int lane) {

@@ -16,6 +16,7 @@ is refused while gradients are enabled.
 from __future__ import annotations
 
 import json
+import operator
 import struct
 from pathlib import Path
 
@@ -60,14 +61,21 @@ class TrellisWeight:
         self.device = trellis.device
         self.index = trellis.device.index       # of the device
         self._bytes = {}                        # rows -> workspace bytes of linear
-        self.trellis = _aligned(trellis.detach(), 16)
-        self.suh = _aligned(suh.detach().half(), 8)
-        self.svh = _aligned(svh.detach().half(), 8)
+        self._fields = (_aligned(trellis.detach(), 16), _aligned(suh.detach().half(), 8),
+                        _aligned(svh.detach().half(), 8))
         # trellis, K, code, suh, svh as the C ABI takes them
         self._args = (self.trellis.data_ptr(), K, self.code_id, self.suh.data_ptr(),
                       self.svh.data_ptr())
         with torch.cuda.device(self.device):
             ops.select_device(self.trellis)
+
+    # fixed, since calls go by their addresses; a copy is made anew
+    trellis = property(lambda self: self._fields[0])
+    suh = property(lambda self: self._fields[1])
+    svh = property(lambda self: self._fields[2])
+
+    def __reduce__(self):
+        return TrellisWeight, (*self._fields, self.K, self.code)
 
     @classmethod
     def from_result(cls, result: dict, device=None) -> "TrellisWeight":
@@ -231,7 +239,7 @@ def linear(x: torch.Tensor, w: TrellisWeight, bias: torch.Tensor | None = None,
     shape = x.shape
     if not shape or shape[-1] != k:
         raise ValueError(f"x {tuple(shape)} for a weight with in = {k}")
-    _no_grad("linear", x, bias, mul, residual)
+    _no_grad("linear", x, bias, mul, residual, out)
     shape = (*shape[:-1], n)
     bias_ptr = mul_ptr = res_ptr = ldm = ldr = 0
     mr = rr = None
@@ -290,13 +298,16 @@ class TrellisExperts:
                     raise ValueError(f"{what} of expert {e} is {w}, expected [{shape[0]}, "
                                      f"{shape[1]}] {first.code} on {first.device}")
         self.device, self.index, self.code_id = first.device, first.index, first.code_id
-        self.weights = (gate, up, down)
+        self.weights = (tuple(gate), tuple(up), tuple(down))
         self._bytes = {}                        # (tokens, top_k) -> workspace bytes of moe
         self.Kmax = tuple(max(w.K for w in ws) for ws in self.weights)
         table = b"".join(struct.pack("<QQQii", w.trellis.data_ptr(), w.suh.data_ptr(),
                                      w.svh.data_ptr(), w.K, 0)
                          for ws in self.weights for w in ws)
         self.table = torch.frombuffer(bytearray(table), dtype=torch.uint8).to(self.device)
+
+    def __reduce__(self):               # the table holds addresses: a copy makes its own
+        return TrellisExperts, self.weights
 
 
 def moe(x: torch.Tensor, router: torch.Tensor, experts: TrellisExperts, top_k: int,
@@ -321,13 +332,13 @@ def moe(x: torch.Tensor, router: torch.Tensor, experts: TrellisExperts, top_k: i
     shape = x.shape
     if not shape or shape[-1] != D:
         raise ValueError(f"x {tuple(shape)} for experts with in = {D}")
-    top_k = int(top_k)
+    top_k = operator.index(top_k)
     if not 1 <= top_k <= min(experts.E, MOE_TOP_K):
         raise ValueError(f"top_k={top_k} with {experts.E} experts (at most {MOE_TOP_K})")
     if router.dtype is not x.dtype and router.dtype is not torch.float32:
         raise ValueError(f"router must be {x.dtype} or float32, got {router.dtype}")
     _check_input("moe", "router", router, (experts.E, D), router.dtype, index)
-    _no_grad("moe", x, router, residual)
+    _no_grad("moe", x, router, residual, out)
     rr, res_ptr, ldr = None, 0, 0
     if residual is not None:
         _check_input("moe", "residual", residual, shape, x.dtype, index)

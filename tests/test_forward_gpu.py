@@ -594,3 +594,34 @@ def test_out_must_not_overlap_what_is_read_whole(fw, oracle):
     layer = Layer(oracle, fw, 128, 128, 2, [4], seed=72)
     with pytest.raises(ValueError, match="overlaps router"):
         fw.moe(rnd((2, 128), torch.bfloat16, 1), buf[:2], layer.experts, 1, out=buf[1:3])
+
+
+def test_copies_of_weights_have_their_own_tensors(fw, oracle):
+    """deepcopy and pickle give weights that no longer need the original's memory."""
+    import copy
+    import gc
+    import pickle
+    prob = Problem(oracle, 256, 128, 4, seed=80)
+    w = prob.weight(fw)
+    layer = Layer(oracle, fw, 128, 128, 3, [4, 5], seed=81)
+    x, xm = rnd((3, 256), torch.bfloat16, 1), rnd((3, 128), torch.bfloat16, 2)
+    router = rnd((3, 128), torch.bfloat16, 3) / 12
+    ref, mref = fw.linear(x, w), fw.moe(xm, router, layer.experts, 2)
+    copies = [copy.deepcopy(w), pickle.loads(pickle.dumps(w))]
+    many = [copy.deepcopy(layer.experts), pickle.loads(pickle.dumps(layer.experts))]
+    old = {w.trellis.data_ptr(), *(e.trellis.data_ptr() for e in layer.experts.weights[0])}
+    for c in copies + [e for m in many for e in m.weights[0]]:
+        assert c.trellis.data_ptr() not in old
+    for t in (w.trellis, *(e.trellis for ws in layer.experts.weights for e in ws)):
+        t.zero_()                       # what a copy must not read
+    del w, layer.experts
+    gc.collect()
+    assert all(torch.equal(fw.linear(x, c), ref) for c in copies)
+    assert all(torch.equal(fw.moe(xm, router, m, 2), mref) for m in many)
+    with pytest.raises(AttributeError):
+        copies[0].trellis = copies[1].trellis
+    with pytest.raises(TypeError):
+        fw.moe(xm, router, many[0], 2.5)
+    o = torch.zeros(3, 128, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    with pytest.raises(ValueError, match="gradient"):
+        fw.linear(x, copies[0], out=o)

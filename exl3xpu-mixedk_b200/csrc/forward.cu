@@ -54,34 +54,40 @@ struct LinearEpilogue {
 
 // ------------------------------------------------------------------ few rows
 struct FewScratch {
-    uint8_t* xh;               // [kb][M][256] rotated rows
+    uint8_t* xh;               // [kb][M][256] rotated rows, and as much for the remainders
     float* inv;                // [kb][M] reciprocal scales
     float* park;
 };
 
-// suh, rotation and rounding of block b of row r.  A warp.
+// suh, rotation and rounding of block b of row r; with LO, which fp16 tensors have, the
+// remainders at dst + lo.  (The rounding of the operand is as large as that of an fp16
+// result: one row with loud channels came out at 0.33e-3 for the 0.21e-3 of the result's
+// rounding alone; eight times finer than that of bf16 it does not show there.)  A warp.
+template <bool LO>
 __device__ __forceinline__ void linear_rotate(const LinearArgs& a, int r, int b, uint8_t* dst,
-                                              float* inv, int swz) {
+                                              float* inv, int swz, size_t lo) {
     const int lane = threadIdx.x & 31, k = b * 128 + 4 * lane;
     float v[4], s[4];
     load4x(a.x, (size_t)r * a.ldx + k, a.dtype, v);
     load4(a.suh + k, s);
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] *= s[j];
-    few_put_block(v, dst, inv, lane, swz);
+    few_put_block<LO>(v, dst, inv, lane, swz, lo);
 }
 
+template <bool LO>
 __global__ void __launch_bounds__(128) linear_rotate_kernel(const LinearArgs a, const FewScratch w) {
     pdl_launch();
     const int i = blockIdx.x * 4 + (threadIdx.x >> 5);
     if (i >= (a.k >> 7) * a.M) return;
-    linear_rotate(a, i % a.M, i / a.M, w.xh + (size_t)i * kRowBytes, w.inv + i, 0);
+    linear_rotate<LO>(a, i % a.M, i / a.M, w.xh + (size_t)i * kRowBytes, w.inv + i, 0,
+                      (size_t)(a.k >> 7) * a.M * kRowBytes);
 }
 
 // Units: (group of 8 G rows, column block).
-template <int G, bool ROTATE>
+template <int G, bool ROTATE, bool LO>
 struct LinearJob {
-    static constexpr bool kRotate = ROTATE, kLo = false;
+    static constexpr bool kRotate = ROTATE, kLo = LO;
     const LinearArgs& a;
     const FewScratch& w;
     const FastDiv& nbn;
@@ -107,18 +113,19 @@ struct LinearJob {
     __device__ __forceinline__ int row_step() const { return a.M; }
     __device__ __forceinline__ const uint8_t* xh() const { return w.xh; }
     __device__ __forceinline__ const float* inv() const { return w.inv; }
+    __device__ __forceinline__ size_t lo() const { return (size_t)(a.k >> 7) * a.M * kRowBytes; }
     __device__ __forceinline__ void wait() const { if (!ROTATE) pdl_wait(); }
     __device__ __forceinline__ void rotate(int r, int b, uint8_t* dst, float* inv, int swz) const {
-        linear_rotate(a, r, b, dst, inv, swz);
+        linear_rotate<LO>(a, r, b, dst, inv, swz, 8 * G * kRowBytes);
     }
 };
 
-template <int CODE, int G, bool ROTATE>
+template <int CODE, int G, bool ROTATE, bool LO>
 __global__ void __launch_bounds__(32 * kFewWarps, 1)
 linear_few_kernel(const LinearArgs a, const FewScratch w, const FewRun run, const FastDiv nbn) {
     extern __shared__ __align__(16) uint8_t sm[];
     pdl_launch();
-    const LinearJob<G, ROTATE> job = {a, w, nbn};
+    const LinearJob<G, ROTATE, LO> job = {a, w, nbn};
     few_run<CODE, G>(job, run, a.K, sm, w.park);
 }
 
@@ -158,12 +165,12 @@ static size_t few_layout(FewScratch* w, int M, int k, int n, int G, int sms, uin
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t o = off; off += up256(bytes); return ws + o; };
     w->park = reinterpret_cast<float*>(take(few_park_bytes(run.units, run.ctas, G)));
-    w->xh = take((size_t)(k >> 7) * M * kRowBytes);
+    w->xh = take((size_t)(k >> 7) * M * 2 * kRowBytes);
     w->inv = reinterpret_cast<float*>(take((size_t)(k >> 7) * M * 4));
     return off;
 }
 
-template <int CODE, int G>
+template <int CODE, int G, bool LO>
 static int few_launch(const LinearArgs& a, int sms, uint8_t* ws, cudaStream_t stream) {
     FewScratch w;
     few_layout(&w, a.M, a.k, a.n, G, sms, ws);
@@ -176,18 +183,18 @@ static int few_launch(const LinearArgs& a, int sms, uint8_t* ws, cudaStream_t st
     if constexpr (G == 1) {
         // one or two rows are rotated where they are used, cheaper than a launch (5120 x
         // 5120, K = 4: 12.2 us against 12.9), if a CTA's share of them fits
-        if (a.M <= 2 && few_smem(a.K, G, most) <= kFewRoom) {
-            rc = launch_kernel<linear_few_kernel<CODE, G, true>>("linear_few launch", dim3(run.ctas),
-                               32 * kFewWarps, few_smem(a.K, G, most), false, stream, a, w, run, nbn);
+        if (a.M <= 2 && few_smem(a.K, G, most, LO) <= kFewRoom) {
+            rc = launch_kernel<linear_few_kernel<CODE, G, true, LO>>("linear_few launch", dim3(run.ctas),
+                               32 * kFewWarps, few_smem(a.K, G, most, LO), false, stream, a, w, run, nbn);
             done = true;
         }
     }
     if (!done) {
-        rc = launch_kernel<linear_rotate_kernel>("linear_rotate launch",
+        rc = launch_kernel<linear_rotate_kernel<LO>>("linear_rotate launch",
                            dim3(((a.k >> 7) * a.M + 3) / 4), 128, 0, false, stream, a, w);
         if (rc) return rc;
-        rc = launch_kernel<linear_few_kernel<CODE, G, false>>("linear_few launch", dim3(run.ctas),
-                           32 * kFewWarps, few_smem(a.K, G, ring), true, stream, a, w, run, nbn);
+        rc = launch_kernel<linear_few_kernel<CODE, G, false, LO>>("linear_few launch", dim3(run.ctas),
+                           32 * kFewWarps, few_smem(a.K, G, ring, LO), true, stream, a, w, run, nbn);
     }
     if (rc) return rc;
     return launch_kernel<linear_finish_kernel<G>>("linear_finish launch", fin, 128, 0, true, stream, a,
@@ -198,7 +205,10 @@ static int few_groups(int M) { return M > 8 ? 2 : 1; }
 
 static int few_dispatch(const LinearArgs& a, int sms, uint8_t* ws, cudaStream_t stream) {
     const int G = few_groups(a.M);
-#define EXL3B_FEW(C) (G == 1 ? few_launch<C, 1>(a, sms, ws, stream) : few_launch<C, 2>(a, sms, ws, stream))
+    const bool lo = a.dtype == X_FP16;
+#define EXL3B_FEW(C) \
+    (G == 1 ? lo ? few_launch<C, 1, true>(a, sms, ws, stream) : few_launch<C, 1, false>(a, sms, ws, stream) \
+            : lo ? few_launch<C, 2, true>(a, sms, ws, stream) : few_launch<C, 2, false>(a, sms, ws, stream))
     switch (a.code) {
         case CODE_MUL1: return EXL3B_FEW(CODE_MUL1);
         case CODE_3INST: return EXL3B_FEW(CODE_3INST);
@@ -211,8 +221,9 @@ static int few_dispatch(const LinearArgs& a, int sms, uint8_t* ws, cudaStream_t 
 // suh, rotation and rounding of whole rows, a CTA each: fp16 [M][k] in the order of k
 // (PAIRED: each 32 k in few_put_block's order, as linear_expand_kernel's), times one power of two a row (its reciprocal in inv [M]), since the matrix unit sums
 // over all of k.  The largest magnitude of the row sets it as in block_scale: entries
-// 2^-25 of it and below lose bits, which is below the rounding of the sum.
-template <bool PAIRED>
+// 2^-25 of it and below lose bits, which is below the rounding of the sum.  With LO the
+// remainders follow as M rows more.
+template <bool PAIRED, bool LO>
 __global__ void __launch_bounds__(256) linear_rotate_rows_kernel(const LinearArgs a, __half* xh, float* inv) {
     __shared__ float part[8];
     constexpr int kHold = 6;                  // blocks a warp keeps in registers; others are read twice
@@ -265,6 +276,11 @@ __global__ void __launch_bounds__(256) linear_rotate_rows_kernel(const LinearArg
             *reinterpret_cast<__half2*>(to + 8) = __floats2half2_rn(v[2], v[3]);
         } else {
             store4(to + 4 * lane, v);
+            if constexpr (LO) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] -= __half2float(__float2half_rn(v[j]));
+                store4(to + (size_t)a.M * a.k + 4 * lane, v);
+            }
         }
     };
 #pragma unroll
@@ -280,7 +296,9 @@ __global__ void __launch_bounds__(256) linear_rotate_rows_kernel(const LinearArg
     }
 }
 
-// Sum of a unit's parked sums of one row, output rotation and epilogue: a warp each.
+// Sum of a unit's parked sums of one row (with LO, and of its remainders' row), output
+// rotation and epilogue: a warp each.
+template <bool LO>
 __global__ void __launch_bounds__(128)
 linear_mid_finish_kernel(const LinearArgs a, const MidArgs w, const FewJoin join, const float* inv) {
     const int lane = threadIdx.x & 31, nb = blockIdx.y, row = blockIdx.x * 4 + (threadIdx.x >> 5);
@@ -292,6 +310,14 @@ linear_mid_finish_kernel(const LinearArgs a, const MidArgs w, const FewJoin join
     pdl_wait();
     float v[4];
     few_sum(w.park, join, parts, u, w.N, row - pass * w.N, lane, 0, 1, v);
+    if constexpr (LO) {
+        const int rest = row + a.M, pass2 = rest / w.N, u2 = pass2 * w.nbn + nb;
+        const FewParts<1> parts2(join, u2);
+        float v2[4];
+        few_sum(w.park, join, parts2, u2, w.N, rest - pass2 * w.N, lane, 0, 1, v2);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += v2[j];
+    }
     const float f = inv[row];
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] *= f;
@@ -332,7 +358,7 @@ static int encode_rows(CUtensorMap* map, const void* base, int k, int rows, int 
 }
 
 struct MidScratch {
-    __half* xh;                // [M][k]
+    __half* xh;                // [M][k], M the rows of the product: with LO twice the call's
     float* inv;                // [M]
     float* park;
 };
@@ -358,31 +384,32 @@ static size_t mid_layout(MidScratch* w, int M, int k, int n, int sms, uint8_t* w
     return off;
 }
 
-template <int CODE>
+template <int CODE, bool LO>
 static int mid_launch(const LinearArgs& a, DeviceState* st, uint8_t* ws, cudaStream_t stream) {
     MidScratch w;
-    mid_layout(&w, a.M, a.k, a.n, st->sms, ws);
+    const int M = LO ? 2 * a.M : a.M;
+    mid_layout(&w, M, a.k, a.n, st->sms, ws);
     MidArgs m;
     m.trellis = a.trellis;
     m.K = a.K;
     m.nbn = a.n >> 7;
-    m.M = a.M;
-    m.N = mid_rows(a.M);
-    m.run = mid_run(a.M, a.k, a.n, st->sms);
+    m.M = M;
+    m.N = mid_rows(M);
+    m.run = mid_run(M, a.k, a.n, st->sms);
     m.park = w.park;
     m.err = st->fwd_err;
     const int fit = (kFewRoom - mid_smem(a.K, m.N, 0)) / (m.N * 256);
     m.stages = fit < 4 ? fit : 4;
     CUtensorMap rows;
-    int rc = encode_rows(&rows, w.xh, a.k, a.M, m.N);
+    int rc = encode_rows(&rows, w.xh, a.k, M, m.N);
     if (rc) return rc;
-    rc = launch_kernel<linear_rotate_rows_kernel<false>>("linear_rotate_rows launch", dim3(a.M), 256, 0, false,
+    rc = launch_kernel<linear_rotate_rows_kernel<false, LO>>("linear_rotate_rows launch", dim3(a.M), 256, 0, false,
                        stream, a, w.xh, w.inv);
     if (rc) return rc;
     rc = launch_kernel<linear_mid_kernel<CODE>>("linear_mid launch", dim3(m.run.ctas), kMidThreads,
                        mid_smem(a.K, m.N, m.stages), true, stream, rows, m);
     if (rc) return rc;
-    return launch_kernel<linear_mid_finish_kernel>("linear_mid_finish launch",
+    return launch_kernel<linear_mid_finish_kernel<LO>>("linear_mid_finish launch",
                          dim3((a.M + 3) / 4, m.nbn), 128, 0, true, stream, a, m, FewJoin(m.run),
                          (const float*)w.inv);
 }
@@ -489,7 +516,7 @@ static int gemm_launch(const LinearArgs& a, DeviceState* st, uint8_t* ws, cudaSt
     int rc = encode_rows(&rows, w.xh, a.k, a.M, 128);
     if (!rc) rc = encode_rows(&cols, w.w, a.k, a.n, 128);
     if (rc) return rc;
-    rc = launch_kernel<linear_rotate_rows_kernel<true>>("linear_rotate_rows launch", dim3(a.M), 256, 0, false,
+    rc = launch_kernel<linear_rotate_rows_kernel<true, false>>("linear_rotate_rows launch", dim3(a.M), 256, 0, false,
                        stream, a, w.xh, w.inv);
     if (rc) return rc;
     rc = launch_kernel<linear_expand_kernel<CODE>>("linear_expand launch", dim3(a.n >> 7, a.k >> 7), 256, 0,
@@ -520,35 +547,45 @@ constexpr int kFewMost = 16;
 // both need.  Measured, decoding against copying (in x out, rows): 5120 x 5120, 512 45 /
 // 52, 1024 79 / 84, 1536 110 / 90; 5120 x 17408, 512 115 / 122, 768 167 / 155, 4096 913 /
 // 605; 17408 x 5120, 1024 203 / 261, 2048 436 / 388; 5120 x 1024, 2048 49 / 55.
-static bool copy_pays(int M, int k, int n, int sms) {
+//
+// With fp16 tensors (`lo`) the first of the two multiplies the remainders of the rows as
+// well, and the GEMM does not: there it would double the time, for an error of the
+// result that is 1.4 to 1.6 times its own rounding's.
+static bool copy_pays(int M, int k, int n, bool lo, int sms) {
     const double kb = k >> 7, nb = n >> 7;
-    const int N = mid_rows(M), passes = (M + N - 1) / N;
+    const int rows = lo ? 2 * M : M, N = mid_rows(rows), passes = (rows + N - 1) / N;
     if (passes * nb * kb > 1e9) return true;           // blocks are counted in 32 bits
     const double mid = 13.0 + 1.15 * passes * nb * kb / sms * (N > 160 ? N : 160) / 256.0 +
-                       3.3e-6 * M * (double)n;
+                       3.3e-6 * rows * (double)n;
     const int tiles = ((M + kGemmTile - 1) / kGemmTile) * ((n + kGemmTile - 1) / kGemmTile);
     const int waves = (tiles + sms / 2 - 1) / (sms / 2);
     const double wave = 0.62 * kb + 2.0;               // at least its epilogue, 11 us
     return 10.0 + 5.2e-7 * k * (double)n + waves * (wave > 11.0 ? wave : 11.0) < mid;
 }
 
+// Of either type of tensors.
 static size_t linear_bytes(int M, int k, int n, int sms) {
     if (M <= kFewMost) {
         FewScratch w;
         return few_layout(&w, M, k, n, few_groups(M), sms, nullptr);
     }
-    if (!copy_pays(M, k, n, sms)) {
+    size_t most = 0;
+    for (int lo = 0; lo < 2; ++lo) {
         MidScratch w;
-        return mid_layout(&w, M, k, n, sms, nullptr);
+        GemmScratch g;
+        const size_t bytes = copy_pays(M, k, n, lo, sms) ? gemm_layout(&g, M, k, n, nullptr)
+                                                         : mid_layout(&w, lo ? 2 * M : M, k, n, sms, nullptr);
+        if (bytes > most) most = bytes;
     }
-    GemmScratch w;
-    return gemm_layout(&w, M, k, n, nullptr);
+    return most;
 }
 
 static int linear_run_all(const LinearArgs& a, DeviceState* st, uint8_t* ws, cudaStream_t stream) {
     if (a.M <= kFewMost) return few_dispatch(a, st->sms, ws, stream);
-    const bool mid = !copy_pays(a.M, a.k, a.n, st->sms);
-#define EXL3B_ROWS(C) (mid ? mid_launch<C>(a, st, ws, stream) : gemm_launch<C>(a, st, ws, stream))
+    const bool lo = a.dtype == X_FP16, mid = !copy_pays(a.M, a.k, a.n, lo, st->sms);
+#define EXL3B_ROWS(C) \
+    (!mid ? gemm_launch<C>(a, st, ws, stream) \
+          : lo ? mid_launch<C, true>(a, st, ws, stream) : mid_launch<C, false>(a, st, ws, stream))
     switch (a.code) {
         case CODE_MUL1: return EXL3B_ROWS(CODE_MUL1);
         case CODE_3INST: return EXL3B_ROWS(CODE_3INST);

@@ -260,7 +260,8 @@ __host__ __device__ inline int few_smem(int Kmax, int G, int blocks, bool lo = f
 //   lo()      with kLo, bytes from a rotated block to its remainders
 //   wait()    -> returns once the rows are there
 // or, with kRotate (every unit has the same rows),
-//   rotate(r, b, dst, inv, swz)   puts block b of row r itself (a warp)
+//   rotate(r, b, dst, inv, swz)   puts block b of row r itself (a warp), with kLo its
+//                                 remainders 8 G rows on
 
 // Multiply this CTA's run and park the sums.  All threads.
 //
@@ -279,7 +280,6 @@ __device__ __forceinline__ void few_run(const Job& job, const FewRun& run, int K
     const int blocks = Job::kRotate ? count : kFewGroups * kRowStages;
     constexpr bool LO = Job::kLo;
     constexpr int kBlockBytes = 8 * G * (LO ? 2 : 1) * kRowBytes;
-    static_assert(!(LO && Job::kRotate), "rows rotated in place have no remainders");
     uint8_t* xh = sm + kFewWarps * few_ring_bytes(Kmax);
     float* inv = reinterpret_cast<float*>(xh + blocks * kBlockBytes);
     const int mine = Job::kRotate ? 0 : grp * kRowStages;      // the group's first row stage
@@ -367,7 +367,7 @@ __device__ __forceinline__ void few_run(const Job& job, const FewRun& run, int K
                         const int rows = job.rows(0), blk = rows == 1 ? j : j >> 1, r = j - blk * rows;
                         int q;
                         const int kblk = run.kb.mod(b0 + blk, q);
-                        job.rotate(r, kblk, xh + (blk * 8 * G + r) * kRowBytes, inv + blk * 8 * G + r,
+                        job.rotate(r, kblk, xh + blk * kBlockBytes + r * kRowBytes, inv + blk * 8 * G + r,
                                    (r & 1) << 6);
                     }
                     __syncthreads();

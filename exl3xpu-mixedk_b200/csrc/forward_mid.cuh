@@ -10,7 +10,7 @@
 // kernel up to some 200 rows.  203 rows of 5120 x 6144 at K = 3: 21.4 us; without the decode
 // 17.1, with one MMA a block of eight 17.1, with neither 14.5, which is the wait for the
 // rows' rotation, their copies and the parking of the sums (37 rows of 6144 x 5120, MCG, K =
-// 6: 18.1, 12.8, 15.9, 9.7).
+// 6, without remainders: 18.1, 12.8, 15.9, 9.7).
 //
 // 18 warps: 16 decode (two groups, blocks in turn; warp w writes the TMEM lanes
 // 32 (w mod 4) .. it may), one issues the MMAs, one loads the rows by TMA.  A group has two A

@@ -334,8 +334,10 @@ int exl3b_decode_trellis(const int16_t* dTrellis, int tk, int tn, int K, int cod
  *         multiples of 4); bias, mul and residual may be NULL.  out may be
  *         the same rows as mul or residual, and must not overlap x
  *   act   0 none, 1 relu, 2 silu, 3 gelu (erf), 4 gelu (tanh form)
- * x is rotated ((x suh) B) and rounded to fp16 once, each 128 of a row at a power
- * of two of their own; fp32 accumulation; one rounding to dtype at the end.
+ * x is rotated ((x suh) B) and rounded to fp16, times a power of two that keeps it
+ * in range; of fp16 tensors the remainder of that rounding is multiplied, too,
+ * except in long prompts (from some 300 to 1000 rows on, where a decoded copy of
+ * the weight pays).  fp32 accumulation; one rounding to dtype at the end.
  * From 17 rows on kernels wait for one another's copies, each wait with a limit:
  * one that runs out (a defect) is told by EXL3B_DEVICE_ERROR from the next call
  * on the device, since this one has returned by then.  ws:

@@ -625,3 +625,19 @@ def test_copies_of_weights_have_their_own_tensors(fw, oracle):
     o = torch.zeros(3, 128, dtype=torch.bfloat16, device="cuda", requires_grad=True)
     with pytest.raises(ValueError, match="gradient"):
         fw.linear(x, copies[0], out=o)
+
+
+@pytest.mark.parametrize("M,k", [(1, 512), (2, 2048), (5, 512), (13, 640), (37, 512), (150, 384), (300, 256)])
+def test_linear_fp16_keeps_its_precision(fw, oracle, M, k):
+    """As test_moe_fp16_keeps_its_precision: the rounding of the result is all there is,
+    with loud channels too, whose blocks round alike in all their places."""
+    prob = Problem(oracle, k, 384, 4, seed=90 + M)
+    w = prob.weight(fw)
+    num = den = 0.0
+    for i in range(1 + 60 // M):
+        x = rnd((M, k), torch.float16, i)
+        x[:, ::128] *= 40.0
+        want = prob.product(f64(x))[0]
+        num += ((f64(fw.linear(x, w)) - want) ** 2).sum()
+        den += (want ** 2).sum()
+    assert np.sqrt(num / den) <= 1.02 * 2.0 ** -11 / math.sqrt(3)

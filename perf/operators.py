@@ -11,7 +11,6 @@ fp32, rounded once) or, where `own` is set, through the package.
 """
 from __future__ import annotations
 
-import functools
 import math
 import os
 import random
@@ -165,7 +164,6 @@ def _activations(g, rows, cols, dt):
     return torch.where(big, x * 12.0, x).to(dt)
 
 
-@functools.lru_cache(maxsize=None)
 def _package():
     path = os.path.join(os.getcwd(), "exl3xpu-mixedk_b200")
     if path not in sys.path:

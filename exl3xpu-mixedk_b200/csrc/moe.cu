@@ -66,6 +66,12 @@ struct MoeArgs {
     float* park;
 };
 
+// The line of p to L2: any address will do (a bulk prefetch would want 16-byte ones,
+// and suh and svh are 8-byte aligned).
+__device__ __forceinline__ void prefetch_line(const void* p) {
+    asm volatile("prefetch.global.L2 [%0];" :: "l"(p));
+}
+
 // ------------------------------------------------------------------ router
 constexpr int kRouterRanks = 4;            // CTAs of a cluster
 constexpr int kRouterWarps = 16;
@@ -220,7 +226,7 @@ moe_router_kernel(const MoeArgs a) {
     constexpr int EE = TT == 1 ? 2 : 1, kWarps = kRouterRanks * kRouterWarps;
     // the experts' table is wanted soon, and has left the cache since the last call
     for (int i = t * 128; i < 3 * a.E * (int)sizeof(exl3b_expert); i += kRouterThreads * 128)
-        asm volatile("prefetch.global.L2 [%0];" :: "l"(reinterpret_cast<const uint8_t*>(a.experts) + i));
+        prefetch_line(reinterpret_cast<const uint8_t*>(a.experts) + i);
     bool wait = true;
     for (int e0 = rank * kRouterWarps + warp; e0 < a.E; e0 += EE * kWarps) {
         const int e1 = e0 + kWarps;
@@ -430,10 +436,6 @@ __device__ __forceinline__ void make_plan(const MoeArgs& a, uint8_t* tmp) {
     }
 }
 
-__device__ __forceinline__ void prefetch_bytes(const void* p, uint32_t bytes) {
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" :: "l"(p), "r"(bytes) : "memory");
-}
-
 // Rotate the tokens for gate and up of every chosen expert (a warp a block); the last
 // CTA makes the plan.  What the joins will want of the experts is brought into L2
 // meanwhile.  (Bringing the tensors, too, delayed the rotation itself: one token 35 -> 43
@@ -458,10 +460,11 @@ moe_rotate_kernel(const MoeArgs a, const FastDiv top_k) {
     load4x(a.x, (size_t)top_k.div(pair) * a.ldx + k, a.dtype, x);
     load4(ch.suh[0] + k, s[0]);
     load4(ch.suh[1] + k, s[1]);
-    if (lane < 4) {            // block b of svh down; the others of F are shared out
-        const __half* v = lane == 0 ? ch.svh[2] : lane == 1 ? ch.svh[0] : lane == 2 ? ch.svh[1] : ch.suh[2];
-        const int n = lane == 0 ? kd : (int)a.kf.d;
-        for (int f = b; f < n; f += kd) prefetch_bytes(v + f * 128, 256);
+    if (lane < 8) {            // block b of svh down; the others of F are shared out; two lanes each
+        const int w = lane >> 1;
+        const __half* v = w == 0 ? ch.svh[2] : w == 1 ? ch.svh[0] : w == 2 ? ch.svh[1] : ch.suh[2];
+        const int n = w == 0 ? kd : (int)a.kf.d;
+        for (int f = b; f < n; f += kd) prefetch_line(v + f * 128 + (lane & 1) * 64);
     }
 #pragma unroll
     for (int m = 0; m < 2; ++m) {

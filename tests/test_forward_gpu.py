@@ -641,3 +641,35 @@ def test_linear_fp16_keeps_its_precision(fw, oracle, M, k):
         num += ((f64(fw.linear(x, w)) - want) ** 2).sum()
         den += (want ** 2).sum()
     assert np.sqrt(num / den) <= 1.02 * 2.0 ** -11 / math.sqrt(3)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_scales_on_8_byte_boundaries(fw, oracle, dtype):
+    """suh and svh may start 4 elements into a buffer, which is what the C header asks
+    of them; such fields are taken as they are and give the same bits."""
+    def shifted(t):
+        v = torch.empty(t.numel() + 8, dtype=t.dtype, device="cuda")
+        at = (8 - v.data_ptr() % 16) // 2 % 8
+        v = v[at:at + t.numel()]
+        v.copy_(t)
+        assert v.data_ptr() % 16 == 8
+        return v
+
+    def move(w):
+        m = fw.TrellisWeight(w.trellis, shifted(w.suh), shifted(w.svh), w.K, w.code)
+        assert m.suh.data_ptr() % 8 == 0 and m.svh.data_ptr() % 8 == 0
+        return m
+
+    layer = Layer(oracle, fw, 384, 256, 5, [3, 5], seed=92)
+    moved = fw.TrellisExperts(*([move(w) for w in ws] for ws in layer.experts.weights))
+    router = rnd((5, 384), dtype, 3) / 20
+    for T in (1, 6, 40):
+        x = rnd((T, 384), dtype, T)
+        got = fw.moe(x, router, moved, 2)
+        assert torch.equal(got, fw.moe(x, router, layer.experts, 2))
+        check(got, *layer.expect(x, router, 2))
+    prob = Problem(oracle, 256, 384, 4, seed=93)
+    w = prob.weight(fw)
+    for M in (1, 12, 40, 2600):
+        x = rnd((M, 256), dtype, M)
+        assert torch.equal(fw.linear(x, move(w)), fw.linear(x, w))

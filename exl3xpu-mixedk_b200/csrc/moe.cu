@@ -343,24 +343,29 @@ __device__ __forceinline__ Plan plan_at(uint8_t* where, int P, int slots_max) {
 
 constexpr int kPlanThreads = 512;
 
-__host__ __device__ inline int plan_scratch(int P, int E) {
-    return up16(P * 4) + up16(E * 8) + (P + 31) / 32 * E;
-}
+// Shared memory of make_plan, each part from a 16-byte boundary to the next.
+struct PlanScratch {
+    int from, before, bytes;   // `where` begins at 0
+    __host__ __device__ PlanScratch(int P, int E)
+        : from(up16(P * 4)), before(from + up16(E * 8)), bytes(before + up16((P + 31) / 32 * E)) {}
+};
 
-// One CTA of kPlanThreads; `tmp`: plan_scratch bytes of shared memory.
+// One CTA of kPlanThreads; `tmp`: PlanScratch::bytes of shared memory.
 template <int G>
 __device__ __forceinline__ void make_plan(const MoeArgs& a, uint8_t* tmp) {
     __shared__ int totals[kPlanThreads / 32];
     constexpr int kWarps = kPlanThreads / 32;
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31, P = a.T * a.top_k, chunks = (P + 31) / 32;
     const Plan p = plan_at(a.plan, P, a.slots_max);
+    const PlanScratch at(P, a.E);
     int* where = reinterpret_cast<int*>(tmp);                   // [P] expert << 8 | place in its chunk
-    int* from = reinterpret_cast<int*>(tmp + up16(P * 4));      // [E] an expert's first pair and slot
+    int* from = reinterpret_cast<int*>(tmp + at.from);          // [E] an expert's first pair and slot
     int* count = from + a.E;                                    // [E] its pairs
-    uint8_t* before = tmp + up16(P * 4) + up16(a.E * 8);        // [chunks][E] then running
+    uint8_t* before = tmp + at.before;                          // [chunks][E] then running
     Chosen own;
     if (t < P) own = a.chosen[t];
-    for (int i = t; i < (chunks * a.E + 3) / 4; i += kPlanThreads) reinterpret_cast<uint32_t*>(before)[i] = 0;
+    for (int i = at.before + 16 * t; i < at.bytes; i += 16 * kPlanThreads)
+        *reinterpret_cast<uint4*>(tmp + i) = make_uint4(0, 0, 0, 0);
     __syncthreads();
     // 32 pairs a warp: how many of the same expert come before a pair there
     for (int c = warp; c < chunks; c += kWarps) {
@@ -697,7 +702,7 @@ static int moe_run(const MoeArgs& a, int sms, cudaStream_t stream) {
     if (rc) return rc;
     constexpr int kWarps = kPlanThreads / 32;
     rc = launch_kernel<moe_rotate_kernel<G, LO>>("moe_rotate launch", dim3((P * kd + kWarps - 1) / kWarps + 1),
-                       kPlanThreads, plan_scratch(P, a.E), true, stream, a, FastDiv(a.top_k));
+                       kPlanThreads, PlanScratch(P, a.E).bytes, true, stream, a, FastDiv(a.top_k));
     if (rc) return rc;
     const int K1 = a.Kmax[0] > a.Kmax[1] ? a.Kmax[0] : a.Kmax[1], plan = plan_bytes(P, a.slots_max);
     const int at1 = up16(few_smem(K1, G, kFewGroups * kRowStages, LO));

@@ -673,3 +673,15 @@ def test_scales_on_8_byte_boundaries(fw, oracle, dtype):
     for M in (1, 12, 40, 2600):
         x = rnd((M, 256), dtype, M)
         assert torch.equal(fw.linear(x, move(w)), fw.linear(x, w))
+
+
+@pytest.mark.parametrize("T,E,top_k", [(1, 5, 3), (1, 6, 6), (1, 7, 1), (9, 11, 4), (40, 13, 7),
+                                       (200, 3, 2)])
+def test_moe_odd_numbers_of_experts(fw, oracle, T, E, top_k):
+    """The plan's byte counts ([choices / 32][experts]) end inside a word of the shared
+    memory that is cleared for them."""
+    assert (T * top_k + 31) // 32 * E % 4
+    layer = Layer(oracle, fw, 128, 128, E, [4], seed=94)
+    x = rnd((T, 128), torch.bfloat16, 1)
+    router = rnd((E, 128), torch.float32, 2) / 12
+    check(fw.moe(x, router, layer.experts, top_k), *layer.expect(x, router, top_k))

@@ -193,8 +193,11 @@ def _call(name: str, index: int, args):
     current in the library (it has its own CUDA runtime) and, where it is not, in torch."""
     f = _functions.get(name)
     if f is None:
+        # before the function: another thread that finds it will look for this, too
+        if "select" not in _functions:
+            _functions["select"] = None if torch.cuda.device_count() == 1 \
+                else lib().exl3b_device_init
         f = _functions[name] = getattr(lib(), name)
-        _functions["select"] = None if torch.cuda.device_count() == 1 else lib().exl3b_device_init
     select = _functions["select"]
     if select is not None:              # with one device it is always the current one
         if torch.cuda.current_device() != index:

@@ -185,3 +185,27 @@ def test_experts_and_moe_refuse():
                           ((x, r.clone().requires_grad_(), ex, 2), {}, "gradient")]:
         with pytest.raises(ValueError, match=msg):
             forward.moe(*args, **kw)
+
+
+def test_first_calls_may_come_from_two_threads(monkeypatch):
+    """A call that begins while another thread's first call is still being prepared."""
+    from types import SimpleNamespace
+
+    from exl3b import forward
+    done = []
+    fake = SimpleNamespace(exl3b_linear=lambda *a: done.append(a) or 0,
+                           exl3b_device_init=lambda index: 0)
+    monkeypatch.setattr(forward, "lib", lambda: fake)
+    monkeypatch.setattr(forward, "_functions", {})
+    monkeypatch.setattr(forward, "_raw_stream", lambda index: 0)
+    first = [True]
+
+    def count():                # the second call comes while the first one asks
+        if first:
+            first.pop()
+            forward._call("exl3b_linear", 0, (2,))
+        return 1
+
+    monkeypatch.setattr(torch.cuda, "device_count", count)
+    forward._call("exl3b_linear", 0, (1,))
+    assert done == [(2, 0), (1, 0)]

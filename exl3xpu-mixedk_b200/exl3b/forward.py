@@ -11,7 +11,8 @@ torch's allocator, so it may be captured into a CUDA graph (make or wrap one
 weight on the device first: that initialises the library there).
 
 Inference only: the weights are integers, and a tensor that requires a gradient
-is refused while gradients are enabled.
+is refused while gradients are enabled, one with a tangent (forward-mode
+differentiation) always.
 """
 from __future__ import annotations
 
@@ -21,6 +22,7 @@ import struct
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 from . import ops
 from .native import check, lib
@@ -55,6 +57,7 @@ class TrellisWeight:
         if tuple(suh.shape) != (k,) or tuple(svh.shape) != (n,):
             raise ValueError(f"suh {tuple(suh.shape)} / svh {tuple(svh.shape)} for a "
                              f"[{k}, {n}] weight")
+        _no_grad("TrellisWeight", suh, svh)
         if not (trellis.is_cuda and suh.device == trellis.device and svh.device == trellis.device):
             raise ValueError("trellis, suh and svh must be on one CUDA device")
         self.k, self.n, self.K, self.code = k, n, K, code
@@ -113,6 +116,10 @@ def _no_grad(op: str, *tensors):
             if t is not None and t.requires_grad:
                 raise ValueError(f"{op} has no gradient: call it under torch.no_grad() or on "
                                  "detached tensors")
+    if forward_ad._current_level >= 0:          # inside a dual_level: no_grad keeps tangents
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{op} has no gradient: a tensor has a tangent")
 
 
 def _check_input(op: str, what: str, t: torch.Tensor, shape, dtype, index: int):

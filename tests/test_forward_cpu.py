@@ -209,3 +209,41 @@ def test_first_calls_may_come_from_two_threads(monkeypatch):
     monkeypatch.setattr(torch.cuda, "device_count", count)
     forward._call("exl3b_linear", 0, (1,))
     assert done == [(2, 0), (1, 0)]
+
+
+def test_tangents_are_refused():
+    """Forward-mode differentiation: a dual tensor does not require a gradient, and its
+    tangent would be lost."""
+    from torch.autograd import forward_ad
+
+    from exl3b import forward
+    w = _Weight()
+    x = torch.zeros(3, 256, dtype=torch.bfloat16)
+    y = torch.zeros(3, 128, dtype=torch.bfloat16)
+    s, tr = torch.ones(128).half(), torch.zeros(8, 8, 64, dtype=torch.int16)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        calls = [lambda: forward.linear(dual(x), w),
+                 lambda: forward.linear(x, w, bias=dual(y[0])),
+                 lambda: forward.linear(x, w, mul=dual(y)),
+                 lambda: forward.linear(x, w, residual=dual(y)),
+                 lambda: forward.linear(x, w, out=dual(y)),
+                 lambda: forward.TrellisWeight(tr, dual(s), s, 4),
+                 lambda: forward.TrellisWeight(tr, s, dual(s), 4)]
+        for call in calls:
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
+                call()
+        with pytest.raises(ValueError, match="in = 256"):       # a plain one goes on
+            forward.linear(x[:, :128], w)
+
+
+def test_fields_that_require_a_gradient_are_refused():
+    from exl3b import forward
+    s, tr = torch.ones(128).half(), torch.zeros(8, 8, 64, dtype=torch.int16)
+    for args in ((tr, s.clone().requires_grad_(), s, 4), (tr, s, s.clone().requires_grad_(), 4)):
+        with pytest.raises(ValueError, match="gradient"):
+            forward.TrellisWeight(*args)
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA device"):
+            forward.TrellisWeight(*args)

@@ -563,6 +563,13 @@ static bool copy_pays(int M, int k, int n, bool lo, int sms) {
     return 10.0 + 5.2e-7 * k * (double)n + waves * (wave > 11.0 ? wave : 11.0) < mid;
 }
 
+// The products, by the numbers of exl3b_linear_product.
+enum Product : int { FEW_ROWS = 1, MID_ROWS = 2, LONG_PROMPT = 3 };
+
+static int product_of(int M, int k, int n, bool lo, int sms) {
+    return M <= kFewMost ? FEW_ROWS : copy_pays(M, k, n, lo, sms) ? LONG_PROMPT : MID_ROWS;
+}
+
 // Of either type of tensors.
 static size_t linear_bytes(int M, int k, int n, int sms) {
     if (M <= kFewMost) {
@@ -573,18 +580,20 @@ static size_t linear_bytes(int M, int k, int n, int sms) {
     for (int lo = 0; lo < 2; ++lo) {
         MidScratch w;
         GemmScratch g;
-        const size_t bytes = copy_pays(M, k, n, lo, sms) ? gemm_layout(&g, M, k, n, nullptr)
-                                                         : mid_layout(&w, lo ? 2 * M : M, k, n, sms, nullptr);
+        const size_t bytes = product_of(M, k, n, lo, sms) == LONG_PROMPT
+                                 ? gemm_layout(&g, M, k, n, nullptr)
+                                 : mid_layout(&w, lo ? 2 * M : M, k, n, sms, nullptr);
         if (bytes > most) most = bytes;
     }
     return most;
 }
 
 static int linear_run_all(const LinearArgs& a, DeviceState* st, uint8_t* ws, cudaStream_t stream) {
-    if (a.M <= kFewMost) return few_dispatch(a, st->sms, ws, stream);
-    const bool lo = a.dtype == X_FP16, mid = !copy_pays(a.M, a.k, a.n, lo, st->sms);
+    const bool lo = a.dtype == X_FP16;
+    const int product = product_of(a.M, a.k, a.n, lo, st->sms);
+    if (product == FEW_ROWS) return few_dispatch(a, st->sms, ws, stream);
 #define EXL3B_ROWS(C) \
-    (!mid ? gemm_launch<C>(a, st, ws, stream) \
+    (product == LONG_PROMPT ? gemm_launch<C>(a, st, ws, stream) \
           : lo ? mid_launch<C, true>(a, st, ws, stream) : mid_launch<C, false>(a, st, ws, stream))
     switch (a.code) {
         case CODE_MUL1: return EXL3B_ROWS(CODE_MUL1);
@@ -630,6 +639,14 @@ size_t exl3b_linear_workspace_bytes(int M, int k, int n) {
     const int sms = device_sms();
     if (sms <= 0) return 0;
     return linear_bytes(M, k, n, sms);
+}
+
+int exl3b_linear_product(int M, int k, int n, int dtype) {
+    if (M <= 0 || k <= 0 || n <= 0 || k % 128 || n % 128 || !sizes_fit(M, k, n) ||
+        (dtype != X_BF16 && dtype != X_FP16))
+        return 0;
+    const int sms = device_sms();
+    return sms > 0 ? product_of(M, k, n, dtype == X_FP16, sms) : 0;
 }
 
 int exl3b_linear(const void* dX, int dtype, int64_t ldx, int M, int k, int n,

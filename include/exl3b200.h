@@ -344,6 +344,10 @@ int exl3b_decode_trellis(const int16_t* dTrellis, int tk, int tn, int K, int cod
  * exl3b_linear_workspace_bytes(M, k, n) bytes, 256-byte aligned (NULL when
  * that is 0), in use until the work queued on `stream` has run. */
 size_t exl3b_linear_workspace_bytes(int M, int k, int n);
+/* Which product exl3b_linear runs for these sizes on the current device: 1 up to 16
+ * rows, 2 the weight decoded as it is multiplied, 3 (long prompts) a decoded fp16
+ * copy of it in the workspace; 0 for arguments that it refuses. */
+int exl3b_linear_product(int M, int k, int n, int dtype);
 int exl3b_linear(const void* dX, int dtype, int64_t ldx, int M, int k, int n,
                  const int16_t* dTrellis, int K, int code, const void* d_suh_f16,
                  const void* d_svh_f16, const void* d_bias, int act,

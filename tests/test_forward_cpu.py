@@ -247,3 +247,12 @@ def test_fields_that_require_a_gradient_are_refused():
             forward.TrellisWeight(*args)
         with torch.no_grad(), pytest.raises(ValueError, match="CUDA device"):
             forward.TrellisWeight(*args)
+
+
+def test_product_of_refused_sizes():
+    from exl3b import native
+    f = native.lib().exl3b_linear_product
+    for args in [(0, 128, 128, 1), (-1, 128, 128, 1), (4, 64, 128, 1), (4, 128, 192, 1),
+                 (4, 128, 128, 0), (4, 128, 128, 3), ((1 << 24) + 1, 128, 128, 1),
+                 (4, (1 << 22) + 128, 128, 2)]:
+        assert f(*args) == 0

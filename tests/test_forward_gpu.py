@@ -685,3 +685,125 @@ def test_moe_odd_numbers_of_experts(fw, oracle, T, E, top_k):
     x = rnd((T, 128), torch.bfloat16, 1)
     router = rnd((E, 128), torch.float32, 2) / 12
     check(fw.moe(x, router, layer.experts, top_k), *layer.expect(x, router, top_k))
+
+
+# ------------------------------------------------------------------ long prompts
+# Rows and sizes at which the decoded copy is multiplied, by a margin of two in the
+# estimates.  5000 x 1280 x 4480: 20 chunks of k pass through the ring of five stages,
+# 20 x 18 tiles of 256 x 256 over the pairs of CTAs give each four or five, and neither
+# the rows nor the columns end on a tile.
+LONG = (5000, 1280, 4480)
+
+
+def product_of(M, k, n, dtype):
+    from exl3b import forward, native
+    return native.lib().exl3b_linear_product(M, k, n, forward.DTYPE_IDS[dtype])
+
+
+def expect_on_gpu(prob, x, bias=None, act=None, mul=None, residual=None):
+    """expect() in fp64 on the device, for many rows"""
+    c = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()
+    d = lambda t: t.double()
+    V, B, suh = c(prob.V), c(_had(1)), c(prob.suh.astype(np.float64))
+    xh = ((d(x) * suh).view(-1, prob.k // 128, 128) @ B).reshape(-1, prob.k)
+    y, tol = xh @ V, ((xh ** 2) @ (V ** 2)).sqrt() * (8 * 2.0 ** -11 / math.sqrt(3)
+                                                     + prob.k / 16 * 2.0 ** -20)
+    if bias is not None:
+        y = y + d(bias)
+    tol = tol + 2.0 ** -20 * y.abs()
+    if act:
+        y, tol = {"silu": lambda t: t * torch.sigmoid(t),
+                  "gelu": torch.nn.functional.gelu}[act](y), tol * 1.13
+    if mul is not None:
+        y, tol = y * d(mul), tol * d(mul).abs()
+    if residual is not None:
+        y = y + d(residual)
+        tol = tol + 2.0 ** -23 * d(residual).abs()
+    half = torch.finfo(x.dtype).eps / 2
+    return y, tol + half * (y.abs() + tol) + torch.finfo(x.dtype).smallest_normal * half
+
+
+def check_on_gpu(got, want, tol):
+    bad = ~((got.double() - want).abs() <= tol)
+    assert not bad.any(), (int(bad.sum()), float(((got.double() - want).abs() / tol).max()),
+                           bad.nonzero()[:4].tolist())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("K,code", [(2, "exl3_mul1"), (3, "exl3_mcg"), (4, "exl3_3inst"),
+                                    (5, "exl3_mul1"), (6, "exl3_mcg"), (7, "exl3_3inst")])
+def test_long_prompt(fw, oracle, K, code, dtype):
+    M, k, n = LONG
+    assert product_of(M, k, n, dtype) == 3
+    prob = Problem(oracle, k, n, K, code, seed=100 + K)
+    w = prob.weight(fw)
+    x, bias = rnd((M, k), dtype, 1), rnd((n,), dtype, 2)
+    x[5] = 0
+    x[300] *= 1e-3
+    mul, res = rnd((M, n), dtype, 3), rnd((M, n), dtype, 4)
+    check_on_gpu(fw.linear(x, w), *expect_on_gpu(prob, x))
+    kw = {"bias": bias, "mul": mul, "residual": res}
+    act = "silu" if K % 2 else "gelu"
+    ref = fw.linear(x, w, activation=act, **kw)
+    check_on_gpu(ref, *expect_on_gpu(prob, x, act=act, **kw))
+    # a column range of a wider buffer, in place on the residual; other columns stay
+    buf = torch.zeros(M, n + 8, dtype=dtype, device="cuda")
+    o = buf[:, 4:-4]
+    o.copy_(res)
+    fw.linear(x, w, bias=bias, activation=act, mul=mul, residual=o, out=o)
+    assert torch.equal(o, ref) and not buf[:, :4].any() and not buf[:, -4:].any()
+    x[9, 3], x[4999, 1000] = float("nan"), float("inf")
+    got = fw.linear(x, w, activation=act, **kw)
+    assert torch.isnan(got[9]).all() and not torch.isfinite(got[4999]).any()
+    keep = torch.ones(M, dtype=torch.bool, device="cuda")
+    keep[[9, 4999]] = False
+    assert torch.equal(got[keep], ref[keep])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_long_prompt_captured_first_then_on_two_streams(fw, oracle, dtype):
+    M, k, n = LONG
+    prob = Problem(oracle, k, n, 4, "exl3_mcg", seed=110)
+    w = prob.weight(fw)
+    xs = [rnd((m, k), dtype, m) for m in (M, M - 300)]
+    assert all(product_of(len(x), k, n, dtype) == 3 for x in xs)
+    outs, graphs = [], []
+    for x in xs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(fw.linear(x, w, activation="silu"))
+        graphs.append(g)
+    for g in graphs:
+        g.replay()
+    for x, o in zip(xs, outs):
+        check_on_gpu(o, *expect_on_gpu(prob, x, act="silu"))
+    want = [o.clone() for o in outs]
+    for x in xs:                         # the graphs read their inputs anew
+        x.copy_(x.flip(0))
+    for g in graphs:
+        g.replay()
+    assert all(torch.equal(o, v.flip(0)) for o, v in zip(outs, want))
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for i in range(6):
+        for s, j in zip(streams, (i % 2, 1 - i % 2)):
+            with torch.cuda.stream(s):
+                got.append((j, fw.linear(xs[j], w, activation="silu")))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, outs[j]) for j, o in got)
+
+
+@pytest.mark.parametrize("M,k,n", [(9000, 256, 4480), (9001, 4992, 1152)])
+def test_long_prompt_other_shapes(fw, oracle, M, k, n):
+    """Fewer chunks than stages; a long k, whose rows are read twice by their rotation."""
+    prob = Problem(oracle, k, n, 5, seed=120)
+    w = prob.weight(fw)
+    for dtype in (torch.bfloat16, torch.float16):
+        assert product_of(M, k, n, dtype) == 3
+        x = rnd((M, k), dtype, 1)
+        check_on_gpu(fw.linear(x, w), *expect_on_gpu(prob, x))
+
+
+def test_products_by_rows(fw):
+    for dtype in (torch.bfloat16, torch.float16):
+        assert [product_of(M, 5120, 5120, dtype) for M in (1, 16, 17, 100, 8192)] == [1, 1, 2, 2, 3]

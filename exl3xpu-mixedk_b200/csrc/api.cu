@@ -36,7 +36,8 @@ int check_cuda(cudaError_t e, const char* what) {
 }
 
 // ---------------------------------------------------------------- wait bound
-// Bound of the LDLQ sweep's device-side waits (ns); exl3b_set_wait_limit_ms.
+// Bound of the device-side waits of the LDLQ sweep and the forward products (ns);
+// exl3b_set_wait_limit_ms.
 static std::atomic<double> g_wait_ns{4.0e9};
 double sweep_wait_ns() { return g_wait_ns.load(std::memory_order_relaxed); }
 

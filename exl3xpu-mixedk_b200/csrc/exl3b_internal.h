@@ -199,7 +199,10 @@ int launch_decode(const int16_t* tr, int tk, int tn, int K, const float* lut, fl
 int launch_verify(const int16_t* tr, int tk, int tn, int K, const float* lut,
                   const float* hatW, int ldw, const int32_t* states, int ld_states, int* bad,
                   cudaStream_t stream);
-// Wait bound (ns) of the sweep's device-side waits (exl3b_set_wait_limit_ms).
+// RC_DEVICE_ERROR, once, after a wait inside a forward kernel ran out (DeviceState::fwd_err).
+int forward_status(DeviceState* st);
+
+// Wait bound (ns) of the sweep's and the forward kernels' waits (exl3b_set_wait_limit_ms).
 double sweep_wait_ns();
 // One-sided block-128 Hadamard (had_left axis 0, had_right axis 1).
 int launch_had_axis(const float* X, int rows, int cols, int axis, float* Y,

@@ -357,6 +357,10 @@ static int encode_rows(CUtensorMap* map, const void* base, int k, int rows, int 
     return RC_OK;
 }
 
+static WaitLimit forward_wait_limit() {
+    return WaitLimit((long long)(sweep_wait_ns() * 2.0));   // at 2 cycles a ns, as the sweep's
+}
+
 struct MidScratch {
     __half* xh;                // [M][k], M the rows of the product: with LO twice the call's
     float* inv;                // [M]
@@ -398,6 +402,7 @@ static int mid_launch(const LinearArgs& a, DeviceState* st, uint8_t* ws, cudaStr
     m.run = mid_run(M, a.k, a.n, st->sms);
     m.park = w.park;
     m.err = st->fwd_err;
+    m.limit = forward_wait_limit();
     const int fit = (kFewRoom - mid_smem(a.K, m.N, 0)) / (m.N * 256);
     m.stages = fit < 4 ? fit : 4;
     CUtensorMap rows;
@@ -523,7 +528,7 @@ static int gemm_launch(const LinearArgs& a, DeviceState* st, uint8_t* ws, cudaSt
                        true, stream, a.trellis, a.K, a.k, a.n, w.w);
     if (rc) return rc;
     const LinearRows e = {a};
-    const GemmArgs g = {a.M, a.k, a.n, w.inv, st->fwd_err};
+    const GemmArgs g = {a.M, a.k, a.n, w.inv, st->fwd_err, forward_wait_limit()};
     const int tiles = ((a.M + kGemmTile - 1) / kGemmTile) * ((a.n + kGemmTile - 1) / kGemmTile);
     const int pairs = tiles < st->sms / 2 ? tiles : st->sms / 2;
     return launch_kernel<linear_gemm_kernel<LinearRows>>("linear_gemm launch", dim3(2 * pairs),
@@ -603,7 +608,7 @@ static int linear_run_all(const LinearArgs& a, DeviceState* st, uint8_t* ws, cud
 #undef EXL3B_ROWS
 }
 
-// A forward kernel's bounded wait ran out in an earlier call.
+// A forward kernel's bounded wait ran out in an earlier call: told once.
 int forward_status(DeviceState* st) {
     volatile int* e = st->fwd_err;
     if (*e == 0) return RC_OK;
@@ -633,6 +638,12 @@ int check_rows(const char* what, const void* p, int64_t ld, int rows, int cols) 
 }  // namespace
 
 extern "C" {
+
+int exl3b_forward_status(void) {
+    DeviceState* st;
+    if (device_state(&st)) { set_error("no usable CUDA device"); return RC_NO_DEVICE; }
+    return forward_status(st);
+}
 
 size_t exl3b_linear_workspace_bytes(int M, int k, int n) {
     if (M <= 0 || k <= 0 || n <= 0 || k % 128 || n % 128 || !sizes_fit(M, k, n)) return 0;

@@ -66,6 +66,7 @@ struct GemmArgs {
     int M, k, n;
     const float* inv;          // [M] reciprocal row scales
     int* err;
+    WaitLimit limit;
 };
 
 // 128-point Hadamard transform of a thread's values, not normalised.
@@ -94,7 +95,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreadsAll, 1)
 linear_gemm_kernel(const __grid_constant__ CUtensorMap rows, const __grid_constant__ CUtensorMap cols,
                    const GemmArgs g, const Epilogue ep) {
     extern __shared__ __align__(1024) uint8_t sm_raw[];
-    __shared__ int fail;
+    __shared__ int fail, peer_fail, sent[2];    // sent: chunks that each CTA has asked for
     __shared__ uint32_t tmem_slot;
     uint8_t* sm = (uint8_t*)(((uintptr_t)sm_raw + 1023) & ~(uintptr_t)1023);
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + kGemmStages * kGemmStage + kGemmEpilogue * kGemmPatch);
@@ -134,7 +135,7 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap rows, const __grid_consta
             int m, n;
             gemm_place(tile, mt, nt, m, n);
             for (int c = 0; c < chunks; ++c) {
-                if (r > 0) ok = bar_wait(empty + 8 * s, (r - 1) & 1, &fail);
+                if (r > 0) ok = bar_wait(empty + 8 * s, (r - 1) & 1, &fail, g.limit);
                 if (!ok) break;
                 const uint32_t dst = shared_addr(sm) + s * kGemmStage, bar = cluster_addr(full + 8 * s, 0);
                 if (rank == 0) bar_expect(full + 8 * s, 2 * kGemmStage);
@@ -145,13 +146,7 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap rows, const __grid_consta
             }
         }
         if (!ok) atomicExch(&fail, 1);
-        // both CTAs' loads land before either's shared memory is released (the pair
-        // meets at the end)
-        if (rank == 0) {
-            const int never = 0;
-            for (int i = max(0, issued - kGemmStages); i < issued; ++i)
-                bar_wait(full + 8 * (i % kGemmStages), (i / kGemmStages) & 1, &never);
-        }
+        cluster_store(cluster_addr(shared_addr(&sent[rank]), 0), issued);
     } else if (t == 32) {
         if (rank == 0) {
             const uint32_t idesc = mma_desc_f16(256, 256);
@@ -159,12 +154,12 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap rows, const __grid_consta
             bool ok = true;
             for (int tile = pair; tile < tiles && ok; tile += pairs, ++lt) {
                 const int acc = lt & 1, use = lt >> 1;
-                if (use > 0) ok = bar_wait(aempty + 8 * acc, (use - 1) & 1, &fail);
+                if (use > 0) ok = bar_wait(aempty + 8 * acc, (use - 1) & 1, &fail, g.limit);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t d = tmem + acc * 256;
                 for (int c = 0; c < chunks; ++c) {
-                    ok = bar_wait(full + 8 * s, r & 1, &fail);
+                    ok = bar_wait(full + 8 * s, r & 1, &fail, g.limit);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t base = shared_addr(sm) + s * kGemmStage;
@@ -184,6 +179,7 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap rows, const __grid_consta
             }
             if (!ok) atomicExch(&fail, 1);
             tc_commit_pair(done);
+            if (!bar_drain(done, 0)) atomicExch(&fail, 1);
         }
     } else if (warp >= 2) {
         // epilogue: lane = row up to the rotation; then, 32 columns at a time through
@@ -201,7 +197,7 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap rows, const __grid_consta
             const int row0 = m * kGemmTile + rank * 128 + 32 * quad, row = row0 + lane;
             const int col = n * kGemmTile + half * 128, have = col < g.n ? min(32, g.M - row0) : 0;
             const float f = row < g.M ? g.inv[row] * kInvSqrt128 : 0.0f;
-            const bool ok = __all_sync(0xffffffffu, bar_wait(afull + 8 * acc, use & 1, &fail));
+            const bool ok = __all_sync(0xffffffffu, bar_wait(afull + 8 * acc, use & 1, &fail, g.limit));
             if (!ok) {
                 if (lane == 0) atomicExch(&fail, 1);
                 break;
@@ -236,14 +232,31 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap rows, const __grid_consta
                 __syncwarp();
             }
         }
+        // the leader's last arrival here, so that none comes after this CTA has ended
+        if (rank == 1 && !bar_drain(done, 0) && lane == 0) atomicExch(&fail, 1);
     }
-    const int never = 0;
-    const bool ok = bar_wait(done, 0, &never);
-    if (__syncthreads_or(!ok || fail)) {
-        if (t == 0) *(volatile int*)g.err = 1;
-    }
+    // Without a failure every load has been multiplied by now.  After one the leader,
+    // at whose barriers both CTAs' loads are counted, sees to it that they have landed
+    // before either's shared memory is released.
+    __syncwarp();
     tc_fence_before();
+    __syncthreads();
+    if (t == 0) cluster_store(cluster_addr(shared_addr(&peer_fail), rank ^ 1), fail);
     cluster_meet();
+    if (fail || peer_fail) {
+        if (t == 0) *(volatile int*)g.err = 1;
+        if (t == 0 && rank == 0) {
+            const int both = min(sent[0], sent[1]), all = max(sent[0], sent[1]);
+            for (int i = max(0, both - kGemmStages); i < all; ++i) {
+                const uint32_t bar = full + 8 * (i % kGemmStages);
+                if (i >= sent[1]) bar_forgo(bar, kGemmStage);       // the other will not ask
+                if (i >= sent[0]) bar_expect(bar, kGemmStage);      // the other has asked ahead
+                bar_drain(bar, (i / kGemmStages) & 1);
+            }
+        }
+        if (t == 0 && rank == 1) bar_drain(done, 0);
+        cluster_meet();
+    }
     if (warp == 1) tc_free_pair(tmem);
 }
 

@@ -34,6 +34,7 @@ struct MidArgs {
     FewRun run;                           // units: (pass, column block)
     float* park;                          // [units + ctas][N][128]
     int* err;
+    WaitLimit limit;
 };
 
 __host__ __device__ inline int mid_smem(int K, int N, int stages) {
@@ -146,7 +147,7 @@ linear_mid_kernel(const __grid_constant__ CUtensorMap rows, const MidArgs a) {
                     const uint32_t to = lanes + kMidA + buf * 64;
                     uint32_t r[16];
                     mid_decode4<K, CODE>(tiles, lw, r);
-                    if (use > 0) ok = bar_wait(aempty + 8 * buf, (use - 1) & 1, &fail);
+                    if (use > 0) ok = bar_wait(aempty + 8 * buf, (use - 1) & 1, &fail, a.limit);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_fence_after();
@@ -162,7 +163,7 @@ linear_mid_kernel(const __grid_constant__ CUtensorMap rows, const MidArgs a) {
                 }
                 if (!ok) break;
                 // the unit's sums: this warp's 32 columns, every fourth group of 32 rows
-                ok = __all_sync(0xffffffffu, bar_wait(dfull, unit & 1, &fail));
+                ok = __all_sync(0xffffffffu, bar_wait(dfull, unit & 1, &fail, a.limit));
                 if (!ok) break;
                 tc_fence_after();
                 const int u = u0 + unit, pass = u / a.nbn;
@@ -194,10 +195,10 @@ linear_mid_kernel(const __grid_constant__ CUtensorMap rows, const MidArgs a) {
             for (int lo = 0; lo < count && ok; ++unit) {
                 const int hi = min(lo + kb - left, count);
                 left = 0;
-                if (unit > 0) ok = bar_wait(dempty, (unit - 1) & 1, &fail);
+                if (unit > 0) ok = bar_wait(dempty, (unit - 1) & 1, &fail, a.limit);
                 for (; i < hi && ok; ++i) {
-                    ok = bar_wait(xfull + 8 * xs_i, xs_n & 1, &fail) &&
-                         bar_wait(afull + 8 * (i & 3), (i >> 2) & 1, &fail);
+                    ok = bar_wait(xfull + 8 * xs_i, xs_n & 1, &fail, a.limit) &&
+                         bar_wait(afull + 8 * (i & 3), (i >> 2) & 1, &fail, a.limit);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t at = tmem + kMidA + (i & 3) * 64, bt = xb + xs_i * a.N * 256;
@@ -220,6 +221,7 @@ linear_mid_kernel(const __grid_constant__ CUtensorMap rows, const MidArgs a) {
             }
             if (!ok) atomicExch(&fail, 1);
             tc_commit(done);                   // tracks every MMA issued
+            if (!bar_drain(done, 0)) atomicExch(&fail, 1);
         }
     } else if (lane == 0) {
         // ------------------------------------------------------------ load rows
@@ -228,7 +230,7 @@ linear_mid_kernel(const __grid_constant__ CUtensorMap rows, const MidArgs a) {
         bool ok = true;
         int b = b0, u = u0, s = 0, n = 0, issued = 0;
         for (int i = 0; i < count; ++i) {
-            if (n > 0) ok = bar_wait(xempty + 8 * s, (n - 1) & 1, &fail);
+            if (n > 0) ok = bar_wait(xempty + 8 * s, (n - 1) & 1, &fail, a.limit);
             if (!ok) break;
             const uint32_t dst = shared_addr(xs) + s * a.N * 256, bar = xfull + 8 * s;
             const int y = u / a.nbn * a.N;
@@ -240,20 +242,14 @@ linear_mid_kernel(const __grid_constant__ CUtensorMap rows, const MidArgs a) {
             if (++s == a.stages) { s = 0; ++n; }
         }
         if (!ok) atomicExch(&fail, 1);
-        {
-            // every issued load lands before the shared memory is released
-            const int never = 0;
-            for (int i = max(0, issued - a.stages); i < issued; ++i)
-                bar_wait(xfull + 8 * (i % a.stages), (i / a.stages) & 1, &never);
-        }
+        // every issued load lands before the shared memory is released
+        for (int i = max(0, issued - a.stages); i < issued; ++i)
+            bar_drain(xfull + 8 * (i % a.stages), (i / a.stages) & 1);
     }
-    const int never = 0;
-    const bool ok = bar_wait(done, 0, &never);
-    if (__syncthreads_or(!ok || fail)) {
-        if (t == 0) *(volatile int*)a.err = 1;
-    }
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
+    if (t == 0 && fail) *(volatile int*)a.err = 1;
     if (warp == kFewWarps)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" :: "r"(tmem) : "memory");
 }

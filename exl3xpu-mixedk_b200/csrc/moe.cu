@@ -787,6 +787,8 @@ int exl3b_moe(const void* dX, int dtype, int64_t ldx, int T, int D, int F, int E
         set_error("moe: workspace %zu < %zu bytes or misaligned", ws_bytes, need);
         return RC_WORKSPACE;
     }
+    const int rc = forward_status(st);
+    if (rc) return rc;
     MoeArgs a;
     memset(&a, 0, sizeof(a));
     a.kd = FastDiv(D / 128);

@@ -1,6 +1,8 @@
 // tc.cuh -- mbarrier, TMA and tcgen05 wrappers of the forward kernels.  Every wait is
-// bounded: it gives up after about two seconds of SM clock, or when another role of
-// the CTA has, and the CTA then drains what it has in flight and ends.
+// bounded.  A wait for another role's handover gives up after the library's wait limit
+// (exl3b_set_wait_limit_ms), or when another role of the CTA has; the CTA then drains
+// what it has in flight, whatever that limit is, and ends.  No wait spans more than one
+// handover or drain, so a long product does not come near the limit.
 #pragma once
 #include <cuda.h>
 #include <stdint.h>
@@ -24,24 +26,40 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
                  :: "r"(bar), "r"(bytes) : "memory");
 }
 
-__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+// The limit of a wait, in SM cycles, and how long one try may sleep, in ns.
+struct WaitLimit {
+    long long cycles;
+    uint32_t sleep;
+    WaitLimit() = default;
+    __host__ __device__ explicit WaitLimit(long long c)
+        : cycles(c), sleep(c < 40000 ? (uint32_t)(c / 2) : 20000u) {}
+};
+
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity, uint32_t sleep) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok) : "r"(bar), "r"(parity), "r"(20000u) : "memory");
+        : "=r"(ok) : "r"(bar), "r"(parity), "r"(sleep) : "memory");
     return ok != 0;
 }
 
-// False when the wait ran out or `fail` (shared memory) is set.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, const int* fail) {
-    if (bar_try(bar, parity)) return true;
+// Wait for a handover; false when the wait ran out or `fail` (shared memory) is set.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, const int* fail,
+                                         const WaitLimit& limit) {
+    if (bar_try(bar, parity, limit.sleep)) return true;
     const long long t0 = clock64();
     for (;;) {
-        if (bar_try(bar, parity)) return true;
-        if (*(const volatile int*)fail || clock64() - t0 > 4000000000LL) return false;
+        if (bar_try(bar, parity, limit.sleep)) return true;
+        if (*(const volatile int*)fail || clock64() - t0 > limit.cycles) return false;
     }
+}
+
+// Wait for what is in flight already (copies, MMAs); false after some two seconds.
+__device__ __forceinline__ bool bar_drain(uint32_t bar, uint32_t parity) {
+    const int never = 0;
+    return bar_wait(bar, parity, &never, WaitLimit(4000000000LL));
 }
 
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
@@ -68,6 +86,12 @@ __device__ __forceinline__ void tc_fence_before() {
 }
 __device__ __forceinline__ void tc_fence_after() {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+
+// Count bytes at a barrier that no copy will bring any more.
+__device__ __forceinline__ void bar_forgo(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;"
+                 :: "r"(bar), "r"(bytes) : "memory");
 }
 
 // Arrive at `bar` when every MMA this thread has issued is done.
@@ -99,6 +123,10 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, int rank) {
     uint32_t r;
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
+}
+
+__device__ __forceinline__ void cluster_store(uint32_t addr, int v) {
+    asm volatile("st.shared::cluster.s32 [%0], %1;" :: "r"(addr), "r"(v) : "memory");
 }
 
 __device__ __forceinline__ void cluster_meet() {

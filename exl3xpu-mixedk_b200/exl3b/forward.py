@@ -226,6 +226,16 @@ def _scratch(cache: dict, key, index: int, size, *args) -> int:
     return nbytes
 
 
+def check_waits(device=None):
+    """Raise if a wait inside a forward kernel that has run on `device` (default: the
+    current one) ran out, which makes its results invalid.  The next linear or moe call
+    there raises it too; work that none follows, a replayed graph's for instance, is
+    asked about here, after synchronising.  Told once."""
+    with torch.cuda.device(device):
+        check("exl3b_device_init", lib().exl3b_device_init(torch.cuda.current_device()))
+        check("exl3b_forward_status", lib().exl3b_forward_status())
+
+
 # ------------------------------------------------------------------ linear
 def linear(x: torch.Tensor, w: TrellisWeight, bias: torch.Tensor | None = None,
            activation: str | None = None, mul: torch.Tensor | None = None,

@@ -72,6 +72,7 @@ SIGNATURES = {
     "exl3b_pack_states": (I, [P, I, I, P, P]),
     "exl3b_unpack_states": (I, [P, I, I, P, P]),
     "exl3b_decode_trellis": (I, [P, I, I, I, I, P, P]),
+    "exl3b_forward_status": (I, []),
     "exl3b_linear_workspace_bytes": (SZ, [I, I, I]),
     "exl3b_linear_product": (I, [I, I, I, I]),
     "exl3b_linear": (I, [P, I, I64, I, I, I, P, I, I, P, P, P, I, P, I64, P, I64, P, I64, P, SZ,

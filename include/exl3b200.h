@@ -79,12 +79,14 @@ int exl3b_profile_end(int kind, double* ms_total, long long* launches, double* u
 int exl3b_device_init(int device);
 
 /* Bound, in milliseconds, of every device-side wait of the LDLQ sweep (a tile
- * waiting for the tile below it in its column, a backpointer-slot claim); 0
- * restores the default of 4000 ms.  A wait that runs out ends its kernel with
- * an error block, and exl3b_ldlq_sweep returns EXL3B_DEVICE_ERROR with the
- * cause in exl3b_last_error(); the context stays usable.  Applies to sweeps
- * started afterwards, in every thread.  No counterpart in the reference (its
- * native encoder has no cross-CTA waits). */
+ * waiting for the tile below it in its column, a backpointer-slot claim) and of
+ * exl3b_linear's products (one role of a kernel waiting for another's piece of
+ * work); 0 restores the default of 4000 ms.  A wait that runs out ends its kernel
+ * with an error: exl3b_ldlq_sweep returns EXL3B_DEVICE_ERROR with the cause in
+ * exl3b_last_error(), exl3b_linear tells it later (exl3b_forward_status); the
+ * context stays usable.  Applies to calls made afterwards, in every thread; a
+ * captured graph keeps the bound it was captured with.  No counterpart in the
+ * reference (its native encoder has no cross-CTA waits). */
 int exl3b_set_wait_limit_ms(double ms);
 
 /* Workspace bytes exl3b_tailbite needs for (nseq, K) on the current device
@@ -322,6 +324,12 @@ int exl3b_decode_trellis(const int16_t* dTrellis, int tk, int tn, int K, int cod
  * inference only (the weights are integers, there is no gradient).
  * =================================================================== */
 
+/* EXL3B_DEVICE_ERROR, once, if a wait of a forward kernel that has run on the
+ * current device ran out (exl3b_set_wait_limit_ms): what these kernels wrote is
+ * not valid.  For work that no later call follows, a replayed graph's for
+ * instance, ask after synchronising. */
+int exl3b_forward_status(void);
+
 /* Linear layer with its epilogue:
  *   out = act(x . W + bias) * mul + residual
  *   W [k][n] = diag(suh) B W_inner B diag(svh) (from_inner, quantize.py:158-164)
@@ -339,8 +347,9 @@ int exl3b_decode_trellis(const int16_t* dTrellis, int tk, int tn, int K, int cod
  * except in long prompts (from some 300 to 1000 rows on, where a decoded copy of
  * the weight pays).  fp32 accumulation; one rounding to dtype at the end.
  * From 17 rows on kernels wait for one another's copies, each wait with a limit:
- * one that runs out (a defect) is told by EXL3B_DEVICE_ERROR from the next call
- * on the device, since this one has returned by then.  ws:
+ * one that runs out (a defect) is told by EXL3B_DEVICE_ERROR from the next
+ * exl3b_linear, exl3b_moe or exl3b_forward_status on the device, since this call
+ * has returned by then.  ws:
  * exl3b_linear_workspace_bytes(M, k, n) bytes, 256-byte aligned (NULL when
  * that is 0), in use until the work queued on `stream` has run. */
 size_t exl3b_linear_workspace_bytes(int M, int k, int n);

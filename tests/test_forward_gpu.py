@@ -807,3 +807,79 @@ def test_long_prompt_other_shapes(fw, oracle, M, k, n):
 def test_products_by_rows(fw):
     for dtype in (torch.bfloat16, torch.float16):
         assert [product_of(M, 5120, 5120, dtype) for M in (1, 16, 17, 100, 8192)] == [1, 1, 2, 2, 3]
+
+
+# ------------------------------------------------------------------ bounded waits
+@pytest.fixture
+def wait_limit():
+    """Sets the limit of device-side waits, in ms; the default returns after the test."""
+    from exl3b import native
+    yield lambda ms: native.call("exl3b_set_wait_limit_ms", float(ms))
+    native.call("exl3b_set_wait_limit_ms", 0.0)
+
+
+@pytest.mark.parametrize("M,k,n,product", [(64, 1280, 512, 2), (*LONG, 3)])
+def test_waits_that_run_out_are_told(fw, oracle, wait_limit, M, k, n, product):
+    """With a limit of a nanosecond the first wait for a piece that is not there yet runs
+    out: the kernel drains what is in flight and ends, the error is told once, and the
+    device goes on working.  Nothing is broken for it; the limit alone is short."""
+    from exl3b.native import Exl3bError
+    prob = Problem(oracle, k, n, 4, seed=130)
+    w = prob.weight(fw)
+    x = rnd((M, k), torch.bfloat16, 1)
+    assert product_of(M, k, n, x.dtype) == product
+    layer = Layer(oracle, fw, 128, 128, 2, [4], seed=131)
+    xm, router = rnd((1, 128), torch.bfloat16, 2), rnd((2, 128), torch.bfloat16, 3)
+    ref, mref = fw.linear(x, w), fw.moe(xm, router, layer.experts, 1)
+    fw.check_waits()
+    told = [lambda: fw.linear(x, w), lambda: fw.moe(xm, router, layer.experts, 1), fw.check_waits]
+    for tell in told:
+        torch.cuda.synchronize()
+        wait_limit(1e-6)
+        fw.linear(x, w)
+        torch.cuda.synchronize()
+        wait_limit(0)
+        with pytest.raises(Exl3bError, match="ran out") as e:
+            tell()
+        assert e.value.rc == 4
+        fw.check_waits()
+        assert torch.equal(fw.linear(x, w), ref)
+        assert torch.equal(fw.moe(xm, router, layer.experts, 1), mref)
+    # a graph keeps the limit that it was captured with, and is asked about afterwards
+    wait_limit(1e-6)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        fw.linear(x, w)
+    wait_limit(0)
+    for _ in range(2):
+        g.replay()
+        torch.cuda.synchronize()
+        with pytest.raises(Exl3bError, match="ran out"):
+            fw.check_waits()
+    assert torch.equal(fw.linear(x, w), ref)
+
+
+@pytest.mark.parametrize("M,k,n,ms,product", [(100, 32768, 131072, 0.15, 2),
+                                              (16384, 8192, 16384, 0.5, 3)])
+def test_products_longer_than_the_limit_of_a_wait(fw, wait_limit, M, k, n, ms, product):
+    """The limit is one of a handover, not of a whole product: ones that run for several
+    times the limit are right (the decoding product some 0.8 ms, the GEMM 3 ms)."""
+    assert product_of(M, k, n, torch.bfloat16) == product
+    g = torch.Generator(device="cuda").manual_seed(1)
+    r = lambda *s: torch.randn(s, generator=g, device="cuda")
+    tr = torch.randint(-32768, 32768, (k // 16, n // 16, 64), generator=g, device="cuda",
+                       dtype=torch.int16)
+    w = fw.TrellisWeight(tr, r(k).half() / math.sqrt(k), r(n).half(), 4)
+    x = r(M, k).bfloat16()
+    ref = fw.linear(x, w)
+    torch.cuda.synchronize()
+    fw.check_waits()
+    wait_limit(ms)
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    a.record()
+    got = fw.linear(x, w)
+    b.record()
+    torch.cuda.synchronize()
+    fw.check_waits()
+    assert a.elapsed_time(b) > 3 * ms
+    assert torch.equal(got, ref)

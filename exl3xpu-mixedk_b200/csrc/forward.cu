@@ -269,18 +269,21 @@ __global__ void __launch_bounds__(256) linear_rotate_rows_kernel(const LinearArg
         for (int j = 0; j < 4; ++j) v[j] *= scale;
         had128_warp(v, lane);
         __half* to = xh + (size_t)row * a.k + b * 128;
-        if (PAIRED) {
-            const int k = 4 * lane;
-            to += (k >> 5) * 32 + ((k & 7) >> 1) * 8 + ((k >> 4) & 1) * 4 + ((k >> 3) & 1) * 2;
-            *reinterpret_cast<__half2*>(to) = __floats2half2_rn(v[0], v[1]);
-            *reinterpret_cast<__half2*>(to + 8) = __floats2half2_rn(v[2], v[3]);
-        } else {
-            store4(to + 4 * lane, v);
-            if constexpr (LO) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] -= __half2float(__float2half_rn(v[j]));
-                store4(to + (size_t)a.M * a.k + 4 * lane, v);
+        auto put = [&](__half* at) {
+            if (PAIRED) {
+                const int k = 4 * lane;
+                at += (k >> 5) * 32 + ((k & 7) >> 1) * 8 + ((k >> 4) & 1) * 4 + ((k >> 3) & 1) * 2;
+                *reinterpret_cast<__half2*>(at) = __floats2half2_rn(v[0], v[1]);
+                *reinterpret_cast<__half2*>(at + 8) = __floats2half2_rn(v[2], v[3]);
+            } else {
+                store4(at + 4 * lane, v);
             }
+        };
+        put(to);
+        if constexpr (LO) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] -= __half2float(__float2half_rn(v[j]));
+            put(to + (size_t)a.M * a.k);
         }
     };
 #pragma unroll
@@ -499,36 +502,36 @@ struct LinearRows {
 };
 
 struct GemmScratch {
-    __half* xh;                // [M][k]
+    __half* xh;                // [M][k], with LO [2 M][k]
     float* inv;                // [M]
     __half* w;                 // [n][k]
 };
 
-static size_t gemm_layout(GemmScratch* w, int M, int k, int n, uint8_t* ws) {
+static size_t gemm_layout(GemmScratch* w, int M, int k, int n, bool lo, uint8_t* ws) {
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t o = off; off += up256(bytes); return ws + o; };
-    w->xh = reinterpret_cast<__half*>(take((size_t)M * k * 2));
+    w->xh = reinterpret_cast<__half*>(take((size_t)M * k * (lo ? 4 : 2)));
     w->inv = reinterpret_cast<float*>(take((size_t)M * 4));
     w->w = reinterpret_cast<__half*>(take((size_t)n * k * 2));
     return off;
 }
 
-template <int CODE>
+template <int CODE, bool LO>
 static int gemm_launch(const LinearArgs& a, DeviceState* st, uint8_t* ws, cudaStream_t stream) {
     GemmScratch w;
-    gemm_layout(&w, a.M, a.k, a.n, ws);
+    gemm_layout(&w, a.M, a.k, a.n, LO, ws);
     CUtensorMap rows, cols;
-    int rc = encode_rows(&rows, w.xh, a.k, a.M, 128);
+    int rc = encode_rows(&rows, w.xh, a.k, LO ? 2 * a.M : a.M, 128);
     if (!rc) rc = encode_rows(&cols, w.w, a.k, a.n, 128);
     if (rc) return rc;
-    rc = launch_kernel<linear_rotate_rows_kernel<true, false>>("linear_rotate_rows launch", dim3(a.M), 256, 0, false,
+    rc = launch_kernel<linear_rotate_rows_kernel<true, LO>>("linear_rotate_rows launch", dim3(a.M), 256, 0, false,
                        stream, a, w.xh, w.inv);
     if (rc) return rc;
     rc = launch_kernel<linear_expand_kernel<CODE>>("linear_expand launch", dim3(a.n >> 7, a.k >> 7), 256, 0,
                        true, stream, a.trellis, a.K, a.k, a.n, w.w);
     if (rc) return rc;
     const LinearRows e = {a};
-    const GemmArgs g = {a.M, a.k, a.n, w.inv, st->fwd_err, forward_wait_limit()};
+    const GemmArgs g = {a.M, a.k, a.n, LO ? 2 : 1, w.inv, st->fwd_err, forward_wait_limit()};
     const int tiles = ((a.M + kGemmTile - 1) / kGemmTile) * ((a.n + kGemmTile - 1) / kGemmTile);
     const int pairs = tiles < st->sms / 2 ? tiles : st->sms / 2;
     return launch_kernel<linear_gemm_kernel<LinearRows>>("linear_gemm launch", dim3(2 * pairs),
@@ -553,9 +556,9 @@ constexpr int kFewMost = 16;
 // 52, 1024 79 / 84, 1536 110 / 90; 5120 x 17408, 512 115 / 122, 768 167 / 155, 4096 913 /
 // 605; 17408 x 5120, 1024 203 / 261, 2048 436 / 388; 5120 x 1024, 2048 49 / 55.
 //
-// With fp16 tensors (`lo`) the first of the two multiplies the remainders of the rows as
-// well, and the GEMM does not: there it would double the time, for an error of the
-// result that is 1.4 to 1.6 times its own rounding's.
+// With fp16 tensors (`lo`) both multiply the remainders of the rows as well, whatever the
+// number of rows: an error must not hang on who shares a batch.  Without them the GEMM
+// would take half the time, for an error of the result of 1.4 to 1.6 times its rounding's.
 static bool copy_pays(int M, int k, int n, bool lo, int sms) {
     const double kb = k >> 7, nb = n >> 7;
     const int rows = lo ? 2 * M : M, N = mid_rows(rows), passes = (rows + N - 1) / N;
@@ -564,7 +567,7 @@ static bool copy_pays(int M, int k, int n, bool lo, int sms) {
                        3.3e-6 * rows * (double)n;
     const int tiles = ((M + kGemmTile - 1) / kGemmTile) * ((n + kGemmTile - 1) / kGemmTile);
     const int waves = (tiles + sms / 2 - 1) / (sms / 2);
-    const double wave = 0.62 * kb + 2.0;               // at least its epilogue, 11 us
+    const double wave = (lo ? 1.24 : 0.62) * kb + 2.0; // at least its epilogue, 11 us
     return 10.0 + 5.2e-7 * k * (double)n + waves * (wave > 11.0 ? wave : 11.0) < mid;
 }
 
@@ -586,7 +589,7 @@ static size_t linear_bytes(int M, int k, int n, int sms) {
         MidScratch w;
         GemmScratch g;
         const size_t bytes = product_of(M, k, n, lo, sms) == LONG_PROMPT
-                                 ? gemm_layout(&g, M, k, n, nullptr)
+                                 ? gemm_layout(&g, M, k, n, lo, nullptr)
                                  : mid_layout(&w, lo ? 2 * M : M, k, n, sms, nullptr);
         if (bytes > most) most = bytes;
     }
@@ -598,7 +601,7 @@ static int linear_run_all(const LinearArgs& a, DeviceState* st, uint8_t* ws, cud
     const int product = product_of(a.M, a.k, a.n, lo, st->sms);
     if (product == FEW_ROWS) return few_dispatch(a, st->sms, ws, stream);
 #define EXL3B_ROWS(C) \
-    (product == LONG_PROMPT ? gemm_launch<C>(a, st, ws, stream) \
+    (product == LONG_PROMPT ? lo ? gemm_launch<C, true>(a, st, ws, stream) : gemm_launch<C, false>(a, st, ws, stream) \
           : lo ? mid_launch<C, true>(a, st, ws, stream) : mid_launch<C, false>(a, st, ws, stream))
     switch (a.code) {
         case CODE_MUL1: return EXL3B_ROWS(CODE_MUL1);

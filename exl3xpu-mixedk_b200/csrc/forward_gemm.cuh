@@ -64,6 +64,7 @@ linear_expand_kernel(const uint8_t* trellis, int K, int k, int n, __half* w) {
 
 struct GemmArgs {
     int M, k, n;
+    int parts;                 // of the rows' values: 2 with the remainders, M rows on
     const float* inv;          // [M] reciprocal row scales
     int* err;
     WaitLimit limit;
@@ -104,7 +105,7 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap rows, const __grid_consta
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
     const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const int mt = (g.M + kGemmTile - 1) / kGemmTile, nt = (g.n + kGemmTile - 1) / kGemmTile;
-    const int tiles = mt * nt, chunks = g.k >> 6;
+    const int tiles = mt * nt, kchunks = g.k >> 6, chunks = g.parts * kchunks;
     if (t == 0) {
         for (int i = 0; i < kGemmStages; ++i) {
             bar_init(full + 8 * i, 1);
@@ -139,8 +140,11 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap rows, const __grid_consta
                 if (!ok) break;
                 const uint32_t dst = shared_addr(sm) + s * kGemmStage, bar = cluster_addr(full + 8 * s, 0);
                 if (rank == 0) bar_expect(full + 8 * s, 2 * kGemmStage);
-                tma_load_pair(dst, &rows, c * 64, m * kGemmTile + rank * 128, bar);
-                tma_load_pair(dst + kGemmBox, &cols, c * 64, n * kGemmTile + rank * 128, bar);
+                // (rows past the last of the values are remainders, or zeros; their sums
+                // are not stored)
+                const int x = c < kchunks ? c : c - kchunks;
+                tma_load_pair(dst, &rows, x * 64, m * kGemmTile + rank * 128 + (x == c ? 0 : g.M), bar);
+                tma_load_pair(dst + kGemmBox, &cols, x * 64, n * kGemmTile + rank * 128, bar);
                 ++issued;
                 if (++s == kGemmStages) { s = 0; ++r; }
             }

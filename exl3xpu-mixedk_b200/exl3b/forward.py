@@ -248,8 +248,8 @@ def linear(x: torch.Tensor, w: TrellisWeight, bias: torch.Tensor | None = None,
     activation: None, "relu", "silu", "gelu" (erf) or "gelu_tanh".  Returns
     [..., n] in x's dtype, or writes `out`, which may be `mul` or `residual`
     themselves.  The sums and the epilogue are fp32, rounded once; x is multiplied as
-    fp16 numbers after its rotation, which bf16 results do not show, and with fp16
-    tensors as pairs of them, except in long prompts (exl3b_linear in the C header)."""
+    fp16 numbers after its rotation, which bf16 results hardly show, and with fp16
+    tensors as pairs of them."""
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation {activation!r}: one of {sorted(map(str, ACTIVATIONS))}")

@@ -343,9 +343,8 @@ int exl3b_forward_status(void);
  *         the same rows as mul or residual, and must not overlap x
  *   act   0 none, 1 relu, 2 silu, 3 gelu (erf), 4 gelu (tanh form)
  * x is rotated ((x suh) B) and rounded to fp16, times a power of two that keeps it
- * in range; of fp16 tensors the remainder of that rounding is multiplied, too,
- * except in long prompts (from some 300 to 1000 rows on, where a decoded copy of
- * the weight pays).  fp32 accumulation; one rounding to dtype at the end.
+ * in range; of fp16 tensors the remainder of that rounding is multiplied, too.
+ * fp32 accumulation; one rounding to dtype at the end.
  * From 17 rows on kernels wait for one another's copies, each wait with a limit:
  * one that runs out (a defect) is told by EXL3B_DEVICE_ERROR from the next
  * exl3b_linear, exl3b_moe or exl3b_forward_status on the device, since this call

@@ -883,3 +883,25 @@ def test_products_longer_than_the_limit_of_a_wait(fw, wait_limit, M, k, n, ms, p
     fw.check_waits()
     assert a.elapsed_time(b) > 3 * ms
     assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("M,k,n", [(160, 2048, 8192), (320, 2560, 2560), (700, 640, 1920), LONG])
+def test_fp16_precision_does_not_hang_on_the_rows(fw, oracle, M, k, n):
+    """From prompts of some hundred rows on, as test_linear_fp16_keeps_its_precision below
+    them: the error is that of rounding the exact values to fp16, and at most 2% more as
+    a root of mean squares (operands of 22 bits and fp32 sums add less than 2^-18 of the
+    magnitudes that are summed, in quadrature)."""
+    rng = np.random.default_rng(140)
+    tr = rng.integers(-32768, 32768, (k // 16, n // 16, 64)).astype(np.int16)
+    suh = (rng.standard_normal(k) / math.sqrt(k)).astype(np.float16)
+    svh = rng.choice([-1.0, 1.0], n).astype(np.float16)
+    c = lambda a: torch.from_numpy(a).cuda()
+    w = fw.TrellisWeight(c(tr), c(suh), c(svh), 4, "exl3_mcg")
+    inner = c(oracle.decode_trellis(tr, oracle.code_lut("exl3_mcg"), 4, k, n)).double()
+    B = c(_had(1))
+    V = (inner.view(k, n // 128, 128) @ B).view(k, n) * c(svh).double()
+    x = rnd((M, k), torch.float16, 1)
+    x[:, ::128] *= 40.0
+    want = ((x.double() * c(suh).double()).view(M, k // 128, 128) @ B).view(M, k) @ V
+    rms = lambda t: float((t.double() - want).square().mean().sqrt())
+    assert rms(fw.linear(x, w)) <= 1.02 * rms(want.half())

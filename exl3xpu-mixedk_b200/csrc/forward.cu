@@ -552,9 +552,15 @@ constexpr int kFewMost = 16;
 // product that decodes as it goes repeats the decode per 256 rows and parks its sums,
 // and the decoded copy costs its way to memory and back but leaves a plain GEMM of whole
 // 256 x 256 tiles.  The estimates are fits in microseconds, without the rotation that
-// both need.  Measured, decoding against copying (in x out, rows): 5120 x 5120, 512 45 /
-// 52, 1024 79 / 84, 1536 110 / 90; 5120 x 17408, 512 115 / 122, 768 167 / 155, 4096 913 /
-// 605; 17408 x 5120, 1024 203 / 261, 2048 436 / 388; 5120 x 1024, 2048 49 / 55.
+// both need, closest where the two are near each other.  Measured in all, decoding /
+// copying (in x out, rows; bf16, K = 4): 5120 x 5120, 512 44 / 52, 768 60 / 57, 1024 77 / 83,
+// 1300 92 / 84; 5120 x 17408, 512 114 / 121, 768 172 / 154, 4096 1044 / 600; 17408 x 5120,
+// 1024 206 / 264, 1300 259 / 271, 2048 448 / 412; 5120 x 1024, 2048 49 / 54, 3000 67 / 60; 2048 x
+// 8192, 400 34 / 32, 512 39 / 33; 640 x 2048, 1024 26 / 23; fp16: 5120 x 17408, 160 97 / 129, 400
+// 175 / 184, 512 213 / 186; 5120 x 5120, 768 98 / 83, 1024 130 / 132.  (It does go to and fro: a row
+// more than 768 is another wave of the GEMM there.)  The slower one is taken, by more than
+// 3%, at 5 of 240 sizes (10 shapes, 96 to 4096 rows, both types; 16% at 640 x 2048 with 1024
+// rows, 7% at most elsewhere) and at 4 of 60 others drawn over all sizes and K (5%).
 //
 // With fp16 tensors (`lo`) both multiply the remainders of the rows as well, whatever the
 // number of rows: an error must not hang on who shares a batch.  Without them the GEMM
@@ -563,12 +569,12 @@ static bool copy_pays(int M, int k, int n, bool lo, int sms) {
     const double kb = k >> 7, nb = n >> 7;
     const int rows = lo ? 2 * M : M, N = mid_rows(rows), passes = (rows + N - 1) / N;
     if (passes * nb * kb > 1e9) return true;           // blocks are counted in 32 bits
-    const double mid = 13.0 + 1.15 * passes * nb * kb / sms * (N > 160 ? N : 160) / 256.0 +
-                       3.3e-6 * rows * (double)n;
+    const double mid = 12.4 + 1.05 * passes * nb * kb / sms * (N > 216 ? N : 216) / 256.0 +
+                       2.65e-6 * rows * (double)n;
     const int tiles = ((M + kGemmTile - 1) / kGemmTile) * ((n + kGemmTile - 1) / kGemmTile);
     const int waves = (tiles + sms / 2 - 1) / (sms / 2);
-    const double wave = (lo ? 1.24 : 0.62) * kb + 2.0; // at least its epilogue, 11 us
-    return 10.0 + 5.2e-7 * k * (double)n + waves * (wave > 11.0 ? wave : 11.0) < mid;
+    const double wave = (lo ? 1.22 : 0.61) * kb + 1.7; // at least its epilogue, 8.4 us
+    return 12.7 + 6.0e-7 * k * (double)n + waves * (wave > 8.4 ? wave : 8.4) < mid;
 }
 
 // The products, by the numbers of exl3b_linear_product.

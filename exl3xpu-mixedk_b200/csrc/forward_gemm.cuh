@@ -7,8 +7,8 @@
 // twice, so that the epilogue of a tile overlaps the next one's MMAs.  In tensor memory
 // a lane is a row, so a thread has all 128 columns of a Hadamard block in registers
 // and no lane needs another's.  Decoding in the product instead (forward_mid.cuh) reads the
-// rows' operand once per 128 columns rather than per 256 and is bound by that: 913 us in
-// all against 605 at 4096 rows of 5120 x 17408 without activation.
+// rows' operand once per 128 columns rather than per 256 and is bound by that: 1044 us in
+// all against 600 at 4096 rows of 5120 x 17408 without activation.
 //
 // Measured there (K = 5, silu and multiply): 553 to 585 us, the matrix pipe busy 79% of
 // the cycles at 1.41 GHz, to which the power limit takes the clock at once (602 thousand

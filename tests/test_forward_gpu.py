@@ -905,3 +905,26 @@ def test_fp16_precision_does_not_hang_on_the_rows(fw, oracle, M, k, n):
     want = ((x.double() * c(suh).double()).view(M, k // 128, 128) @ B).view(M, k) @ V
     rms = lambda t: float((t.double() - want).square().mean().sqrt())
     assert rms(fw.linear(x, w)) <= 1.02 * rms(want.half())
+
+
+@pytest.mark.parametrize("k,n,dtype,decoding,copying", [
+    # rows at which one product took at least 5% less time than the other
+    (5120, 5120, torch.bfloat16, (96, 400, 512, 1024), (768, 1300, 2048, 4096)),
+    (5120, 5120, torch.float16, (256, 400), (768, 1300, 4096)),
+    (5120, 17408, torch.bfloat16, (256, 400, 512), (768, 1024, 4096)),
+    (5120, 17408, torch.float16, (160, 256), (512, 768, 4096)),
+    (17408, 5120, torch.bfloat16, (400, 768, 1024), (1536, 2048, 4096)),
+    (17408, 5120, torch.float16, (400, 512, 1024), (768, 1300, 4096)),
+    (5120, 1024, torch.bfloat16, (1024, 2048), (3000, 4096)),
+    (5120, 1024, torch.float16, (1024, 2048), (3000, 4096)),
+    (2048, 8192, torch.bfloat16, (96, 256), (512, 768, 2048)),
+    (2048, 8192, torch.float16, (160, 256), (400, 512, 1300)),
+    (128, 17408, torch.bfloat16, (96, 160), (512, 1024)),
+    (128, 17408, torch.float16, (64,), (256, 400)),
+    (2048, 768, torch.bfloat16, (512, 2048), (4096,)),
+])
+def test_the_faster_product_is_taken(fw, k, n, dtype, decoding, copying):
+    if torch.cuda.get_device_properties(0).multi_processor_count != 148:
+        pytest.skip("measured on 148 SMs")
+    assert [product_of(M, k, n, dtype) for M in (*decoding, *copying)] \
+        == [2] * len(decoding) + [3] * len(copying)

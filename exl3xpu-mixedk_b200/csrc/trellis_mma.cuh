@@ -24,20 +24,18 @@ namespace exl3b {
 // Values of two states, packed in fp16 (lo: s0).  The formulas are those of
 // build_code_lut; each value is one rounding to fp16 of an exact expression, as
 // the table's.  Integer multiplies, dp4a and packed fp16 share one pipe at half rate,
-// logic, shifts, byte permutes and vabsdiff4 the other: the work is spread over both
-// (mul1, K = 4: 53 cycles a tile and scheduler; both byte sums as dp4a and the pack as
-// a permute 58; byte sums by an 8-bit matrix instruction 60).
+// logic, shifts and byte permutes the other (mul1, K = 4: 54 cycles a tile and scheduler;
+// the sums apart, packed by a permute, 58; one of them by an absolute difference from zero
+// 53, but 1% more in whole products at K = 4; by an 8-bit matrix instruction 60).
 template <int CODE>
 __device__ __forceinline__ uint32_t code_pair(uint32_t s0, uint32_t s1) {
     uint32_t r;
     if constexpr (CODE == CODE_MUL1) {
         // 0x6400 | b is 1024 + b in fp16 for b < 1024: the byte sum (<= 1020) lands
-        // in the mantissa, and one fused multiply-add gives the value
-        const uint32_t h0 = __dp4a(s0 * 0x83DCD12Du, 0x01010101u, 0x6400u);
-        uint32_t h1;
-        asm("vabsdiff4.u32.u32.u32.add %0, %1, %2, %3;"
-            : "=r"(h1) : "r"(s1 * 0x83DCD12Du), "r"(0), "r"(0x6400));
-        const uint32_t p = h1 * 65536u + h0;
+        // in the mantissa, and one fused multiply-add gives the value.  The second sum
+        // is added to the word that holds the first in its upper half.
+        const uint32_t h1 = __dp4a(s1 * 0x83DCD12Du, 0x01010101u, 0x6400u);
+        const uint32_t p = __dp4a(s0 * 0x83DCD12Du, 0x01010101u, h1 * 65536u + 0x6400u);
         asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(p), "r"(0x1EEE1EEEu), "r"(0xC931C931u));
     } else {
         uint32_t x0, x1;
@@ -48,7 +46,8 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t s0, uint32_t s1) {
             x0 = s0 * 0xCBAC1FEDu;
             x1 = s1 * 0xCBAC1FEDu;
         }
-        // (x & m) ^ c as one instruction: 0x6a is (a & b) ^ c
+        // (x & m) ^ c as one instruction (0x6a = 0xf0 & 0xcc ^ 0xaa, by its definition);
+        // left to the compiler it is two: 8 rows of 5120 x 17408, MCG, 29.7 -> 34.1 us
         asm("lop3.b32 %0, %0, %1, %2, 0x6a;" : "+r"(x0) : "r"(0x8FFF8FFFu), "r"(0x3B603B60u));
         asm("lop3.b32 %0, %0, %1, %2, 0x6a;" : "+r"(x1) : "r"(0x8FFF8FFFu), "r"(0x3B603B60u));
         const __half2 y0 = *reinterpret_cast<const __half2*>(&x0);

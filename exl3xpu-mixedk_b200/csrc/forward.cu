@@ -84,32 +84,23 @@ __global__ void __launch_bounds__(128) linear_rotate_kernel(const LinearArgs a, 
                       (size_t)(a.k >> 7) * a.M * kRowBytes);
 }
 
-// Units: (group of 8 G rows, column block).
+// Units: the column blocks; every one has all of the rows, at most 8 G.
 template <int G, bool ROTATE, bool LO>
 struct LinearJob {
     static constexpr bool kRotate = ROTATE, kLo = LO;
     const LinearArgs& a;
     const FewScratch& w;
-    const FastDiv& nbn;
     struct Cursor {
         const uint8_t* tiles;
         uint32_t kt_bytes;
-        int K, left;               // column blocks from here to the last
+        int K;
     };
     __device__ __forceinline__ Cursor cursor(int u) const {
-        int rg;
-        const int nb = nbn.mod(u, rg);
-        return {a.trellis + (size_t)nb * 256 * a.K, nbn.d * 256 * a.K, a.K, (int)nbn.d - nb};
+        return {a.trellis + (size_t)u * 256 * a.K, (uint32_t)(a.n >> 7) * 256 * a.K, a.K};
     }
-    __device__ __forceinline__ void next(Cursor& c) const {
-        c.tiles += 256 * a.K;
-        if (--c.left == 0) {       // the next group of rows
-            c.tiles = a.trellis;
-            c.left = (int)nbn.d;
-        }
-    }
-    __device__ __forceinline__ int rows(int u) const { return min(8 * G, a.M - nbn.div(u) * 8 * G); }
-    __device__ __forceinline__ size_t row(int u, int r) const { return nbn.div(u) * 8 * G + r; }
+    __device__ __forceinline__ void next(Cursor& c) const { c.tiles += 256 * a.K; }
+    __device__ __forceinline__ int rows(int) const { return a.M; }
+    __device__ __forceinline__ size_t row(int, int r) const { return r; }
     __device__ __forceinline__ int row_step() const { return a.M; }
     __device__ __forceinline__ const uint8_t* xh() const { return w.xh; }
     __device__ __forceinline__ const float* inv() const { return w.inv; }
@@ -122,10 +113,10 @@ struct LinearJob {
 
 template <int CODE, int G, bool ROTATE, bool LO>
 __global__ void __launch_bounds__(32 * kFewWarps, 1)
-linear_few_kernel(const LinearArgs a, const FewScratch w, const FewRun run, const FastDiv nbn) {
+linear_few_kernel(const LinearArgs a, const FewScratch w, const FewRun run) {
     extern __shared__ __align__(16) uint8_t sm[];
     pdl_launch();
-    const LinearJob<G, ROTATE, LO> job = {a, w, nbn};
+    const LinearJob<G, ROTATE, LO> job = {a, w};
     few_run<CODE, G>(job, run, a.K, sm, w.park);
 }
 
@@ -139,11 +130,10 @@ linear_finish_kernel(const LinearArgs a, const FewScratch w, const FewJoin join)
     const int nb = blockIdx.x, row = blockIdx.y, col = nb * 128 + 4 * lane;
     LinearEpilogue ep;
     if (warp == 0) ep.load(a, row, col);
-    const int u = row / (8 * G) * gridDim.x + nb;
-    const FewParts<kFewGroups> parts(join, u);
+    const FewParts<kFewGroups> parts(join, nb);
     pdl_wait();
     float v[4];
-    few_sum(w.park, join, parts, u, 8 * G, row % (8 * G), lane, warp, 4, v);
+    few_sum(w.park, join, parts, nb, 8 * G, row, lane, warp, 4, v);
     if (warp) sum[warp - 1][lane] = make_float4(v[0], v[1], v[2], v[3]);
     __syncthreads();
     if (warp) return;
@@ -155,13 +145,11 @@ linear_finish_kernel(const LinearArgs a, const FewScratch w, const FewJoin join)
 
 static size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 
-static FewRun linear_run(int M, int k, int n, int G, int sms) {
-    return FewRun(FastDiv(k >> 7), (n >> 7) * ((M + 8 * G - 1) / (8 * G)), sms);
-}
+static FewRun linear_run(int k, int n, int sms) { return FewRun(FastDiv(k >> 7), n >> 7, sms); }
 
 // Workspace of the few-rows path, laid out at ws.
 static size_t few_layout(FewScratch* w, int M, int k, int n, int G, int sms, uint8_t* ws) {
-    const FewRun run = linear_run(M, k, n, G, sms);
+    const FewRun run = linear_run(k, n, sms);
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t o = off; off += up256(bytes); return ws + o; };
     w->park = reinterpret_cast<float*>(take(few_park_bytes(run.units, run.ctas, G)));
@@ -174,9 +162,8 @@ template <int CODE, int G, bool LO>
 static int few_launch(const LinearArgs& a, int sms, uint8_t* ws, cudaStream_t stream) {
     FewScratch w;
     few_layout(&w, a.M, a.k, a.n, G, sms, ws);
-    const FewRun run = linear_run(a.M, a.k, a.n, G, sms);
+    const FewRun run = linear_run(a.k, a.n, sms);
     const dim3 fin(a.n >> 7, a.M);
-    const FastDiv nbn(a.n >> 7);
     const int most = run.least + (run.longer ? 1 : 0), ring = kFewGroups * kRowStages;
     int rc = RC_OK;
     bool done = false;
@@ -185,7 +172,7 @@ static int few_launch(const LinearArgs& a, int sms, uint8_t* ws, cudaStream_t st
         // 5120, K = 4: 12.2 us against 12.9), if a CTA's share of them fits
         if (a.M <= 2 && few_smem(a.K, G, most, LO) <= kFewRoom) {
             rc = launch_kernel<linear_few_kernel<CODE, G, true, LO>>("linear_few launch", dim3(run.ctas),
-                               32 * kFewWarps, few_smem(a.K, G, most, LO), false, stream, a, w, run, nbn);
+                               32 * kFewWarps, few_smem(a.K, G, most, LO), false, stream, a, w, run);
             done = true;
         }
     }
@@ -194,7 +181,7 @@ static int few_launch(const LinearArgs& a, int sms, uint8_t* ws, cudaStream_t st
                            dim3(((a.k >> 7) * a.M + 3) / 4), 128, 0, false, stream, a, w);
         if (rc) return rc;
         rc = launch_kernel<linear_few_kernel<CODE, G, false, LO>>("linear_few launch", dim3(run.ctas),
-                           32 * kFewWarps, few_smem(a.K, G, ring, LO), true, stream, a, w, run, nbn);
+                           32 * kFewWarps, few_smem(a.K, G, ring, LO), true, stream, a, w, run);
     }
     if (rc) return rc;
     return launch_kernel<linear_finish_kernel<G>>("linear_finish launch", fin, 128, 0, true, stream, a,

@@ -79,10 +79,11 @@ constexpr int kRouterThreads = 32 * kRouterWarps;
 
 // A sum kept as a pair of fp32 (its value and the rounding errors' sum).  The choice of
 // experts must not hang on the batch, so a logit is always summed in the same order,
-// and should hang on rounding as little as it can: eight products at a time are summed
-// in fp32, those sums without loss, which leaves about 2^-28 of the logit.  (fp64
-// additions and conversions run at a 1/64 of the fp32 rate here: 7 us a token; the
-// lossless sum of every product cost 3 us more than this at 64 tokens.)
+// nor on how long a row is: eight products at a time are summed in fp32, those sums
+// without loss.  What is left are the eights' own roundings, as a root of mean squares
+// 2^-26 of the logits' for bf16 tensors and 2^-24.4 for fp16 ones or an fp32 router, at
+// any D.  (fp64 additions and conversions run at a 1/64 of the fp32 rate here: 7 us a
+// token; the lossless sum of every product cost 3 us more than this at 64 tokens.)
 struct PairSum {
     float s = 0.0f, c = 0.0f;
     __device__ __forceinline__ void add(float p) {      // two-sum (Knuth)

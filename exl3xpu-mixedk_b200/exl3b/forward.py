@@ -4,7 +4,9 @@
     moe      a mixture-of-experts layer for a few tokens, its experts EXL3 tensors
 
 The consumer's side of the quantizer: what a layer computes from the fields the
-quantizer stores (trellis, suh, svh), without writing a dense weight.  Weights
+quantizer stores (trellis, suh, svh).  A weight is decoded as it is multiplied;
+only for long prompts is it decoded once into the call's workspace, where the copy
+takes 2 bytes a weight (exl3b_linear_product in the C header tells when).  Weights
 are wrapped once (TrellisWeight); a call takes CUDA tensors, runs on torch's
 current stream of their device and allocates its output and workspace through
 torch's allocator, so it may be captured into a CUDA graph (make or wrap one

@@ -349,7 +349,8 @@ int exl3b_forward_status(void);
  * one that runs out (a defect) is told by EXL3B_DEVICE_ERROR from the next
  * exl3b_linear, exl3b_moe or exl3b_forward_status on the device, since this call
  * has returned by then.  ws:
- * exl3b_linear_workspace_bytes(M, k, n) bytes, 256-byte aligned (NULL when
+ * exl3b_linear_workspace_bytes(M, k, n) bytes (the larger need of the two types; for
+ * long prompts with a decoded copy of the weight, 2 k n), 256-byte aligned (NULL when
  * that is 0), in use until the work queued on `stream` has run. */
 size_t exl3b_linear_workspace_bytes(int M, int k, int n);
 /* Which product exl3b_linear runs for these sizes on the current device: 1 up to 16
